@@ -84,6 +84,32 @@ int b200moe_router(int device, void* stream, int mode, const void* hidden,
                    int E, int K, int normalize, void* logits, void* probs, void* scores,
                    long long* indices, int* counts, int logits_given);
 
+/* Grouped expert selection with a balance bias, on the caller's logits
+ * (beside the selections of b200moe_router, whose scores have neither groups
+ * nor a bias that is left out of the weights). Per token t, with the experts
+ * in n_group groups of S = E / n_group consecutive ids:
+ *   s_e   = 1 / (1 + exp(-l_e))  or  softmax(l)_e       (scoring)
+ *   key_e = s_e + bias_e         (bias NULL: s_e; the bias is used here only)
+ *   the topk_group groups with the largest sum of their best group_top (1 or
+ *   2) keys stay; equal sums: the lower group
+ *   indices[t][k]: the K best keys of those groups in descending order; equal
+ *   keys: the lower expert id
+ *   scores[t][k] = s of indices[t][k], divided by (their sum + 1e-20) when
+ *   normalize, times scale
+ * Selections are those of the formula in 64-bit arithmetic; scores are fp32.
+ * NaN keys and sums rank above every number; an expert whose logit is -inf
+ * has s_e = 0 (softmax of a row of -inf: NaN). logits: fp32 or bf16 rows of
+ * ld_logits elements; bias: fp32 [E] or NULL; counts: int32 [E] or NULL,
+ * zeroed and filled on the stream. E <= 512, n_group <= 32 dividing E,
+ * K <= 32 and at most topk_group * S. */
+#define B200MOE_SCORE_SIGMOID 0
+#define B200MOE_SCORE_SOFTMAX 1
+
+int b200moe_route_grouped(int device, void* stream, const void* logits, int logits_bf16,
+                          long long ld_logits, const float* bias, int T, int E, int K, int n_group,
+                          int topk_group, int group_top, int scoring, int normalize, float scale,
+                          float* scores, long long* indices, int* counts);
+
 /* Compact routing record of one router call (the per-layer capture of
  * moe_serving/record_routing.py:71-77: expert ids as int16, routing weights
  * as fp16): out_indices[i] = (int16) indices[i], out_scores[i] =
@@ -110,6 +136,56 @@ int b200moe_route_record(int device, void* stream, const long long* indices, con
 int b200moe_act_quant_fp8(int device, void* stream, const void* x, long long ldx, const int* map,
                           int map_div, int rows, int k_valid, int k_pad, void* q, float* s,
                           const int* row_offsets, int expert_lo, int expert_hi);
+
+/* Int8 activation quantisation of the int8 experts: per bf16 row r,
+ * s[r] = amax / 127 over its k_valid values (1 where that is zero) and
+ * q[r][c] = x[r][c] / s[r] rounded to nearest even; 0 for k_valid <= c < k_pad.
+ * A row that holds NaN or an infinity gets that as its scale.
+ * inverse (device int32 [rows][copies], the inverse of b200moe_permute) or
+ * NULL: when given, row r is quantised once and written to each of the places
+ * inverse[r][0 .. copies - 1] of the rows_out output rows (places outside
+ * [0, rows_out), such as the -1 of a dropped slot, are skipped); else to r
+ * (copies 1, rows_out >= rows). row_offsets / expert_lo / expert_hi as in
+ * b200moe_act_quant_fp8: only places of the rank's experts are written.
+ * k_valid % 8 == 0, ldx % 8 == 0, k_pad % 16 == 0, k_pad <= 32768, x and q
+ * 16-byte aligned. q: int8 [rows_out][k_pad]; s: fp32 [rows_out]. */
+int b200moe_act_quant_int8(int device, void* stream, const void* x, long long ldx, int rows,
+                           int k_valid, int k_pad, const int* inverse, int copies, int rows_out,
+                           const int* row_offsets, int expert_lo, int expert_hi, void* q, float* s);
+
+/* Rows that are already in 8 bits (a norm's output) to their places in the
+ * permuted order: out[d] = q[r] (row_bytes bytes), out_scale[d][g] =
+ * scale[r][g] for every place d = inverse[r][c] within [0, rows_out) (and,
+ * with row_offsets, of the rank's experts). row_bytes % 16 == 0, 16-byte
+ * aligned; groups >= 1 fp32 scales per row. */
+int b200moe_scatter_rows_8bit(int device, void* stream, const void* q, int row_bytes,
+                              const float* scale, int groups, int rows, const int* inverse,
+                              int copies, int rows_out, const int* row_offsets, int expert_lo,
+                              int expert_hi, void* out, float* out_scale);
+
+/* RMS norm with the residual's addition before it and an 8-bit copy after it
+ * (the post-attention norm in front of the router and the experts): per row,
+ *   h   = bf16(x + residual)    (residual NULL: h = x), stored to residual_out
+ *                               (may be residual itself; NULL: not stored)
+ *   y   = h / sqrt(mean(h^2) + eps) * weight            in fp32
+ *   out = bf16(y)               (out NULL: not stored)
+ *   quant B200MOE_QUANT_FP8:  scale[t][g] = amax / 448 over y's columns
+ *     [128 g, 128 g + 128), q = e4m3(y / scale) (nearest even, saturating):
+ *     the rows and scales of b200moe_w8a8_gemm, from y before its rounding
+ *   quant B200MOE_QUANT_INT8: scale[t] = amax / 127 over the row, q = y / scale
+ *     rounded to nearest even: the rows and scales of b200moe_int8_gemm
+ *   scale 1 where the quotient is zero; q = 0 for H <= c < k_pad.
+ * x, residual, residual_out, out: bf16 rows of ldx, ldr, ldro, ldo elements
+ * (multiples of 8, 16-byte aligned); weight: bf16 or fp32 [H]; H % 8 == 0,
+ * H <= 32768; k_pad % 16 == 0, H <= k_pad <= 32768. */
+#define B200MOE_QUANT_NONE 0
+#define B200MOE_QUANT_FP8 1
+#define B200MOE_QUANT_INT8 2
+
+int b200moe_add_rmsnorm(int device, void* stream, const void* x, long long ldx,
+                        const void* residual, long long ldr, void* residual_out, long long ldro,
+                        const void* weight, int weight_f32, float eps, int T, int H, void* out,
+                        long long ldo, int quant, void* q, int k_pad, float* scale);
 
 /* ------------------------------------------------------------ permutation
  * Expert-contiguous permutation of the T*K (token, slot) assignments.
@@ -205,6 +281,7 @@ int b200moe_permute_noalloc(int device, void* stream, const long long* indices, 
 #define B200MOE_W_BF16 0
 #define B200MOE_W_FP8 1
 #define B200MOE_W_MXFP4 2
+#define B200MOE_W_INT8 3      /* b200moe_int8_gemm only */
 
 #define B200MOE_EPI_SWIGLU 0
 #define B200MOE_EPI_CLAMP_SWIGLU 1
@@ -218,6 +295,11 @@ int b200moe_permute_noalloc(int device, void* stream, const long long* indices, 
  * rounding, no row weight; ldo in floats, a multiple of 4). */
 #define B200MOE_EPI_CLAMP_SWIGLU_F32 3
 #define B200MOE_EPI_DOWN_F32 4
+/* The epilogues of b200moe_int8_gemm besides CLAMP_SWIGLU_F32, fp32 throughout
+ * with one rounding: SWIGLU_F32 (gated) out = bf16(g / (1 + exp(-g)) * u) with
+ * g and u the biased sums; DOWN_ONCE out = bf16((D + bias) * row weight). */
+#define B200MOE_EPI_SWIGLU_F32 5
+#define B200MOE_EPI_DOWN_ONCE 6
 
 typedef struct b200moe_gemm_args {
   /* rows */
@@ -278,6 +360,28 @@ size_t b200moe_gemm_args_size(void);
  * bias must be NULL / unused; token_tile is 0 (choose) or 16, 32, 64, 128. */
 int b200moe_w8a8_gemm(int device, void* stream, const b200moe_gemm_args* args, const void* q,
                       const float* q_scale);
+
+/* Int8 grouped GEMM (dense with one expert and offsets NULL: all max_rows
+ * rows are its own): int8 rows with one scale each
+ * times int8 weights with one scale per output channel. For weight row f and
+ * permuted row n, the inner sum exact in int32:
+ *   D[n, f] = q_scale[n] * w_scale[f] * sum_k W[f, k] * q[n, k]  (+ bias[f])
+ * planes = 2: gated, EPI_SWIGLU_F32 or EPI_CLAMP_SWIGLU_F32; planes = 1:
+ * EPI_DOWN_ONCE, with the row's routing weight when row_weight is given.
+ * weight: [n_experts][feature tiles][k_pad / 128] images of 128 rows x 128
+ * int8, the 16-byte chunk c of row r stored at chunk position c ^ (r & 7).
+ * A feature tile of one plane is 128 features; a gated tile has 64 features,
+ * rows 32 j + 0..15 the gate rows and 32 j + 16..31 the up rows of features
+ * 16 j .. 16 j + 15. w_scale and bias (fp32, bias may be NULL):
+ * [n_experts][feature tiles][128] in the same row order. q: int8
+ * [b_rows][k_pad] in permuted row order (b200moe_act_quant_int8), q_scale:
+ * fp32 [b_rows]. wfmt = B200MOE_W_INT8; k_pad % 128 == 0, k_pad < 131072 (the
+ * int32 sum cannot overflow); b_src, ldb, k_valid, b_map, b_div, sc_br, sc_bc
+ * and the args' bias are unused (b_map and bias NULL). token_tile is 0
+ * (choose) or 16, 32, 64, 128, 256. Rows past the last expert's are not
+ * written. */
+int b200moe_int8_gemm(int device, void* stream, const b200moe_gemm_args* args, const void* q,
+                      const float* q_scale, const float* w_scale, const float* bias);
 
 /* ------------------------------------------------------------ combine
  * out[t, :] = ordered bf16 sum over the slots k of token t of the

@@ -19,8 +19,11 @@ OK, ERR_INVALID, ERR_UNSUPPORTED, ERR_CUDA = 0, 1, 2, 3
 STATUS_WAIT_TIMEOUT, STATUS_BAD_TILE, STATUS_BAD_INDEX, STATUS_PEER_TIMEOUT = 1, 2, 4, 8
 
 ROUTER_QWEN3, ROUTER_GPT_OSS, ROUTER_NATIVE = 0, 1, 2
-W_BF16, W_FP8, W_MXFP4 = 0, 1, 2
+W_BF16, W_FP8, W_MXFP4, W_INT8 = 0, 1, 2, 3
 EPI_SWIGLU, EPI_CLAMP_SWIGLU, EPI_DOWN, EPI_CLAMP_SWIGLU_F32, EPI_DOWN_F32 = 0, 1, 2, 3, 4
+EPI_SWIGLU_F32, EPI_DOWN_ONCE = 5, 6
+SCORE_SIGMOID, SCORE_SOFTMAX = 0, 1
+QUANT_NONE, QUANT_FP8, QUANT_INT8 = 0, 1, 2
 ORDER_EXPERT, ORDER_RANK_SLOT, ORDER_SLOT_SUM = 0, 1, 2
 PERMUTE_SCRATCH_BYTES = 1 << 20
 
@@ -29,13 +32,18 @@ EXPORTED = (
     "b200moe_version",
     "b200moe_device_status",
     "b200moe_router",
+    "b200moe_route_grouped",
     "b200moe_route_record",
     "b200moe_act_quant_fp8",
+    "b200moe_act_quant_int8",
+    "b200moe_scatter_rows_8bit",
+    "b200moe_add_rmsnorm",
     "b200moe_permute_workspace",
     "b200moe_permute",
     "b200moe_permute_noalloc",
     "b200moe_expert_gemm",
     "b200moe_w8a8_gemm",
+    "b200moe_int8_gemm",
     "b200moe_combine",
     "b200moe_combine_f32",
     "b200moe_append_shared_slot",
@@ -151,6 +159,26 @@ def _load() -> ctypes.CDLL:
     lib.b200moe_act_quant_fp8.restype = c_int
     lib.b200moe_act_quant_fp8.argtypes = [c_int, c_void_p, c_void_p, c_longlong, c_void_p, c_int, c_int,
                                           c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int]
+    lib.b200moe_route_grouped.restype = c_int
+    lib.b200moe_route_grouped.argtypes = [
+        c_int, c_void_p, c_void_p, c_int, c_longlong, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
+        c_int, c_float, c_void_p, c_void_p, c_void_p,
+    ]
+    lib.b200moe_act_quant_int8.restype = c_int
+    lib.b200moe_act_quant_int8.argtypes = [
+        c_int, c_void_p, c_void_p, c_longlong, c_int, c_int, c_int, c_void_p, c_int, c_int, c_void_p, c_int,
+        c_int, c_void_p, c_void_p,
+    ]
+    lib.b200moe_scatter_rows_8bit.restype = c_int
+    lib.b200moe_scatter_rows_8bit.argtypes = [
+        c_int, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_void_p, c_int, c_int, c_void_p, c_int, c_int,
+        c_void_p, c_void_p,
+    ]
+    lib.b200moe_add_rmsnorm.restype = c_int
+    lib.b200moe_add_rmsnorm.argtypes = [
+        c_int, c_void_p, c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_int,
+        c_float, c_int, c_int, c_void_p, c_longlong, c_int, c_void_p, c_int, c_void_p,
+    ]
     lib.b200moe_permute_workspace.restype = c_int
     lib.b200moe_permute_workspace.argtypes = [c_int, c_int, c_int, POINTER(c_size_t)]
     lib.b200moe_permute.restype = c_int
@@ -166,6 +194,8 @@ def _load() -> ctypes.CDLL:
     lib.b200moe_expert_gemm.argtypes = [c_int, c_void_p, POINTER(GemmArgs)]
     lib.b200moe_w8a8_gemm.restype = c_int
     lib.b200moe_w8a8_gemm.argtypes = [c_int, c_void_p, POINTER(GemmArgs), c_void_p, c_void_p]
+    lib.b200moe_int8_gemm.restype = c_int
+    lib.b200moe_int8_gemm.argtypes = [c_int, c_void_p, POINTER(GemmArgs), c_void_p, c_void_p, c_void_p, c_void_p]
     lib.b200moe_gemm_args_size.restype = c_size_t
     lib.b200moe_gemm_args_size.argtypes = []
     if lib.b200moe_gemm_args_size() != ctypes.sizeof(GemmArgs):

@@ -50,6 +50,7 @@ int* g_status_ptr[kMaxDevices] = {};
 int g_sm_count[kMaxDevices] = {};
 bool g_gemm_attr[kMaxDevices] = {};
 bool g_w8a8_attr[kMaxDevices][4] = {};
+bool g_int8_attr[kMaxDevices][5] = {};
 void* g_permute_scratch_ptr[kMaxDevices] = {};
 
 int use_device(int device, int** status) {
@@ -67,6 +68,18 @@ int use_device(int device, int** status) {
   if (status) *status = g_status_ptr[device];
   return B200MOE_OK;
 }
+
+// Puts back the device that was current before the call.
+struct DeviceScope {
+  int prev = -1;
+  DeviceScope() {
+    if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
+  }
+  ~DeviceScope() {
+    int now = -1;
+    if (prev >= 0 && cudaGetDevice(&now) == cudaSuccess && now != prev) cudaSetDevice(prev);
+  }
+};
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
@@ -146,6 +159,169 @@ int b200moe_router(int device, void* stream, int mode, const void* hidden, long 
   B200_CUDA(b200::launch_router_select(st, mode, logits, T, E, K, normalize,
                                        mode == B200MOE_ROUTER_QWEN3 ? probs : nullptr, scores,
                                        indices, counts));
+  return B200MOE_OK;
+}
+
+int b200moe_route_grouped(int device, void* stream, const void* logits, int logits_bf16,
+                          long long ld_logits, const float* bias, int T, int E, int K, int n_group,
+                          int topk_group, int group_top, int scoring, int normalize, float scale,
+                          float* scores, long long* indices, int* counts) {
+  B200_CHECK(T >= 0 && E >= 1 && K >= 1, "bad sizes T=%d E=%d K=%d", T, E, K);
+  B200_CHECK(n_group >= 1 && E % n_group == 0, "n_group %d must divide E=%d", n_group, E);
+  B200_CHECK(topk_group >= 1 && topk_group <= n_group, "topk_group %d must be in [1, %d]", topk_group, n_group);
+  B200_CHECK(group_top == 1 || group_top == 2, "group_top must be 1 or 2");
+  B200_CHECK(scoring == B200MOE_SCORE_SIGMOID || scoring == B200MOE_SCORE_SOFTMAX, "bad scoring %d", scoring);
+  B200_CHECK(logits_bf16 == 0 || logits_bf16 == 1, "logits_bf16 must be 0 or 1");
+  if (E > 512 || n_group > 32 || K > 32)
+    return fail(B200MOE_ERR_UNSUPPORTED, "grouped routing supports E <= 512, n_group <= 32 and K <= 32 (E=%d "
+                "n_group=%d K=%d)", E, n_group, K);
+  B200_CHECK(K <= topk_group * (E / n_group), "K=%d exceeds the %d experts of the kept groups", K,
+             topk_group * (E / n_group));
+  B200_CHECK(ld_logits >= E, "ld_logits must be at least E");
+  B200_CHECK(T == 0 || (logits && scores && indices), "logits, scores and indices are required");
+  DeviceScope scope;
+  int rc = use_device(device, nullptr);
+  if (rc) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (counts) B200_CUDA(cudaMemsetAsync(counts, 0, sizeof(int) * E, st));
+  if (T == 0) return B200MOE_OK;
+  b200::RouteParams p{};
+  p.logits = logits;
+  p.bf16 = logits_bf16;
+  p.ld = ld_logits;
+  p.bias = bias;
+  p.T = T;
+  p.K = K;
+  p.S = E / n_group;
+  p.G = n_group;
+  p.P = pow2_ceil(n_group);
+  p.keep = topk_group;
+  p.top = group_top;
+  p.softmax = scoring == B200MOE_SCORE_SOFTMAX;
+  p.normalize = normalize != 0;
+  p.scale = scale;
+  p.scores = scores;
+  p.indices = indices;
+  p.counts = counts;
+  B200_CUDA(b200::launch_route_grouped(st, p));
+  return B200MOE_OK;
+}
+
+int b200moe_act_quant_int8(int device, void* stream, const void* x, long long ldx, int rows,
+                           int k_valid, int k_pad, const int* inverse, int copies, int rows_out,
+                           const int* row_offsets, int expert_lo, int expert_hi, void* q, float* s) {
+  B200_CHECK(rows >= 0 && k_valid >= 1 && k_pad >= k_valid && rows_out >= 0 && copies >= 1,
+             "bad sizes rows=%d k_valid=%d k_pad=%d rows_out=%d copies=%d", rows, k_valid, k_pad, rows_out, copies);
+  B200_CHECK(k_valid % 8 == 0 && k_pad % 16 == 0 && ldx % 8 == 0 && ldx >= k_valid,
+             "need k_valid %% 8 == 0, k_pad %% 16 == 0, ldx %% 8 == 0 and ldx >= k_valid");
+  if (k_pad > 8 * b200::kNormMaxVecs)
+    return fail(B200MOE_ERR_UNSUPPORTED, "at most %d columns (k_pad=%d)", 8 * b200::kNormMaxVecs, k_pad);
+  B200_CHECK(inverse || (copies == 1 && rows_out >= rows), "without inverse, copies is 1 and rows_out at least rows");
+  B200_CHECK(row_offsets == nullptr || (expert_lo >= 0 && expert_hi >= expert_lo), "bad expert range");
+  if (rows == 0 || rows_out == 0) return B200MOE_OK;
+  B200_CHECK(x && q && s, "x, q and s are required");
+  B200_CHECK(aligned16(x) && aligned16(q), "x and q must be 16-byte aligned");
+  DeviceScope scope;
+  int rc = use_device(device, nullptr);
+  if (rc) return rc;
+  b200::QuantInt8Params p{};
+  p.x = static_cast<const __nv_bfloat16*>(x);
+  p.ldx = ldx;
+  p.rows = rows;
+  p.k_valid = k_valid;
+  p.k_pad = k_pad;
+  p.inverse = inverse;
+  p.copies = copies;
+  p.rows_out = rows_out;
+  p.range = row_offsets;
+  p.expert_lo = expert_lo;
+  p.expert_hi = expert_hi;
+  p.q = static_cast<uint8_t*>(q);
+  p.scale = s;
+  B200_CUDA(b200::launch_act_quant_int8(static_cast<cudaStream_t>(stream), p));
+  return B200MOE_OK;
+}
+
+int b200moe_scatter_rows_8bit(int device, void* stream, const void* q, int row_bytes,
+                              const float* scale, int groups, int rows, const int* inverse,
+                              int copies, int rows_out, const int* row_offsets, int expert_lo,
+                              int expert_hi, void* out, float* out_scale) {
+  B200_CHECK(rows >= 0 && row_bytes >= 16 && row_bytes % 16 == 0 && groups >= 1 && copies >= 1 && rows_out >= 0,
+             "bad sizes rows=%d row_bytes=%d groups=%d copies=%d rows_out=%d", rows, row_bytes, groups, copies,
+             rows_out);
+  B200_CHECK(row_offsets == nullptr || (expert_lo >= 0 && expert_hi >= expert_lo), "bad expert range");
+  if (rows == 0 || rows_out == 0) return B200MOE_OK;
+  B200_CHECK(q && scale && inverse && out && out_scale, "q, scale, inverse, out and out_scale are required");
+  B200_CHECK(aligned16(q) && aligned16(out), "q and out must be 16-byte aligned");
+  DeviceScope scope;
+  int rc = use_device(device, nullptr);
+  if (rc) return rc;
+  b200::ScatterRowsParams p{};
+  p.q = static_cast<const uint8_t*>(q);
+  p.row_bytes = row_bytes;
+  p.scale = scale;
+  p.groups = groups;
+  p.rows = rows;
+  p.inverse = inverse;
+  p.copies = copies;
+  p.rows_out = rows_out;
+  p.range = row_offsets;
+  p.expert_lo = expert_lo;
+  p.expert_hi = expert_hi;
+  p.out = static_cast<uint8_t*>(out);
+  p.out_scale = out_scale;
+  B200_CUDA(b200::launch_scatter_rows_8bit(static_cast<cudaStream_t>(stream), p));
+  return B200MOE_OK;
+}
+
+int b200moe_add_rmsnorm(int device, void* stream, const void* x, long long ldx,
+                        const void* residual, long long ldr, void* residual_out, long long ldro,
+                        const void* weight, int weight_f32, float eps, int T, int H, void* out,
+                        long long ldo, int quant, void* q, int k_pad, float* scale) {
+  B200_CHECK(T >= 0 && H >= 8 && H % 8 == 0, "need T >= 0 and H a positive multiple of 8 (T=%d H=%d)", T, H);
+  B200_CHECK(quant >= B200MOE_QUANT_NONE && quant <= B200MOE_QUANT_INT8, "bad quant %d", quant);
+  B200_CHECK(weight_f32 == 0 || weight_f32 == 1, "weight_f32 must be 0 or 1");
+  B200_CHECK(eps >= 0.f, "eps must not be negative");
+  if (H > 8 * b200::kNormMaxVecs)
+    return fail(B200MOE_ERR_UNSUPPORTED, "at most %d columns (H=%d)", 8 * b200::kNormMaxVecs, H);
+  if (quant != B200MOE_QUANT_NONE) {
+    B200_CHECK(k_pad >= H && k_pad % 16 == 0, "k_pad must be at least H and a multiple of 16");
+    if (k_pad > 8 * b200::kNormMaxVecs)
+      return fail(B200MOE_ERR_UNSUPPORTED, "at most %d columns (k_pad=%d)", 8 * b200::kNormMaxVecs, k_pad);
+  }
+  B200_CHECK(ldx >= H && ldx % 8 == 0, "ldx must be at least H and a multiple of 8");
+  B200_CHECK(!residual || (ldr >= H && ldr % 8 == 0), "ldr must be at least H and a multiple of 8");
+  B200_CHECK(!residual_out || (residual && ldro >= H && ldro % 8 == 0),
+             "residual_out needs a residual and ldro at least H, a multiple of 8");
+  B200_CHECK(!out || (ldo >= H && ldo % 8 == 0), "ldo must be at least H and a multiple of 8");
+  if (T == 0) return B200MOE_OK;
+  B200_CHECK(x && weight, "x and weight are required");
+  B200_CHECK(quant == B200MOE_QUANT_NONE || (q && scale), "q and scale are required");
+  B200_CHECK(aligned16(x) && aligned16(residual) && aligned16(residual_out) && aligned16(weight) && aligned16(out) &&
+                 (quant == B200MOE_QUANT_NONE || aligned16(q)),
+             "x, residual, residual_out, weight, out and q must be 16-byte aligned");
+  DeviceScope scope;
+  int rc = use_device(device, nullptr);
+  if (rc) return rc;
+  b200::NormParams p{};
+  p.x = static_cast<const __nv_bfloat16*>(x);
+  p.ldx = ldx;
+  p.res = static_cast<const __nv_bfloat16*>(residual);
+  p.ldr = ldr;
+  p.res_out = static_cast<__nv_bfloat16*>(residual_out);
+  p.ldro = ldro;
+  p.weight = weight;
+  p.weight_f32 = weight_f32;
+  p.eps = eps;
+  p.T = T;
+  p.H = H;
+  p.out = static_cast<__nv_bfloat16*>(out);
+  p.ldo = ldo;
+  p.quant = quant;
+  p.q = static_cast<uint8_t*>(q);
+  p.k_pad = k_pad;
+  p.scale = scale;
+  B200_CUDA(b200::launch_add_rmsnorm(static_cast<cudaStream_t>(stream), p));
   return B200MOE_OK;
 }
 
@@ -642,6 +818,120 @@ int b200moe_w8a8_gemm(int device, void* stream, const b200moe_gemm_args* a, cons
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid, 1, 1);
   cfg.blockDim = dim3(b200::kW8A8Threads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  void* args[] = {&qmap, &p};
+  B200_CUDA(cudaLaunchKernelExC(&cfg, kern, args));
+  return B200MOE_OK;
+}
+
+int b200moe_int8_gemm(int device, void* stream, const b200moe_gemm_args* a, const void* q,
+                      const float* q_scale, const float* w_scale, const float* bias) {
+  B200_CHECK(a != nullptr, "args is NULL");
+  if (a->max_rows <= 0) return B200MOE_OK;
+  B200_CHECK(a->weight && q && q_scale && w_scale && a->out, "weight, q, q_scale, w_scale, out are required");
+  B200_CHECK(a->offsets || (a->n_experts == 1 && a->expert_begin == 0), "more than one expert needs offsets");
+  B200_CHECK(a->wfmt == B200MOE_W_INT8, "the int8 GEMM needs int8 weights");
+  B200_CHECK(a->planes == 1 || a->planes == 2, "planes must be 1 or 2");
+  B200_CHECK((a->planes == 2 && (a->epilogue == B200MOE_EPI_SWIGLU_F32 || a->epilogue == B200MOE_EPI_CLAMP_SWIGLU_F32)) ||
+                 (a->planes == 1 && a->epilogue == B200MOE_EPI_DOWN_ONCE),
+             "the int8 GEMM supports SWIGLU_F32 and CLAMP_SWIGLU_F32 with two planes, DOWN_ONCE with one");
+  B200_CHECK(a->bias == nullptr, "the bias is an argument of its own (fp32, tile row order)");
+  B200_CHECK(a->b_map == nullptr, "the int8 GEMM reads quantised permuted rows (b_map must be NULL)");
+  B200_CHECK(a->planes == 1 || a->row_weight == nullptr, "routing weights need the down epilogue");
+  B200_CHECK(a->n_experts >= 1 && a->expert_begin >= 0, "bad expert range");
+  if (a->n_experts > 1024) return fail(B200MOE_ERR_UNSUPPORTED, "at most 1024 experts per launch");
+  B200_CHECK(a->feat_pad >= 128 && a->feat_pad % 128 == 0, "feat_pad must be a positive multiple of 128");
+  B200_CHECK(a->n_feat >= 1 && a->n_feat <= a->feat_pad, "n_feat out of range");
+  B200_CHECK(a->k_pad >= 128 && a->k_pad % 128 == 0, "k_pad must be a positive multiple of 128");
+  if (a->k_pad >= 131072)
+    return fail(B200MOE_ERR_UNSUPPORTED, "k_pad must be below 131072, where the int32 sum could overflow");
+  B200_CHECK(a->b_rows >= 1 && a->b_rows >= a->max_rows, "q must have at least max_rows rows");
+  B200_CHECK(aligned16(q) && aligned16(a->weight), "q and weight must be 16-byte aligned");
+  B200_CHECK(a->ldo >= a->n_feat && a->ldo % 8 == 0 && a->n_feat % 8 == 0 && aligned16(a->out),
+             "output rows must be 16-byte aligned (ldo %% 8 == 0, n_feat %% 8 == 0)");
+  if (a->row_weight) B200_CHECK(a->row_src != nullptr, "row_weight needs row_src");
+  B200_CHECK(a->token_tile == 0 || a->token_tile == 16 || a->token_tile == 32 || a->token_tile == 64 ||
+                 a->token_tile == 128 || a->token_tile == 256,
+             "token_tile must be 0, 16, 32, 64, 128 or 256");
+  DeviceScope scope;
+  int* sp = nullptr;
+  int rc = use_device(device, &sp);
+  if (rc) return rc;
+
+  const bool is_gated = a->planes == 2;
+  int bn = a->token_tile;
+  if (bn == 0) {
+    // 1.5x the mean rows per expert, so that one tile usually holds an expert's rows
+    const long long avg = (3ll * a->max_rows + 2ll * a->n_experts - 1) / (2ll * a->n_experts);
+    bn = std::min(256, std::max(16, pow2_ceil(static_cast<int>(std::min(avg, 1ll << 20)))));
+  }
+  const int feat_tiles = a->feat_pad / (is_gated ? 64 : 128);
+  const long long tiles_ub = (long long)(std::min(a->n_experts, a->max_rows) + a->max_rows / bn) * feat_tiles;
+  if (tiles_ub > 0x7fffffffll) return fail(B200MOE_ERR_UNSUPPORTED, "too many tiles");
+
+  b200::Int8Params p{};
+  p.offsets = a->offsets;
+  p.dense_rows = a->max_rows;
+  p.expert_begin = a->expert_begin;
+  p.n_experts = a->n_experts;
+  p.gated = is_gated ? 1 : 0;
+  p.feat_tiles = feat_tiles;
+  p.n_feat = a->n_feat;
+  p.nkb = a->k_pad / 128;
+  p.wtiles = static_cast<const uint8_t*>(a->weight);
+  p.wscale = w_scale;
+  p.bias = bias;
+  p.qs = q_scale;
+  p.epi = a->epilogue;
+  p.alpha = a->alpha;
+  p.limit = a->limit;
+  p.row_w = a->row_weight;
+  p.row_w_bf16 = a->row_weight_bf16;
+  p.row_src = a->row_src;
+  p.out = static_cast<__nv_bfloat16*>(a->out);
+  p.ldo = a->ldo;
+  p.status = sp;
+  p.box = std::min(bn, 64);
+  // shared memory: stages of a 16 KB weight image and bn x 128 B token rows,
+  // the epilogue's scales, barriers and the tile prefix
+  const uint32_t budget = 232448u - 2048u;
+  p.stage_bytes = 16384u + static_cast<uint32_t>(bn) * 128u;
+  const uint32_t xbytes = (b200::int8_epilogue_bytes(bn) + 1023u) & ~1023u;
+  const uint32_t barbytes = ((8u * (2u * 16u + 5u) + 8u + 4u * (a->n_experts + 1) + 1023u) / 1024u) * 1024u;
+  p.ns = static_cast<int>(std::min<uint32_t>(16u, (budget - xbytes - barbytes) / p.stage_bytes));
+  if (p.ns < 2) return fail(B200MOE_ERR_UNSUPPORTED, "shared memory plan does not fit (token_tile=%d)", bn);
+  p.x_off = p.ns * p.stage_bytes;
+  p.bar_off = p.x_off + xbytes;
+  const uint32_t smem = p.bar_off + barbytes + 1024u;   // + alignment slack
+  p.tmem_cols = static_cast<uint32_t>(std::max(32, 2 * bn));
+
+  PFN_cuTensorMapEncodeTiled_v12000 enc = encode_fn();
+  if (!enc) return fail(B200MOE_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+  CUtensorMap qmap;
+  {
+    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(a->k_pad), static_cast<cuuint64_t>(a->b_rows)};
+    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(a->k_pad)};
+    const cuuint32_t box[2] = {128, static_cast<cuuint32_t>(p.box)};
+    const cuuint32_t estr[2] = {1, 1};
+    CUresult cr = enc(&qmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(q), dims, strides, box, estr,
+                      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (cr != CUDA_SUCCESS) return fail(B200MOE_ERR_CUDA, "activation tensor map failed (%d)", (int)cr);
+  }
+  const int ti = bn == 16 ? 0 : bn == 32 ? 1 : bn == 64 ? 2 : bn == 128 ? 3 : 4;
+  const void* kern = b200::int8_kernel_ptr(bn);
+  {
+    std::lock_guard<std::mutex> lock(g_mu);
+    if (!g_int8_attr[device][ti]) {
+      B200_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448 - 1024));
+      g_int8_attr[device][ti] = true;
+    }
+  }
+  const int grid = static_cast<int>(std::min<long long>(g_sm_count[device], tiles_ub));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid, 1, 1);
+  cfg.blockDim = dim3(b200::kInt8Threads, 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = static_cast<cudaStream_t>(stream);
   void* args[] = {&qmap, &p};

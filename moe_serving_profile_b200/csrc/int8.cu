@@ -1,0 +1,312 @@
+// Int8 grouped GEMM: int8 token rows with one scale each times int8 expert
+// weights with one scale per output channel, on the tensor cores
+// (tcgen05.mma kind::i8, exact int32 sums in tensor memory).
+//
+//   D[n, f] = qs[n] * ws[f] * sum_k Q[n, k] * W[f, k]  (+ bias[f])
+//
+// The whole sum over k is one integer, so the scales meet it once, in the
+// epilogue, which works in fp32 and rounds once to bf16:
+//   SwiGLU          bf16(g / (1 + exp(-g)) * u)
+//   clamped SwiGLU  g = min(g, limit), u = clamp(u), bf16(g / (1 + exp(-alpha g)) * (u + 1))
+//   down            bf16(D * routing weight of the row)
+//
+// Weights are the MMA's M = 128 operand, token rows its N: decode tiles of a
+// few rows then waste no tensor work, and N follows each tile's row count. A
+// weight tile's k-block (128 rows x 128 columns) is stored as the 16 KB image
+// that the MMA reads (128-byte swizzle), so one bulk copy moves it. In a gated
+// tile, rows 32 q + 0..15 are gate rows and 32 q + 16..31 the up rows of the
+// same 16 features: one warp holds both halves of its features and trades
+// them by a lane exchange.
+//
+// 320 threads: warp 0 copies, warp 1 issues the MMAs, warps 2-9 run the
+// epilogue (two per 32-lane quarter of tensor memory, alternating 16-column
+// chunks). Two accumulator slots let the epilogue of a tile overlap the next
+// tile's products.
+#include "internal.h"
+#include "ptx.cuh"
+
+namespace b200 {
+namespace i8 {
+
+constexpr unsigned kFull = 0xffffffffu;
+constexpr int kThreads = kInt8Threads;
+constexpr int kEpi = kThreads - 64;
+constexpr uint32_t kAStage = 16384;   // 128 weight rows x 128 int8
+
+enum { kEpiClampF32 = 3, kEpiSwigluF32 = 5, kEpiDownOnce = 6 };
+
+struct Tile {
+  int e, ft, row0, nrows;
+};
+
+struct Ring {
+  int n, idx;
+  uint32_t phase;
+  __device__ explicit Ring(int n_) : n(n_), idx(0), phase(0u) {}
+  __device__ void next() {
+    if (++idx == n) {
+      idx = 0;
+      phase ^= 1u;
+    }
+  }
+};
+
+// Rows [x, y) of local expert e in the permuted order (no offsets: one expert
+// holds all rows).
+__device__ __forceinline__ int2 expert_rows(const Int8Params& p, int e) {
+  if (p.offsets == nullptr) return make_int2(0, p.dense_rows);
+  return make_int2(p.offsets[p.expert_begin + e], p.offsets[p.expert_begin + e + 1]);
+}
+
+// Tile t: feature tile t % feat_tiles of row chunk t / feat_tiles. An expert's
+// rows are cut into ceil(rows / BN) chunks of equal size rounded up to 16 (the
+// MMA's N granule), so that no chunk is nearly empty.
+template <int BN>
+__device__ __forceinline__ Tile decode_tile(int t, const int* prefix, const Int8Params& p) {
+  Tile r;
+  const int u = t / p.feat_tiles;
+  r.ft = t - u * p.feat_tiles;
+  int lo = 0, hi = p.n_experts;   // largest lo with prefix[lo] <= u
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (prefix[mid] <= u) lo = mid; else hi = mid;
+  }
+  r.e = lo;
+  const int sub = u - prefix[lo], parts = prefix[lo + 1] - prefix[lo];
+  const int2 rows = expert_rows(p, lo);
+  const int start = rows.x, cnt = rows.y - rows.x;
+  const int size = (((cnt + parts - 1) / parts) + 15) & ~15;
+  r.row0 = start + sub * size;
+  r.nrows = min(size, cnt - sub * size);   // rounding up may leave the last chunk empty
+  return r;
+}
+
+__device__ __forceinline__ float row_weight(const Int8Params& p, int row) {
+  const int src = p.row_src[row];
+  return p.row_w_bf16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p.row_w)[src])
+                      : reinterpret_cast<const float*>(p.row_w)[src];
+}
+
+__device__ __forceinline__ float gated(const Int8Params& p, float g, float u) {
+  float a = 1.f;
+  if (p.epi == kEpiClampF32) {
+    g = g > p.limit ? p.limit : g;
+    u = u < -p.limit ? -p.limit : (u > p.limit ? p.limit : u);
+    u += 1.f;
+    a = p.alpha;
+  }
+  return g / (1.f + expf(-a * g)) * u;
+}
+
+template <int BN>
+__global__ void __launch_bounds__(kThreads, 1)
+    int8_gemm_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ Int8Params p) {
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_u32 = smem_u32(smem_raw);
+  const uint32_t base_u32 = (raw_u32 + 1023u) & ~1023u;
+  uint8_t* sbase = smem_raw + (base_u32 - raw_u32);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  uint64_t* full = reinterpret_cast<uint64_t*>(sbase + p.bar_off);
+  uint64_t* empty = full + p.ns;
+  uint64_t* acc_full = empty + p.ns;    // [2]
+  uint64_t* acc_empty = acc_full + 2;   // [2]
+  uint64_t* mma_done = acc_empty + 2;
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(mma_done + 1);
+  int* s_total = reinterpret_cast<int*>(s_tmem + 1);
+  int* prefix = s_total + 1;            // [n_experts + 1]: row chunks of the experts before
+
+  if (warp == 0) {
+    const int bad = *reinterpret_cast<volatile int*>(p.status) & kStatusWaitTimeout;
+    int acc = 0;
+    if (lane == 0) prefix[0] = 0;
+    for (int base = 0; base < p.n_experts; base += 32) {
+      const int e = base + lane;
+      int nt = 0;
+      if (e < p.n_experts) {
+        const int2 rows = expert_rows(p, e);
+        nt = (rows.y - rows.x + BN - 1) / BN;
+      }
+      int incl = nt;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(kFull, incl, o);
+        if (lane >= o) incl += v;
+      }
+      if (e < p.n_experts) prefix[e + 1] = acc + incl;
+      acc += __shfl_sync(kFull, incl, 31);
+    }
+    if (lane == 0) {
+      *s_total = bad ? 0 : acc * p.feat_tiles;   // after a wait gave up: nothing to do
+      for (int i = 0; i < p.ns; ++i) {
+        mbar_init(&full[i], 1);
+        mbar_init(&empty[i], 1);
+      }
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(&acc_full[i], 1);
+        mbar_init(&acc_empty[i], kEpi / 32);
+      }
+      mbar_init(mma_done, 1);
+      fence_mbar_init();
+      tma_prefetch_desc(&qmap);
+    }
+  }
+  if (warp == 1) {
+    tmem_alloc(s_tmem, p.tmem_cols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *s_tmem;
+  const int total = *s_total;
+
+  if (warp == 0) {
+    // ------------------------------------------------ copies
+    if (lane == 0) {
+      Ring ring(p.ns);
+      int issued = 0;
+      bool ok = true;
+      for (int t = blockIdx.x; ok && t < total; t += gridDim.x) {
+        const Tile tl = decode_tile<BN>(t, prefix, p);
+        if (tl.nrows <= 0) continue;
+        const uint8_t* wt = p.wtiles + (long long)(tl.e * p.feat_tiles + tl.ft) * p.nkb * kAStage;
+        const int boxes = (tl.nrows + p.box - 1) / p.box;
+        for (int k = 0; k < p.nkb; ++k, ring.next(), ++issued) {
+          const int s = ring.idx;
+          if (!wait_bounded(&empty[s], ring.phase ^ 1u, p.status)) {
+            ok = false;
+            break;
+          }
+          uint8_t* st = sbase + s * p.stage_bytes;
+          mbar_arrive_expect_tx(&full[s], kAStage + boxes * p.box * 128);
+          bulk_load(st, wt + (long long)k * kAStage, kAStage, &full[s]);
+          for (int b = 0; b < boxes; ++b)
+            tma_load_2d(st + kAStage + b * p.box * 128, &qmap, &full[s], k * 128, tl.row0 + b * p.box);
+        }
+      }
+      // every issued copy has landed before the CTA may exit
+      for (int i = max(0, issued - p.ns); i < issued; ++i)
+        wait_bounded(&full[i % p.ns], (i / p.ns) & 1, p.status, 32);
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------ MMAs
+    if (lane == 0) {
+      Ring ring(p.ns);
+      int tc = 0;
+      bool ok = true;
+      for (int t = blockIdx.x; ok && t < total; t += gridDim.x) {
+        const Tile tl = decode_tile<BN>(t, prefix, p);
+        if (tl.nrows <= 0) continue;
+        const int slot = tc & 1;
+        if (!wait_bounded(&acc_empty[slot], ((tc >> 1) & 1) ^ 1, p.status)) break;
+        const uint32_t idesc = idesc_s8_s32(128, (tl.nrows + 15) & ~15);
+        const uint32_t d = tmem + static_cast<uint32_t>(slot * BN);
+        for (int k = 0; k < p.nkb; ++k, ring.next()) {
+          const int s = ring.idx;
+          if (!wait_bounded(&full[s], ring.phase, p.status)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t st = base_u32 + s * p.stage_bytes;
+          const uint64_t ad = sdesc_k_sw128(st), bd = sdesc_k_sw128(st + kAStage);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) umma_s8(d, ad + 2 * j, bd + 2 * j, idesc, (k | j) != 0 ? 1u : 0u);
+          umma_commit(&empty[s]);
+        }
+        umma_commit(&acc_full[slot]);
+        ++tc;
+      }
+      // all issued MMAs have finished before tensor memory is released
+      umma_commit(mma_done);
+      wait_bounded(mma_done, 0, p.status);
+    }
+  } else {
+    // ------------------------------------------------ epilogue
+    // Warp w reads lanes 32 (w % 4) .. + 31 of tensor memory: lane i holds
+    // weight row r = 32 (w % 4) + i of the tile.
+    const int q = warp & 3, r = q * 32 + lane;
+    const int first = (warp - 2) >> 2;   // this warp's first 16-column chunk
+    const int te = threadIdx.x - 64;
+    const uint32_t tq = tmem + (static_cast<uint32_t>(q * 32) << 16);
+    float* xs = reinterpret_cast<float*>(sbase + p.x_off);   // [2 tiles][row scales BN | row weights BN]
+    const bool is_gate = lane < 16;
+    int tc = 0;
+    for (int t = blockIdx.x; t < total; t += gridDim.x) {
+      const Tile tl = decode_tile<BN>(t, prefix, p);
+      if (tl.nrows <= 0) continue;
+      const int slot = tc & 1;
+      float* sa = xs + (tc & 1) * (2 * BN);
+      float* rw = sa + BN;
+      for (int n = te; n < BN; n += kEpi) {
+        const bool in = n < tl.nrows;
+        sa[n] = in ? p.qs[tl.row0 + n] : 0.f;
+        rw[n] = in && p.row_w ? row_weight(p, tl.row0 + n) : 1.f;
+      }
+      const long long wrow = (long long)(tl.e * p.feat_tiles + tl.ft) * 128 + r;
+      const float ws = p.wscale[wrow];
+      const float bias = p.bias ? p.bias[wrow] : 0.f;
+      const int f = p.gated ? tl.ft * 64 + q * 16 + (lane & 15) : tl.ft * 128 + r;
+      // publishes the tile's scales and lets the eight warps agree on success
+      if (!named_bar_and(1, kEpi, wait_bounded(&acc_full[slot], (tc >> 1) & 1, p.status))) break;
+      tc_fence_after();
+      uint16_t* out = reinterpret_cast<uint16_t*>(p.out) + (long long)tl.row0 * p.ldo + f;
+      for (int c0 = first * 16; c0 < tl.nrows; c0 += 32) {
+        uint32_t v[16];
+        tmem_ld16(tq + static_cast<uint32_t>(slot * BN + c0), v);
+        tmem_ld_wait();
+        float d[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          d[j] = fmaf(static_cast<float>(static_cast<int>(v[j])), sa[c0 + j] * ws, bias);
+        if (p.gated) {
+#pragma unroll
+          for (int j = 0; j < 16; j += 2) {
+            // gate lanes keep column j, up lanes column j + 1
+            const float got = __shfl_xor_sync(kFull, is_gate ? d[j + 1] : d[j], 16);
+            const float y = is_gate ? gated(p, d[j], got) : gated(p, got, d[j + 1]);
+            const int n = c0 + j + (is_gate ? 0 : 1);
+            if (n < tl.nrows && f < p.n_feat)
+              out[(long long)n * p.ldo] = static_cast<uint16_t>(__bfloat16_as_ushort(__float2bfloat16_rn(y)));
+          }
+        } else if (f < p.n_feat) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            if (c0 + j < tl.nrows)
+              out[(long long)(c0 + j) * p.ldo] =
+                  static_cast<uint16_t>(__bfloat16_as_ushort(__float2bfloat16_rn(d[j] * rw[c0 + j])));
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&acc_empty[slot]);
+      ++tc;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, p.tmem_cols);
+  }
+}
+
+}  // namespace i8
+
+// Row scales and routing weights of two tiles.
+uint32_t int8_epilogue_bytes(int bn) { return 16u * static_cast<uint32_t>(bn); }
+
+const void* int8_kernel_ptr(int bn) {
+  switch (bn) {
+    case 16: return reinterpret_cast<const void*>(&i8::int8_gemm_kernel<16>);
+    case 32: return reinterpret_cast<const void*>(&i8::int8_gemm_kernel<32>);
+    case 64: return reinterpret_cast<const void*>(&i8::int8_gemm_kernel<64>);
+    case 128: return reinterpret_cast<const void*>(&i8::int8_gemm_kernel<128>);
+    case 256: return reinterpret_cast<const void*>(&i8::int8_gemm_kernel<256>);
+    default: return nullptr;
+  }
+}
+
+}  // namespace b200

@@ -47,6 +47,96 @@ uint32_t w8a8_epilogue_bytes(int bn, int gated);
 int w8a8_tmem_buffers(int bn);      // group accumulators in tensor memory (4: the MMAs run 3 groups ahead)
 const void* w8a8_kernel_ptr(int bn);   // token tile 16, 32, 64 or 128; else NULL
 
+// Grouped expert routing (route.cu).
+struct RouteParams {
+  const void* logits;          // fp32 or bf16 rows of ld elements
+  int bf16;
+  long long ld;
+  const float* bias;           // [E] or NULL
+  int T, K, S, G, P;           // S experts in each of G groups, P the power of two >= G
+  int keep, top;               // groups kept, keys in a group's sum (1 or 2)
+  int softmax, normalize;
+  float scale;
+  float* scores;
+  long long* indices;
+  int* counts;
+};
+cudaError_t launch_route_grouped(cudaStream_t st, const RouteParams& p);
+
+// RMS norm with residual and 8-bit output, and the 8-bit row movers (norm.cu).
+struct NormParams {
+  const __nv_bfloat16* x;
+  long long ldx;
+  const __nv_bfloat16* res;    // NULL: no residual
+  long long ldr;
+  __nv_bfloat16* res_out;      // NULL: the sum is not stored
+  long long ldro;
+  const void* weight;
+  int weight_f32;
+  float eps;
+  int T, H;
+  __nv_bfloat16* out;          // NULL: no bf16 output
+  long long ldo;
+  int quant;                   // 0 none, 1 e4m3 per 128 columns, 2 int8 per row
+  uint8_t* q;                  // [T][k_pad]
+  int k_pad;
+  float* scale;
+};
+constexpr int kNormMaxVecs = 4096;   // 1024 threads x 4 vectors of 8 columns
+cudaError_t launch_add_rmsnorm(cudaStream_t st, const NormParams& p);
+
+struct QuantInt8Params {
+  const __nv_bfloat16* x;
+  long long ldx;
+  int rows, k_valid, k_pad;
+  const int* inverse;          // [rows][copies] places in the permuted order, or NULL: row r goes to r
+  int copies, rows_out;
+  const int* range;            // expert offsets: only places of [expert_lo, expert_hi), or NULL
+  int expert_lo, expert_hi;
+  uint8_t* q;
+  float* scale;
+};
+cudaError_t launch_act_quant_int8(cudaStream_t st, const QuantInt8Params& p);
+
+struct ScatterRowsParams {
+  const uint8_t* q;
+  int row_bytes;
+  const float* scale;
+  int groups, rows;
+  const int* inverse;
+  int copies, rows_out;
+  const int* range;
+  int expert_lo, expert_hi;
+  uint8_t* out;
+  float* out_scale;
+};
+cudaError_t launch_scatter_rows_8bit(cudaStream_t st, const ScatterRowsParams& p);
+
+// Int8 grouped GEMM (int8.cu): kernel parameters, filled by the host.
+struct Int8Params {
+  const int* offsets;          // permuted-row offsets of the global experts; NULL: one expert, all dense_rows rows
+  int dense_rows;
+  int expert_begin, n_experts;
+  int gated, feat_tiles, n_feat, nkb;
+  const uint8_t* wtiles;       // [n_experts][feat_tiles][nkb][128 rows x 128 bytes, swizzled]
+  const float* wscale;         // [n_experts][feat_tiles][128], tile row order
+  const float* bias;           // as wscale, or NULL
+  const float* qs;             // [rows]
+  int epi;
+  float alpha, limit;
+  const void* row_w;
+  int row_w_bf16;
+  const int* row_src;
+  __nv_bfloat16* out;
+  long long ldo;
+  int* status;
+  int ns, box;                 // pipeline stages, token rows per copy
+  uint32_t stage_bytes, x_off, bar_off, tmem_cols;
+};
+constexpr int kInt8Threads = 320;    // copy warp, MMA warp, 8 epilogue warps
+const void* int8_kernel_ptr(int bn); // token tile 16, 32, 64, 128 or 256; else NULL
+uint32_t int8_epilogue_bytes(int bn);
+
 size_t permute_workspace_bytes(int T, int K, int E);
 cudaError_t launch_permute(cudaStream_t st, const long long* indices, int T, int K, int E,
                            int* counts, int* offsets, int* perm_src, int* inverse,

@@ -290,6 +290,25 @@ B200_DEVI void umma_e4m3(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32
       : "memory");
 }
 
+// Instruction descriptor: kind::i8, A = B = signed 8-bit, D = S32, both K-major.
+__host__ __device__ constexpr uint32_t idesc_s8_s32(int M, int N) {
+  return (2u << 4)                                  // D format S32
+         | (1u << 7)                                // A signed
+         | (1u << 10)                               // B signed
+         | (static_cast<uint32_t>(N >> 3) << 17)    // N / 8
+         | (static_cast<uint32_t>(M >> 4) << 24);   // M / 16
+}
+
+// D (+)= A * B for one 32-byte (32 x int8) slice of K.
+B200_DEVI void umma_s8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(tmem_d),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
 // Instruction descriptor: kind::f16, A = B = BF16, D = F32, both K-major.
 __host__ __device__ constexpr uint32_t idesc_bf16_f32(int M, int N) {
   return (1u << 4)                                  // D format F32

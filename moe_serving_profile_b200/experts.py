@@ -20,7 +20,7 @@ from functools import lru_cache
 import torch
 
 from moe_serving_profile_b200 import _lib, ops
-from moe_serving_profile_b200.layout import ExpertWeights
+from moe_serving_profile_b200.layout import ExpertWeights, Int8Linear
 
 
 @lru_cache(maxsize=None)
@@ -68,6 +68,9 @@ def run_experts(w: ExpertWeights, hidden: torch.Tensor, perm: ops.Permutation,
     T, H = hidden.shape
     if H != w.hidden:
         raise ValueError(f"hidden size {H} does not match the experts' {w.hidden}")
+    if w.fmt == _lib.W_INT8:   # rows are exact sums of integers: no tile size changes them
+        return run_experts_int8(w, hidden, perm, weights, K=K, num_experts=num_experts, expert_begin=expert_begin,
+                                contrib=contrib, copies=K if b_map_div is None else b_map_div)
     tokens = T if tile_tokens is None else tile_tokens
     act = gate_up(w, hidden, perm, K=K, num_experts=num_experts, expert_begin=expert_begin,
                   b_map_div=b_map_div, tokens=tokens)
@@ -122,17 +125,136 @@ def down(w: ExpertWeights, act: torch.Tensor, perm: ops.Permutation,
     return contrib
 
 
+def _local_range(w: ExpertWeights, perm: ops.Permutation, num_experts: int, expert_begin: int) -> dict:
+    """The quantisers' row range of a rank that holds some of the experts."""
+    lo, hi = expert_begin, expert_begin + w.n_experts
+    return dict(offsets=perm.offsets, expert_lo=lo, expert_hi=hi) if (lo, hi) != (0, num_experts) else {}
+
+
+def int8_gate_up(w: ExpertWeights, hidden: torch.Tensor | ops.QuantRows, perm: ops.Permutation, *, K: int,
+                 num_experts: int, expert_begin: int, copies: int | None = None,
+                 out: torch.Tensor | None = None) -> torch.Tensor:
+    """Gated projection of int8 experts: act [T*K, I_p] bf16. ``hidden`` are
+    bf16 token rows, quantised once per token into the permuted order, or
+    token rows a norm already quantised (ops.QuantRows)."""
+    if w.fmt != _lib.W_INT8:
+        raise ValueError("int8_gate_up needs int8 expert weights")
+    local = _local_range(w, perm, num_experts, expert_begin)
+    copies = K if copies is None else copies
+    R = perm.perm_src.numel()
+    if isinstance(hidden, ops.QuantRows):
+        T = hidden.q.shape[0]
+        rows = ops.scatter_rows_8bit(hidden.checked(torch.int8, w.h_k, w.w1.device), perm.inverse, copies, **local)
+    else:
+        T = hidden.shape[0]
+        if hidden.shape[1] != w.hidden:
+            raise ValueError(f"hidden size {hidden.shape[1]} does not match the experts' {w.hidden}")
+        rows = ops.act_quant_int8(hidden, k_pad=w.h_k, inverse=perm.inverse, copies=copies, **local)
+    act = torch.empty(R, w.i_pad, device=w.w1.device, dtype=torch.bfloat16) if out is None else out
+    return ops.int8_gemm(offsets=perm.offsets, expert_begin=expert_begin, n_experts=w.n_experts, max_rows=R,
+                         planes=2, feat_pad=w.i_pad, n_feat=w.inter, k_pad=w.h_k, weight=w.w1, weight_scale=w.s1,
+                         rows=rows, epilogue=w.gated_epilogue, bias=w.b1, alpha=w.alpha, limit=w.limit, out=act,
+                         token_tile=tile_policy(T, copies, num_experts))
+
+
+def int8_down(w: ExpertWeights, act: torch.Tensor, perm: ops.Permutation, weights: torch.Tensor | None, *, K: int,
+              num_experts: int, expert_begin: int, contrib: torch.Tensor | None = None) -> torch.Tensor:
+    """Down projection of int8 experts on gated bf16 rows ``act`` (permuted
+    order, the first ``w.inter`` columns are read), times the routing weights
+    [T, K] when given: contribution rows [T*K, H] bf16."""
+    if w.fmt != _lib.W_INT8:
+        raise ValueError("int8_down needs int8 expert weights")
+    local = _local_range(w, perm, num_experts, expert_begin)
+    R = perm.perm_src.numel()
+    rows = ops.act_quant_int8(act[:, :w.inter], k_pad=w.i_pad, **local)
+    if contrib is None:
+        contrib = torch.empty(R, w.hidden, device=act.device, dtype=torch.bfloat16)
+    return ops.int8_gemm(offsets=perm.offsets, expert_begin=expert_begin, n_experts=w.n_experts, max_rows=R,
+                         planes=1, feat_pad=w.h_f, n_feat=w.hidden, k_pad=w.i_pad, weight=w.w2, weight_scale=w.s2,
+                         rows=rows, epilogue=_lib.EPI_DOWN_ONCE, bias=w.b2,
+                         row_weight=None if weights is None else weights.reshape(-1),
+                         row_src=None if weights is None else perm.perm_src, out=contrib,
+                         token_tile=tile_policy(R, 1, num_experts))
+
+
+def run_experts_int8(w: ExpertWeights, hidden: torch.Tensor | ops.QuantRows, perm: ops.Permutation,
+                     weights: torch.Tensor | None, *, K: int, num_experts: int, expert_begin: int,
+                     contrib: torch.Tensor | None = None, copies: int | None = None) -> torch.Tensor:
+    """Contribution rows of int8 experts: int8 token rows (one scale each)
+    times int8 weights (one scale per channel), the gated activations rounded
+    to bf16 and quantised again for the down projection."""
+    act = int8_gate_up(w, hidden, perm, K=K, num_experts=num_experts, expert_begin=expert_begin, copies=copies)
+    return int8_down(w, act, perm, weights, K=K, num_experts=num_experts, expert_begin=expert_begin,
+                     contrib=contrib)
+
+
+def run_experts_int8_placed(w: ExpertWeights, x: torch.Tensor, offsets: torch.Tensor, *,
+                            tokens: int) -> torch.Tensor:
+    """Expert outputs (no routing weight) of bf16 rows already in expert-major
+    order, ``offsets`` (int32 [n_experts + 1]) their segments; rows past the
+    last segment are neither read nor written. ``tokens``: the rows expected,
+    for the token tile."""
+    R = x.shape[0]
+    bn = tile_policy(tokens, 1, w.n_experts)
+    local = dict(offsets=offsets, expert_lo=0, expert_hi=w.n_experts)
+    act = torch.empty(R, w.i_pad, device=x.device, dtype=torch.bfloat16)
+    ops.int8_gemm(offsets=offsets, expert_begin=0, n_experts=w.n_experts, max_rows=R, planes=2, feat_pad=w.i_pad,
+                  n_feat=w.inter, k_pad=w.h_k, weight=w.w1, weight_scale=w.s1,
+                  rows=ops.act_quant_int8(x, k_pad=w.h_k, **local), epilogue=w.gated_epilogue, bias=w.b1,
+                  alpha=w.alpha, limit=w.limit, out=act, token_tile=bn)
+    y = torch.empty(R, w.hidden, device=x.device, dtype=torch.bfloat16)
+    return ops.int8_gemm(offsets=offsets, expert_begin=0, n_experts=w.n_experts, max_rows=R, planes=1,
+                         feat_pad=w.h_f, n_feat=w.hidden, k_pad=w.i_pad, weight=w.w2, weight_scale=w.s2,
+                         rows=ops.act_quant_int8(act[:, :w.inter], k_pad=w.i_pad, **local),
+                         epilogue=_lib.EPI_DOWN_ONCE, bias=w.b2, out=y, token_tile=bn)
+
+
+def int8_swiglu(w: ExpertWeights, x: torch.Tensor) -> torch.Tensor:
+    """The one expert of ``w`` on every row of bf16 ``x`` [T, H]."""
+    if w.fmt != _lib.W_INT8 or w.n_experts != 1:
+        raise ValueError("int8_swiglu needs the int8 weights of one expert")
+    T = x.shape[0]
+    bn = tile_policy(T, 1, 1, cover=1.0)
+    act = torch.empty(T, w.i_pad, device=x.device, dtype=torch.bfloat16)
+    ops.int8_gemm(offsets=None, expert_begin=0, n_experts=1, max_rows=T, planes=2, feat_pad=w.i_pad, n_feat=w.inter,
+                  k_pad=w.h_k, weight=w.w1, weight_scale=w.s1, rows=ops.act_quant_int8(x, k_pad=w.h_k),
+                  epilogue=w.gated_epilogue, bias=w.b1, alpha=w.alpha, limit=w.limit, out=act, token_tile=bn)
+    y = torch.empty(T, w.hidden, device=x.device, dtype=torch.bfloat16)
+    return ops.int8_gemm(offsets=None, expert_begin=0, n_experts=1, max_rows=T, planes=1, feat_pad=w.h_f,
+                         n_feat=w.hidden, k_pad=w.i_pad, weight=w.w2, weight_scale=w.s2,
+                         rows=ops.act_quant_int8(act[:, :w.inter], k_pad=w.i_pad), epilogue=_lib.EPI_DOWN_ONCE,
+                         bias=w.b2, out=y, token_tile=bn)
+
+
+def int8_linear(w: Int8Linear, x: torch.Tensor | ops.QuantRows, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Dense int8 projection of bf16 rows ``x`` [T, K], or of rows a norm
+    already quantised: bf16 [T, N]."""
+    rows = x if isinstance(x, ops.QuantRows) else None
+    if rows is None:
+        if x.shape[-1] != w.in_features:
+            raise ValueError(f"x has {x.shape[-1]} columns, the projection takes {w.in_features}")
+        rows = ops.act_quant_int8(x, k_pad=w.k_pad)
+    T = rows.q.shape[0]
+    if out is None:
+        out = torch.empty(T, w.out_features, device=w.w.device, dtype=torch.bfloat16)
+    return ops.int8_gemm(offsets=None, expert_begin=0, n_experts=1, max_rows=T, planes=1, feat_pad=w.n_pad,
+                         n_feat=w.out_features, k_pad=w.k_pad, weight=w.w, weight_scale=w.scale, rows=rows,
+                         epilogue=_lib.EPI_DOWN_ONCE, bias=w.bias, out=out, token_tile=tile_policy(T, 1, 1, cover=1.0))
+
+
 def run_experts_w8a8(w: ExpertWeights, hidden: torch.Tensor, perm: ops.Permutation,
                      weights: torch.Tensor | None, *, K: int, num_experts: int, expert_begin: int,
                      contrib: torch.Tensor | None = None,
-                     b_map_div: int | None = None) -> torch.Tensor:
+                     b_map_div: int | None = None, rows: ops.QuantRows | None = None) -> torch.Tensor:
     """``run_experts`` in the reference's efficient FP8 numerics (W8A8,
     moe_serving/efficient_kernels.py:243-274): the routed token rows and the
     gated activations are quantised to e4m3 per (row, 128-column group) and
     multiplied with the e4m3 weights on the tensor cores; FP32 block scales
     of both sides are applied per group in fp32. With ``weights`` the rows
     are bf16(bf16(y) * w); grouped_fp8's own combine takes them unscaled
-    (weights None) and scales them by bf16(w) in the slot-sum combine."""
+    (weights None) and scales them by bf16(w) in the slot-sum combine. ``rows``:
+    the token rows already in that form (a norm's output), which only move to
+    their places then."""
     if w.fmt != _lib.W_FP8 or w.block[1] != 128 or w.block[0] % 64:
         raise ValueError("W8A8 needs FP8 weights with scale blocks of 128 columns (rows a multiple of 64)")
     T, H = hidden.shape
@@ -143,9 +265,12 @@ def run_experts_w8a8(w: ExpertWeights, hidden: torch.Tensor, perm: ops.Permutati
     bn = tile_policy(T, K, num_experts, 128)
     div = K if b_map_div is None else b_map_div
     # only this rank's rows are quantised (other ranks' rows are never read)
-    lo, hi = expert_begin, expert_begin + w.n_experts
-    local = dict(offsets=perm.offsets, expert_lo=lo, expert_hi=hi) if (lo, hi) != (0, num_experts) else {}
-    q, qs = ops.act_quant_fp8(hidden, k_pad=w.h_k, rows_src=perm.perm_src, src_div=div, **local)
+    local = _local_range(w, perm, num_experts, expert_begin)
+    if rows is not None:
+        placed = ops.scatter_rows_8bit(rows.checked(torch.float8_e4m3fn, w.h_k, dev), perm.inverse, div, **local)
+        q, qs = placed.q, placed.scale
+    else:
+        q, qs = ops.act_quant_fp8(hidden, k_pad=w.h_k, rows_src=perm.perm_src, src_div=div, **local)
     act = torch.empty(R, w.i_pad, device=dev, dtype=torch.bfloat16)
     ops.w8a8_gemm(offsets=perm.offsets, expert_begin=expert_begin, n_experts=w.n_experts, max_rows=R,
                   planes=2, feat_pad=w.i_pad, n_feat=w.inter, k_pad=w.h_k, weight=w.w1,
@@ -205,7 +330,8 @@ def check_inputs(hidden: torch.Tensor, indices: torch.Tensor, weights: torch.Ten
 
 def layer_forward(w: ExpertWeights, hidden: torch.Tensor, indices: torch.Tensor,
                   weights: torch.Tensor, *, num_experts: int, expert_begin: int,
-                  parallel=None, numerics: str = "reference") -> torch.Tensor:
+                  parallel=None, numerics: str = "reference",
+                  rows: ops.QuantRows | None = None) -> torch.Tensor:
     """Replicated-token expert layer: the reference's ``ParallelExperts.forward``.
 
     numerics "reference": contributions of all experts reach every rank and
@@ -217,10 +343,22 @@ def layer_forward(w: ExpertWeights, hidden: torch.Tensor, indices: torch.Tensor,
     grouped_fp8 (moe_serving/efficient_kernels.py:243-274) with its fp32
     slot-sum combine; GPT-OSS MXFP4 weights its fused path (grouped_mxfp4,
     :157-206: fp32 epilogues and an fp32 slot-order scatter-reduce); the
-    rank partials of both are all-reduced.
+    rank partials of both are all-reduced. Int8 weights run their int8 products
+    (``run_experts_int8``: routing weights in the down epilogue, an fp32 slot
+    sum, then the all-reduce); they have no other numerics.
+    ``rows``: the tokens in the 8-bit form of the W8A8 FP8 or int8 experts (the
+    norm's second output), which are then not quantised again.
     """
     hidden, indices, weights = check_inputs(hidden, indices, weights)
     T, K = indices.shape
+    if w.fmt == _lib.W_INT8 and numerics != "efficient":
+        raise ValueError(f"int8 experts compute with int8 activations: numerics must be 'efficient', got {numerics!r}")
+    if rows is not None:
+        if numerics != "efficient" or w.fmt not in (_lib.W_FP8, _lib.W_INT8):
+            raise ValueError("quantised rows need the efficient numerics of FP8 or int8 experts")
+        rows.checked(torch.int8 if w.fmt == _lib.W_INT8 else torch.float8_e4m3fn, w.h_k, hidden.device)
+        if rows.q.shape[0] != T:
+            raise ValueError(f"{rows.q.shape[0]} quantised rows for {T} tokens")
     if T == 0:
         return torch.empty_like(hidden)
     size = 1 if parallel is None else parallel.size
@@ -240,12 +378,21 @@ def layer_forward(w: ExpertWeights, hidden: torch.Tensor, indices: torch.Tensor,
         part = run_experts_mxfp4_efficient(w, hidden, perm, weights, indices, K=K,
                                            num_experts=num_experts, expert_begin=expert_begin)
         return part if size == 1 else parallel.reduce(part)
+    if w.fmt == _lib.W_INT8:
+        # rows scaled by the fp32 routing weights before their one rounding,
+        # then summed in fp32
+        y = run_experts_int8(w, hidden if rows is None else rows, perm, weights, K=K, num_experts=num_experts,
+                             expert_begin=expert_begin)
+        part = ops.combine(y, perm.inverse, indices, order=_lib.ORDER_SLOT_SUM, expert_lo=expert_begin,
+                           expert_hi=expert_begin + w.n_experts)
+        return part if size == 1 else parallel.reduce(part)
     if numerics == "efficient" and w.fmt == _lib.W_FP8:
         # W8A8 experts (grouped_fp8) with its local combine: unscaled rows
         # times bf16 routing weights, fp32 sum over each token's slots, one
         # rounding (efficient_kernels.py:269-273), then the all-reduce of the
         # rank partials (:274)
-        y = run_experts_w8a8(w, hidden, perm, None, K=K, num_experts=num_experts, expert_begin=expert_begin)
+        y = run_experts_w8a8(w, hidden, perm, None, K=K, num_experts=num_experts, expert_begin=expert_begin,
+                             rows=rows)
         part = ops.combine(y, perm.inverse, indices, order=_lib.ORDER_SLOT_SUM, expert_lo=expert_begin,
                            expert_hi=expert_begin + w.n_experts, weights=weights)
         return part if size == 1 else parallel.reduce(part)

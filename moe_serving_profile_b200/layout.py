@@ -24,6 +24,12 @@ scale 127 = 2^0).
   FP8 with block scales covering whole 64 x 64 halves, the two fp32 scales of
   rows 0-63 and 64-127 plus 8 zero bytes; other FP8 blocks, 128 x 4 fp32
   (row, 16-column chunk); MXFP4, 128 x 2 ue8m0 bytes (row, 32-column group).
+* Int8 weights (one fp32 scale per output channel) are stored as the 16 KB
+  images the int8 GEMM multiplies from: ``[E_loc][feat_tiles][H_p / 128][128
+  rows][128 columns]`` with ``H_p = ceil(H / 128) * 128``, chunk c of row r at
+  c ^ (r & 7). Rows 32 j + 0..15 of a gated tile are the gate rows and 32 j +
+  16..31 the up rows of features 16 j .. 16 j + 15. Scales and biases are fp32
+  ``[E_loc][feat_tiles][128]`` in the same row order.
 """
 
 from __future__ import annotations
@@ -66,7 +72,7 @@ class ExpertWeights:
 
     @property
     def h_k(self) -> int:
-        return _ceil(self.hidden, 64)
+        return _ceil(self.hidden, 128 if self.fmt == _lib.W_INT8 else 64)
 
     @property
     def h_f(self) -> int:
@@ -196,6 +202,126 @@ def fp8_experts(gate: torch.Tensor, gate_scale: torch.Tensor, up: torch.Tensor,
                          pack_fp8_blobs(w1, s1, 2, inter, (br, bc)),
                          pack_fp8_blobs(w2.unsqueeze(1), s2.unsqueeze(1), 1, hidden, (br, bc)),
                          block=(br, bc))
+
+
+def quantize_int8(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """[..., channels, K] -> int8 of the same shape and fp32 scales [...,
+    channels]: amax / 127 per channel (1 for a channel of zeros), round to
+    nearest even."""
+    w = w.float()
+    scale = w.abs().amax(dim=-1) / 127.0
+    scale = torch.where(scale > 0, scale, torch.ones_like(scale))
+    return torch.round(w / scale[..., None]).clamp_(-127, 127).to(torch.int8), scale
+
+
+def _int8_rows(t: torch.Tensor) -> torch.Tensor:
+    """[planes, F_p, ...] -> [feat_tiles, 128, ...] in the int8 tiles' row
+    order (two planes: 16 gate rows, then the 16 up rows of the same features)."""
+    P, F = t.shape[:2]
+    rest = tuple(t.shape[2:])
+    if P == 2:
+        return t.reshape(2, F // 16, 16, *rest).transpose(0, 1).reshape(F // 64, 128, *rest)
+    return t.reshape(F // 128, 128, *rest)
+
+
+def _int8_tiles(w: torch.Tensor, feat_pad: int, k_pad: int) -> torch.Tensor:
+    """int8 [E, planes, F, K] -> [E, feat_tiles, k_pad / 128, 128, 128] images."""
+    E, P, F, K = w.shape
+    ft = feat_pad // (64 if P == 2 else 128)
+    out = torch.empty(E, ft, k_pad // 128, 128, 128, device=w.device, dtype=torch.int8)
+    chunk = torch.arange(8, device=w.device)
+    for e in range(E):   # one expert at a time bounds the scratch memory
+        full = torch.zeros(P, feat_pad, k_pad, device=w.device, dtype=torch.int8)
+        full[:, :F, :K] = w[e]
+        rows = _int8_rows(full).reshape(ft, 16, 8, k_pad // 128, 8, 16)   # [tile, row / 8, row % 8, block, chunk, 16]
+        dst = out[e].view(ft, k_pad // 128, 16, 8, 8, 16)
+        for r in range(8):
+            dst[:, :, :, r] = rows[:, :, r].index_select(3, chunk ^ r).transpose(1, 2)
+    return out
+
+
+def _int8_channels(v: torch.Tensor | None, feat_pad: int) -> torch.Tensor | None:
+    """fp32 [E, planes, F] -> [E, feat_tiles, 128] in the tiles' row order."""
+    if v is None:
+        return None
+    E, P, F = v.shape
+    full = torch.zeros(E, P, feat_pad, device=v.device, dtype=torch.float32)
+    full[:, :, :F] = v
+    return torch.stack([_int8_rows(full[e]) for e in range(E)])
+
+
+def _check_int8(w: torch.Tensor, scale: torch.Tensor, what: str) -> None:
+    if w.dtype != torch.int8:
+        raise ValueError(f"{what} weights must be int8, got {w.dtype}")
+    if scale.shape != w.shape[:-1]:
+        raise ValueError(f"{what} needs one scale per channel {tuple(w.shape[:-1])}, got {tuple(scale.shape)}")
+
+
+def int8_experts(gate: torch.Tensor, gate_scale: torch.Tensor, up: torch.Tensor, up_scale: torch.Tensor,
+                 down: torch.Tensor, down_scale: torch.Tensor, gate_bias: torch.Tensor | None = None,
+                 up_bias: torch.Tensor | None = None, down_bias: torch.Tensor | None = None,
+                 gated_epilogue: int = _lib.EPI_SWIGLU_F32, alpha: float = 1.702,
+                 limit: float = 7.0) -> ExpertWeights:
+    """gate/up: int8 [E, I, H] with scales [E, I]; down: int8 [E, H, I] with
+    scales [E, H]; biases [E, I] / [E, H]."""
+    E, inter, hidden = gate.shape
+    _check_dims(hidden, inter)
+    for w, s, what in ((gate, gate_scale, "gate"), (up, up_scale, "up"), (down, down_scale, "down")):
+        _check_int8(w, s, what)
+    if up.shape != gate.shape or down.shape != (E, hidden, inter):
+        raise ValueError("gate, up and down shapes disagree")
+    if gated_epilogue not in (_lib.EPI_SWIGLU_F32, _lib.EPI_CLAMP_SWIGLU_F32):
+        raise ValueError("int8 experts gate with SWIGLU_F32 or CLAMP_SWIGLU_F32")
+    if (gate_bias is None) != (up_bias is None):
+        raise ValueError("gate and up biases come together")
+    I_p, H_p = _ceil(inter, 128), _ceil(hidden, 128)
+    b1 = None if gate_bias is None else torch.stack([gate_bias.float(), up_bias.float()], dim=1)
+    b2 = None if down_bias is None else down_bias.float()[:, None]
+    return ExpertWeights(_lib.W_INT8, E, hidden, inter,
+                         _int8_tiles(torch.stack([gate, up], dim=1), I_p, H_p),
+                         _int8_tiles(down[:, None], H_p, I_p),
+                         s1=_int8_channels(torch.stack([gate_scale.float(), up_scale.float()], dim=1), I_p),
+                         s2=_int8_channels(down_scale.float()[:, None], H_p),
+                         b1=_int8_channels(b1, I_p), b2=_int8_channels(b2, H_p),
+                         gated_epilogue=gated_epilogue, alpha=alpha, limit=limit)
+
+
+def int8_experts_from(gate: torch.Tensor, up: torch.Tensor, down: torch.Tensor, **more) -> ExpertWeights:
+    """``int8_experts`` of floating-point weights, quantised per channel."""
+    parts = [t for w in (gate, up, down) for t in quantize_int8(w)]
+    return int8_experts(*parts, **more)
+
+
+@dataclass
+class Int8Linear:
+    """A dense int8 projection [out_features, in_features] in tile layout."""
+
+    out_features: int
+    in_features: int
+    w: torch.Tensor
+    scale: torch.Tensor
+    bias: torch.Tensor | None = None
+
+    @property
+    def n_pad(self) -> int:
+        return _ceil(self.out_features, 128)
+
+    @property
+    def k_pad(self) -> int:
+        return _ceil(self.in_features, 128)
+
+
+def int8_linear(weight: torch.Tensor, scale: torch.Tensor, bias: torch.Tensor | None = None) -> Int8Linear:
+    """int8 weight [N, K] with one scale per output channel [N], bias [N]."""
+    if weight.dim() != 2:
+        raise ValueError("weight must be [out_features, in_features]")
+    _check_int8(weight, scale, "linear")
+    N, K = weight.shape
+    _check_dims(K, N)
+    N_p, K_p = _ceil(N, 128), _ceil(K, 128)
+    return Int8Linear(N, K, _int8_tiles(weight[None, None], N_p, K_p),
+                      _int8_channels(scale.float()[None, None], N_p),
+                      _int8_channels(None if bias is None else bias.float()[None, None], N_p))
 
 
 def bf16_experts(gate: torch.Tensor, up: torch.Tensor, down: torch.Tensor,

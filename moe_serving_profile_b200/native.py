@@ -32,9 +32,10 @@ import torch
 import torch.distributed as dist
 
 from moe_serving_profile_b200 import _lib, ops
-from moe_serving_profile_b200.experts import _max_tile, check_inputs, run_experts, tile_policy
-from moe_serving_profile_b200.layout import ExpertWeights, bf16_experts
-from moe_serving_profile_b200.router import native_route
+from moe_serving_profile_b200.experts import (_max_tile, check_inputs, int8_swiglu, run_experts,
+                                              run_experts_int8_placed, tile_policy)
+from moe_serving_profile_b200.layout import ExpertWeights, bf16_experts, int8_experts_from
+from moe_serving_profile_b200.router import GroupedRouting, native_route
 
 
 # --------------------------------------------------------------------------- collectives
@@ -188,13 +189,21 @@ class RoutingStats:
 
 
 # --------------------------------------------------------------------------- experts
+def _pack_swiglu(gate: torch.Tensor, up: torch.Tensor, down: torch.Tensor, storage: str) -> ExpertWeights:
+    if storage not in ("bf16", "int8"):
+        raise ValueError(f"storage must be 'bf16' or 'int8', got {storage!r}")
+    return (int8_experts_from if storage == "int8" else bf16_experts)(gate, up, down)
+
+
 class LocalSwiGLUExperts(torch.nn.Module):
     """The experts one rank owns (moe_serving/moe.py:58-81): ``gate_up``
     [local_experts, 2 * intermediate, hidden] bf16 with the gate half first,
     ``down`` [local_experts, hidden, intermediate]. The weights are packed
-    once into the grouped GEMM's K-major layout."""
+    once into the grouped GEMM's K-major layout. ``storage="int8"`` quantises
+    them per output channel at that point and computes with int8 activations
+    (experts.run_experts_int8)."""
 
-    def __init__(self, gate_up: torch.Tensor, down: torch.Tensor):
+    def __init__(self, gate_up: torch.Tensor, down: torch.Tensor, storage: str = "bf16"):
         super().__init__()
         if gate_up.dtype != torch.bfloat16 or down.dtype != torch.bfloat16:
             raise ValueError("LocalSwiGLUExperts weights must be bfloat16")
@@ -202,7 +211,7 @@ class LocalSwiGLUExperts(torch.nn.Module):
         self.intermediate = down.shape[2]
         self.num_experts = gate_up.shape[0]
         inter = self.intermediate
-        self.weights = bf16_experts(gate_up[:, :inter], gate_up[:, inter:], down)
+        self.weights = _pack_swiglu(gate_up[:, :inter], gate_up[:, inter:], down, storage)
 
     def forward(self, hidden: torch.Tensor, local_expert_ids: torch.Tensor) -> torch.Tensor:
         """Row i of the result is expert local_expert_ids[i] applied to row i."""
@@ -222,17 +231,18 @@ class SharedSwiGLU(torch.nn.Module):
     bf16. gate / up [I_s, H], down [H, I_s], score [1, H]. The two
     projections run as a one-expert launch of the grouped GEMM over all T rows
     (SwiGLU epilogue, then the down epilogue); the [T, 1] score projection and
-    the final scaling are a GEMV and one elementwise multiply."""
+    the final scaling are a GEMV and one elementwise multiply.
+    ``storage="int8"`` as in LocalSwiGLUExperts."""
 
     def __init__(self, gate: torch.Tensor, up: torch.Tensor, down: torch.Tensor,
-                 score: torch.Tensor):
+                 score: torch.Tensor, storage: str = "bf16"):
         super().__init__()
         for t in (gate, up, down, score):
             if t.dtype != torch.bfloat16:
                 raise ValueError("SharedSwiGLU weights must be bfloat16")
         self.hidden = down.shape[0]
         self.intermediate = down.shape[1]
-        self.weights = bf16_experts(gate[None], up[None], down[None])
+        self.weights = _pack_swiglu(gate[None], up[None], down[None], storage)
         self.score = torch.nn.Parameter(score, requires_grad=False)
 
     def forward(self, hidden: torch.Tensor) -> torch.Tensor:
@@ -241,6 +251,9 @@ class SharedSwiGLU(torch.nn.Module):
             return hidden.new_empty(0, self.hidden)
         w = self.weights
         hidden = hidden.contiguous()
+        if w.fmt == _lib.W_INT8:
+            score = torch.sigmoid(torch.nn.functional.linear(hidden, self.score))
+            return score * int8_swiglu(w, hidden)
         offsets = torch.zeros(2, dtype=torch.int32, device=hidden.device)
         offsets[1] = T
         bn = tile_policy(T, 1, 1)
@@ -310,6 +323,8 @@ def run_experts_received(w, rows: torch.Tensor, offsets: torch.Tensor, *, tile_t
     The token tile follows the global batch (``tile_tokens`` tokens routed
     to ``num_experts`` experts, ``K`` each), as on one GPU."""
     R = rows.shape[0]
+    if w.fmt == _lib.W_INT8:
+        return run_experts_int8_placed(w, rows, offsets, tokens=tile_tokens * K // max(num_experts // w.n_experts, 1))
     bn = tile_policy(tile_tokens, K, num_experts, _max_tile(w))
     act = torch.empty(R, w.i_pad, device=rows.device, dtype=torch.bfloat16)
     ops.expert_gemm(offsets=offsets, expert_begin=0, n_experts=w.n_experts, max_rows=R, wfmt=w.fmt,
@@ -419,12 +434,19 @@ class MoELayer(torch.nn.Module):
     routed launch: every token gets one more slot routed to it (expert E,
     weight sigmoid(hidden . score)), and the ordered combine adds that slot
     last, which is the reference's ``output + shared(hidden)`` bit for bit.
+    ``routing`` (router.GroupedRouting) selects by grouped routing with a
+    balance bias instead of the reference's softmax top-k; ``renormalize`` then
+    is its normalisation.
     """
 
     def __init__(self, gate_weight: torch.Tensor, experts: LocalSwiGLUExperts, plan: ExpertPlan,
                  top_k: int, renormalize: bool = True, shared: SharedSwiGLU | None = None,
-                 collective: Collective | None = None, layer_id: int = 0, logits: str = "exact"):
+                 collective: Collective | None = None, layer_id: int = 0, logits: str = "exact",
+                 routing: GroupedRouting | None = None):
         super().__init__()
+        if routing is not None and logits != "exact":
+            raise ValueError("grouped routing takes its logits from F.linear (logits='exact')")
+        self.routing = routing
         if logits not in ("exact", "fused"):
             raise ValueError(f"logits must be 'exact' or 'fused', got {logits!r}")
         self.logits_mode = logits   # "exact": fp32 F.linear as moe.route does; "fused": fixed-order kernel
@@ -456,8 +478,11 @@ class MoELayer(torch.nn.Module):
     def forward(self, hidden: torch.Tensor) -> tuple[torch.Tensor, RoutingStats]:
         if self.logits_mode == "exact":
             lg = torch.nn.functional.linear(hidden.float(), self.gate_weight.float()).contiguous()
-            out = ops.router(_lib.ROUTER_NATIVE, None, self.gate_weight, None, self.top_k,
-                             self.renormalize, logits=lg)
+            if self.routing is not None:
+                out = self.routing.select(lg, self.top_k, self.renormalize)
+            else:
+                out = ops.router(_lib.ROUTER_NATIVE, None, self.gate_weight, None, self.top_k,
+                                 self.renormalize, logits=lg)
         else:
             out = ops.router(_lib.ROUTER_NATIVE, hidden, self.gate_weight, None, self.top_k,
                              self.renormalize)

@@ -93,6 +93,51 @@ def router(mode: int, hidden: torch.Tensor, weight: torch.Tensor, bias: torch.Te
     return RouterOut(logits_t, probs, scores, indices, counts)
 
 
+def _same_device(t: torch.Tensor | None, device: int, what: str) -> None:
+    if t is not None and (not t.is_cuda or t.device.index != device):
+        raise ValueError(f"{what} must be on cuda:{device}, got {t.device}")
+
+
+SCORING = {"sigmoid": _lib.SCORE_SIGMOID, "softmax": _lib.SCORE_SOFTMAX}
+
+
+def route_grouped(logits: torch.Tensor, bias: torch.Tensor | None, top_k: int, *, n_group: int = 1,
+                  topk_group: int = 1, group_top: int = 2, scoring: str = "sigmoid", normalize: bool = True,
+                  scale: float = 1.0) -> RouterOut:
+    """Expert selection with a balance bias and expert groups
+    (b200moe_route_grouped): ``scoring`` of the fp32 or bf16 ``logits``
+    [T, E], the fp32 ``bias`` [E] added for the selection only, the
+    ``topk_group`` groups of ``n_group`` with the largest sum of their best
+    ``group_top`` keys kept, the ``top_k`` best keys selected (equal keys:
+    the lower id), their scores renormalised and times ``scale``. scores are
+    fp32 [T, K] in descending order of the keys."""
+    device = _dev(logits, "logits")
+    if logits.dtype not in (torch.float32, torch.bfloat16) or logits.dim() != 2 or logits.stride(1) != 1:
+        raise ValueError("logits must be a 2D float32 or bfloat16 tensor with contiguous rows")
+    if scoring not in SCORING:
+        raise ValueError(f"scoring must be one of {tuple(SCORING)}, got {scoring!r}")
+    T, E = logits.shape
+    if bias is not None:
+        _same_device(bias, device, "bias")
+        if bias.dtype != torch.float32 or bias.shape != (E,) or not bias.is_contiguous():
+            raise ValueError(f"bias must be contiguous float32 [{E}]")
+    if not 1 <= top_k <= E:   # before the outputs of that width are allocated
+        raise ValueError(f"top_k must be in [1, {E}], got {top_k}")
+    dev = logits.device
+    scores = torch.empty(T, top_k, device=dev, dtype=torch.float32)
+    indices = torch.empty(T, top_k, device=dev, dtype=torch.int64)
+    counts = torch.empty(E, device=dev, dtype=torch.int32)
+    check(
+        lib.b200moe_route_grouped(
+            device, _stream(device), _ptr(logits), int(logits.dtype == torch.bfloat16),
+            logits.stride(0) if T > 1 else E, _ptr(bias), T, E, top_k, n_group, topk_group, group_top,
+            SCORING[scoring], int(normalize), float(scale), _ptr(scores), _ptr(indices), _ptr(counts),
+        ),
+        "route_grouped",
+    )
+    return RouterOut(logits, None, scores, indices, counts)
+
+
 def route_record(indices: torch.Tensor, scores: torch.Tensor,
                  out_indices: torch.Tensor | None = None,
                  out_scores: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
@@ -150,6 +195,163 @@ def act_quant_fp8(x: torch.Tensor, k_pad: int | None = None, rows_src: torch.Ten
         "act_quant_fp8",
     )
     return q, s
+
+
+@dataclass
+class QuantRows:
+    """Rows in 8 bits with their scales: e4m3 ``q`` [rows, k_pad] with fp32
+    ``scale`` [rows, ceil(k_pad / 128)] (W8A8 FP8 experts) or int8 ``q`` with
+    ``scale`` [rows] (int8 experts and products)."""
+
+    q: torch.Tensor
+    scale: torch.Tensor
+
+    def checked(self, dtype: torch.dtype, k_pad: int, device: torch.device) -> "QuantRows":
+        """Self, if these are ``dtype`` rows of width ``k_pad`` on ``device``."""
+        rows = self.q.shape[0]
+        shape = (rows,) if dtype == torch.int8 else (rows, -(-k_pad // 128))
+        if self.q.dtype != dtype or self.q.dim() != 2 or self.q.shape[1] != k_pad or not self.q.is_contiguous():
+            raise ValueError(f"quantised rows must be contiguous {dtype} [rows, {k_pad}], got {self.q.dtype} "
+                             f"{tuple(self.q.shape)}")
+        if self.scale.dtype != torch.float32 or tuple(self.scale.shape) != shape or not self.scale.is_contiguous():
+            raise ValueError(f"row scales must be contiguous float32 {shape}")
+        if self.q.device != device or self.scale.device != device:
+            raise ValueError(f"quantised rows must be on {device}")
+        return self
+
+
+def _quant_range(offsets, expert_lo: int, expert_hi: int, device: int) -> None:
+    if offsets is not None:
+        _same_device(offsets, device, "offsets")
+        if (offsets.dtype != torch.int32 or not offsets.is_contiguous()
+                or not 0 <= expert_lo <= expert_hi < offsets.numel()):
+            raise ValueError("offsets must be contiguous int32 with 0 <= expert_lo <= expert_hi < offsets.numel()")
+
+
+def _inverse_rows(inverse, rows: int, copies: int, device: int) -> None:
+    _same_device(inverse, device, "inverse")
+    if inverse.dtype != torch.int32 or not inverse.is_contiguous() or inverse.numel() != rows * copies:
+        raise ValueError(f"inverse must be contiguous int32 of rows * copies = {rows * copies} elements")
+
+
+def act_quant_int8(x: torch.Tensor, k_pad: int | None = None, inverse: torch.Tensor | None = None,
+                   copies: int = 1, offsets: torch.Tensor | None = None, expert_lo: int = 0,
+                   expert_hi: int = 0) -> QuantRows:
+    """Int8 rows of bf16 ``x`` with one scale each (amax / 127). With
+    ``inverse`` (a permutation's, int32 [rows * copies]) row r is quantised
+    once and written to each of its ``copies`` places of the permuted order.
+    With ``offsets`` only the places [offsets[expert_lo], offsets[expert_hi])
+    are written."""
+    device = _dev(x, "x")
+    if x.dtype != torch.bfloat16 or x.dim() != 2 or x.stride(1) != 1:
+        raise ValueError("x must be a 2-D bfloat16 tensor with unit column stride")
+    rows, k_valid = x.shape
+    k_pad = -(-k_valid // 128) * 128 if k_pad is None else k_pad
+    rows_out = rows
+    if inverse is not None:
+        _inverse_rows(inverse, rows, copies, device)
+        rows_out = inverse.numel()
+    elif copies != 1:
+        raise ValueError("copies need inverse")
+    _quant_range(offsets, expert_lo, expert_hi, device)
+    q = torch.empty((rows_out, k_pad), device=x.device, dtype=torch.int8)
+    s = torch.empty((rows_out,), device=x.device, dtype=torch.float32)
+    check(
+        lib.b200moe_act_quant_int8(device, _stream(device), _ptr(x), x.stride(0) if rows > 1 else k_valid, rows,
+                                   k_valid, k_pad, _ptr(inverse), copies, rows_out, _ptr(offsets), int(expert_lo),
+                                   int(expert_hi), _ptr(q), _ptr(s)),
+        "act_quant_int8",
+    )
+    return QuantRows(q, s)
+
+
+def scatter_rows_8bit(rows: QuantRows, inverse: torch.Tensor, copies: int, offsets: torch.Tensor | None = None,
+                      expert_lo: int = 0, expert_hi: int = 0) -> QuantRows:
+    """Quantised token rows at their ``copies`` places each of the permuted
+    order (``inverse``: a permutation's); with ``offsets`` only the places
+    [offsets[expert_lo], offsets[expert_hi])."""
+    device = _dev(rows.q, "rows")
+    rows = rows.checked(rows.q.dtype, rows.q.shape[1], rows.q.device)
+    if rows.q.dtype not in (torch.int8, torch.float8_e4m3fn):
+        raise ValueError(f"rows must be int8 or float8_e4m3fn, got {rows.q.dtype}")
+    n, width = rows.q.shape
+    _inverse_rows(inverse, n, copies, device)
+    _quant_range(offsets, expert_lo, expert_hi, device)
+    R = inverse.numel()
+    groups = rows.scale.numel() // max(n, 1) or 1
+    q = torch.empty((R, width), device=rows.q.device, dtype=rows.q.dtype)
+    s = torch.empty((R,) + tuple(rows.scale.shape[1:]), device=rows.q.device, dtype=torch.float32)
+    check(
+        lib.b200moe_scatter_rows_8bit(device, _stream(device), _ptr(rows.q), width, _ptr(rows.scale), groups, n,
+                                      _ptr(inverse), copies, R, _ptr(offsets), int(expert_lo), int(expert_hi),
+                                      _ptr(q), _ptr(s)),
+        "scatter_rows_8bit",
+    )
+    return QuantRows(q, s)
+
+
+# --------------------------------------------------------------------------- norm
+@dataclass
+class NormOut:
+    out: torch.Tensor | None        # bf16 [T, H]: the normed rows
+    residual: torch.Tensor | None   # bf16 [T, H]: x + residual (None without a residual)
+    rows: QuantRows | None          # the normed rows in 8 bits
+
+
+QUANT = {None: _lib.QUANT_NONE, "fp8": _lib.QUANT_FP8, "int8": _lib.QUANT_INT8}
+
+
+def add_rmsnorm(x: torch.Tensor, weight: torch.Tensor, eps: float, *, residual: torch.Tensor | None = None,
+                residual_out: torch.Tensor | None = None, quant: str | None = None, k_pad: int | None = None,
+                normed: bool = True) -> NormOut:
+    """RMS norm of bf16 rows ``x`` [T, H], or of their sum with ``residual``
+    (b200moe_add_rmsnorm). The sum is written to ``residual_out`` (a new
+    tensor by default; ``residual`` itself for an update in place). ``quant``
+    "fp8" or "int8" also returns the normed rows in the 8-bit form of the W8A8
+    FP8 or the int8 experts, padded to ``k_pad`` columns (default: what those
+    experts take); ``normed=False`` leaves the bf16 output out."""
+    device = _dev(x, "x")
+    _bf16_rows(x, "x")
+    if quant not in QUANT:
+        raise ValueError(f"quant must be one of {tuple(QUANT)}, got {quant!r}")
+    T, H = x.shape
+    if weight.dtype not in (torch.bfloat16, torch.float32) or weight.shape != (H,) or not weight.is_contiguous():
+        raise ValueError(f"weight must be contiguous bfloat16 or float32 [{H}]")
+    _same_device(weight, device, "weight")
+    if quant is None and not normed:
+        raise ValueError("nothing to compute: no quantised rows and no bf16 output")
+    for t, what in ((residual, "residual"), (residual_out, "residual_out")):
+        if t is not None:
+            _bf16_rows(t, what)
+            _same_device(t, device, what)
+            if t.shape != x.shape:
+                raise ValueError(f"{what} must have x's shape {tuple(x.shape)}, got {tuple(t.shape)}")
+    if residual is None and residual_out is not None:
+        raise ValueError("residual_out needs a residual")
+    if residual is not None and residual_out is None:
+        residual_out = torch.empty(T, H, device=x.device, dtype=torch.bfloat16)
+    out = torch.empty(T, H, device=x.device, dtype=torch.bfloat16) if normed else None
+    rows = None
+    if quant is not None:
+        if k_pad is None:
+            k_pad = -(-H // 64) * 64 if quant == "fp8" else -(-H // 128) * 128
+        dtype = torch.float8_e4m3fn if quant == "fp8" else torch.int8
+        shape = (T, -(-k_pad // 128)) if quant == "fp8" else (T,)
+        rows = QuantRows(torch.empty((T, k_pad), device=x.device, dtype=dtype),
+                         torch.empty(shape, device=x.device, dtype=torch.float32))
+
+    def ld(t):
+        return 0 if t is None else (t.stride(0) if T > 1 else H)
+
+    check(
+        lib.b200moe_add_rmsnorm(
+            device, _stream(device), _ptr(x), ld(x), _ptr(residual), ld(residual), _ptr(residual_out),
+            ld(residual_out), _ptr(weight), int(weight.dtype == torch.float32), float(eps), T, H, _ptr(out), ld(out),
+            QUANT[quant], _ptr(rows.q) if rows else None, k_pad if rows else 0, _ptr(rows.scale) if rows else None,
+        ),
+        "add_rmsnorm",
+    )
+    return NormOut(out, residual_out, rows)
 
 
 # --------------------------------------------------------------------------- permutation
@@ -336,6 +538,65 @@ def w8a8_gemm(*, offsets: torch.Tensor, expert_begin: int, n_experts: int, max_r
     a.ldo = out.stride(0)
     check(lib.b200moe_w8a8_gemm(device, _stream(device), ctypes.byref(a), _ptr(q), _ptr(q_scale)),
           "w8a8_gemm")
+    return out
+
+
+def int8_gemm(*, offsets: torch.Tensor | None, expert_begin: int, n_experts: int, max_rows: int, planes: int,
+              feat_pad: int, n_feat: int, k_pad: int, weight: torch.Tensor, weight_scale: torch.Tensor,
+              rows: QuantRows, epilogue: int, bias: torch.Tensor | None = None, alpha: float = 1.702,
+              limit: float = 7.0, row_weight: torch.Tensor | None = None, row_src: torch.Tensor | None = None,
+              out: torch.Tensor, token_tile: int = 0) -> torch.Tensor:
+    """Int8 grouped GEMM (b200moe_int8_gemm): int8 weight tiles with one fp32
+    scale per channel times int8 permuted rows with one scale each
+    (``act_quant_int8``'s outputs). ``offsets`` None: one expert holds all
+    ``max_rows`` rows."""
+    device = _dev(weight, "weight")
+    _bf16_rows(out, "output")
+    rows = rows.checked(torch.int8, k_pad, weight.device)
+    tiles = n_experts * (feat_pad // (64 if planes == 2 else 128))
+    if weight.dtype != torch.int8 or not weight.is_contiguous() or weight.numel() != tiles * 128 * k_pad:
+        raise ValueError(f"weight must be contiguous int8 tiles of {tiles * 128 * k_pad} elements")
+    for t, what in ((weight_scale, "weight_scale"), (bias, "bias")):
+        if t is not None and (t.dtype != torch.float32 or not t.is_contiguous() or t.numel() != tiles * 128
+                              or t.device != weight.device):
+            raise ValueError(f"{what} must be contiguous float32 of {tiles * 128} elements on {weight.device}")
+    if out.device != weight.device or out.shape[0] < max_rows or out.shape[1] < n_feat:
+        raise ValueError(f"output must hold {max_rows} rows of {n_feat} columns on {weight.device}")
+    if offsets is not None:
+        _same_device(offsets, device, "offsets")
+        if offsets.dtype != torch.int32 or not offsets.is_contiguous() or offsets.numel() <= expert_begin + n_experts:
+            raise ValueError("offsets must be contiguous int32 covering the experts")
+    a = _lib.GemmArgs()
+    a.offsets = _ptr(offsets)
+    a.expert_begin = expert_begin
+    a.n_experts = n_experts
+    a.max_rows = max_rows
+    a.token_tile = token_tile
+    a.wfmt = _lib.W_INT8
+    a.planes = planes
+    a.feat_pad = feat_pad
+    a.n_feat = n_feat
+    a.k_pad = k_pad
+    a.weight = _ptr(weight)
+    a.b_rows = rows.q.shape[0]
+    a.b_div = 1
+    a.epilogue = epilogue
+    a.alpha = alpha
+    a.limit = limit
+    if row_weight is not None:
+        _same_device(row_weight, device, "row_weight")
+        _same_device(row_src, device, "row_src")
+        if row_weight.dtype not in (torch.float32, torch.bfloat16) or not row_weight.is_contiguous():
+            raise ValueError("row_weight must be contiguous float32 or bfloat16")
+        if row_src is None or row_src.dtype != torch.int32 or row_src.numel() < max_rows:
+            raise ValueError("row_weight needs row_src (int32, one entry per row)")
+        a.row_weight = _ptr(row_weight)
+        a.row_weight_bf16 = int(row_weight.dtype == torch.bfloat16)
+        a.row_src = _ptr(row_src)
+    a.out = _ptr(out)
+    a.ldo = out.stride(0) if out.shape[0] > 1 else out.shape[1]
+    check(lib.b200moe_int8_gemm(device, _stream(device), ctypes.byref(a), _ptr(rows.q), _ptr(rows.scale),
+                                _ptr(weight_scale), _ptr(bias)), "int8_gemm")
     return out
 
 

@@ -8,7 +8,8 @@ fills with ``ExpertProjection(weight, scales, block_size)`` for ``gate_proj``,
 no scales), and ``forward(hidden [T,H] bf16, indices [T,K] int64 global ids,
 weights [T,K] fp32) -> [T,H] bf16`` already reduced over the EP group.
 ``numerics="efficient"`` runs the W8A8 experts of the reference's
-grouped_fp8 (moe_serving/efficient_kernels.py:243-274).
+grouped_fp8 (moe_serving/efficient_kernels.py:243-274), or, for int8 weights
+with channel scales, their int8 products.
 
 On the first forward (or an explicit ``prepare()``) the per-expert modules
 are packed into the device layout of :mod:`layout` and released, as the
@@ -29,7 +30,8 @@ NUMERICS = ("reference", "fast", "efficient")
 
 class ExpertProjection(nn.Module):
     """One projection's storage: weight [out, in] (e4m3 or bf16), optional fp32
-    block scales [ceil(out/br), ceil(in/bc)] (moe_serving/qwen3_parallel.py:56-70)."""
+    block scales [ceil(out/br), ceil(in/bc)] (moe_serving/qwen3_parallel.py:56-70).
+    An int8 weight has one fp32 scale per output channel, [out]."""
 
     def __init__(self, weight, scales=None, block_size=(128, 128)):
         super().__init__()
@@ -70,7 +72,14 @@ class ParallelExperts(nn.Module):
         gw = torch.stack([p.weight for p in g])
         uw = torch.stack([p.weight for p in u])
         dw = torch.stack([p.weight for p in d])
-        if g[0].scales is not None:
+        if g[0].weight.dtype == torch.int8:
+            if self.numerics != "efficient":
+                raise ValueError("int8 experts compute with int8 activations: numerics must be 'efficient'")
+            if any(p.scales is None or p.weight.dtype != torch.int8 for p in g + u + d):
+                raise ValueError("all int8 projections need int8 weights and channel scales")
+            gs, us, ds = (torch.stack([p.scales.reshape(-1) for p in ps]) for ps in projs)
+            self.packed = layout.int8_experts(gw, gs, uw, us, dw, ds)
+        elif g[0].scales is not None:
             blocks = {p.block_size for p in g + u + d}
             if len(blocks) != 1 or any(p.scales is None for p in g + u + d):
                 raise ValueError("all FP8 projections need scales with one block size")
@@ -83,8 +92,10 @@ class ParallelExperts(nn.Module):
         self.local = None
         return self.packed
 
-    def forward(self, hidden, indices, weights):
+    def forward(self, hidden, indices, weights, rows=None):
+        """``rows``: the tokens already in the 8-bit form of the efficient
+        numerics (norm.AddRMSNorm's ``rows``)."""
         w = self.prepare()
         return _experts.layer_forward(w, hidden, indices, weights,
                                       num_experts=self.global_experts, expert_begin=self.start,
-                                      parallel=self.parallel, numerics=self.numerics)
+                                      parallel=self.parallel, numerics=self.numerics, rows=rows)

@@ -31,6 +31,8 @@ different kernel, and summation order, for a slice.
 
 from __future__ import annotations
 
+from dataclasses import dataclass
+
 import torch
 import torch.distributed as dist
 import torch.nn.functional as F
@@ -144,6 +146,76 @@ class GptOssRouter(nn.Module):
                                                  self.top_k, False, self.parallel, self.logits_mode)
         self.last_counts = counts
         return logits, scores, indices
+
+
+@dataclass
+class GroupedRouting:
+    """How grouped routing selects (ops.route_grouped): ``n_group`` groups of
+    consecutive experts, of which the ``topk_group`` with the largest sum of
+    their best ``group_top`` keys stay; ``bias`` (fp32 [E] or None) is added to
+    the scores for the selection only; ``scale`` multiplies the weights."""
+
+    n_group: int = 1
+    topk_group: int = 1
+    group_top: int = 2
+    scoring: str = "sigmoid"
+    scale: float = 1.0
+    bias: torch.Tensor | None = None
+
+    def select(self, logits: torch.Tensor, top_k: int, normalize: bool) -> ops.RouterOut:
+        return ops.route_grouped(logits, self.bias, top_k, n_group=self.n_group, topk_group=self.topk_group,
+                                 group_top=self.group_top, scoring=self.scoring, normalize=normalize,
+                                 scale=self.scale)
+
+
+class GroupedRouter(nn.Module):
+    """Router with sigmoid or softmax scores, a balance bias and expert groups
+    (ops.route_grouped). Returns (logits [T,E], scores fp32 [T,K], indices
+    int64 [T,K]), the module interface of the routers above.
+
+    config: ``num_experts``, ``num_experts_per_tok``, ``hidden_size`` and, with
+    these defaults, ``n_group`` 1, ``topk_group`` 1, ``group_top`` 2,
+    ``scoring_func`` "sigmoid", ``norm_topk_prob`` True and
+    ``routed_scaling_factor`` 1.0. ``balance_bias`` (fp32 [E]) starts at zero.
+    logits "fp32" (default): F.linear of fp32 copies, so that close experts
+    are not tied by a bf16 logit; "exact": F.linear in the hidden type, as the
+    other routers."""
+
+    def __init__(self, config, logits: str = "fp32"):
+        super().__init__()
+        if logits not in ("fp32", "exact"):
+            raise ValueError(f"logits must be 'fp32' or 'exact', got {logits!r}")
+        self.logits_mode = logits
+        self.top_k = config.num_experts_per_tok
+        self.num_experts = config.num_experts
+        self.hidden_dim = config.hidden_size
+        self.norm_topk_prob = bool(getattr(config, "norm_topk_prob", True))
+        self.weight = nn.Parameter(torch.zeros(self.num_experts, self.hidden_dim), requires_grad=False)
+        self.balance_bias = nn.Parameter(torch.zeros(self.num_experts, dtype=torch.float32), requires_grad=False)
+        self.n_group = getattr(config, "n_group", 1)
+        self.topk_group = getattr(config, "topk_group", 1)
+        self.group_top = getattr(config, "group_top", 2)
+        self.scoring = getattr(config, "scoring_func", "sigmoid")
+        self.scale = float(getattr(config, "routed_scaling_factor", 1.0))
+        if self.num_experts % self.n_group:
+            raise ValueError(f"{self.num_experts} experts do not divide into {self.n_group} groups")
+        if self.scoring not in ops.SCORING:
+            raise ValueError(f"scoring_func must be one of {tuple(ops.SCORING)}, got {self.scoring!r}")
+        self.last_counts: torch.Tensor | None = None
+
+    def forward(self, hidden_states: torch.Tensor):
+        h = hidden_states.reshape(-1, self.hidden_dim)
+        if not h.is_cuda:
+            raise ValueError(f"hidden states must be a CUDA tensor (b200moe has no CPU path), got {h.device}")
+        if self.logits_mode == "fp32":
+            logits = F.linear(h.float(), self.weight.float())
+        else:
+            logits = F.linear(h, self.weight.to(h.dtype))
+        out = ops.route_grouped(logits, self.balance_bias.float(), self.top_k, n_group=self.n_group,
+                                topk_group=self.topk_group, group_top=self.group_top, scoring=self.scoring,
+                                normalize=self.norm_topk_prob, scale=self.scale)
+        self.last_counts = out.counts
+        return out.logits, out.scores, out.indices
 
 
 def native_route(hidden: torch.Tensor, gate_weight: torch.Tensor, top_k: int,
