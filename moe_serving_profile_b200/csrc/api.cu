@@ -183,7 +183,8 @@ int b200moe_route_grouped(int device, void* stream, const void* logits, int logi
   int rc = use_device(device, nullptr);
   if (rc) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (counts) B200_CUDA(cudaMemsetAsync(counts, 0, sizeof(int) * E, st));
+  const int blocks = b200::route_grouped_blocks(T, g_sm_count[device]);
+  if (counts && blocks != 1) B200_CUDA(cudaMemsetAsync(counts, 0, sizeof(int) * E, st));
   if (T == 0) return B200MOE_OK;
   b200::RouteParams p{};
   p.logits = logits;
@@ -203,7 +204,7 @@ int b200moe_route_grouped(int device, void* stream, const void* logits, int logi
   p.scores = scores;
   p.indices = indices;
   p.counts = counts;
-  B200_CUDA(b200::launch_route_grouped(st, p));
+  B200_CUDA(b200::launch_route_grouped(st, p, blocks));
   return B200MOE_OK;
 }
 

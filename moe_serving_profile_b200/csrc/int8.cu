@@ -87,16 +87,17 @@ __device__ __forceinline__ float row_weight(const Int8Params& p, int row) {
                       : reinterpret_cast<const float*>(p.row_w)[src];
 }
 
-__device__ __forceinline__ float gated(const Int8Params& p, float g, float u) {
-  float a = 1.f;
-  if (p.epi == kEpiClampF32) {
-    g = g > p.limit ? p.limit : g;
-    u = u < -p.limit ? -p.limit : (u > p.limit ? p.limit : u);
-    u += 1.f;
-    a = p.alpha;
-  }
-  return g / (1.f + expf(-a * g)) * u;
+// g / (1 + exp(-a g)) * u with the hardware exp2 and reciprocal: off by
+// |a g| + 8 steps of 2^-23 at most, far inside the bf16 rounding that follows.
+// Infinite exponentials give 0, NaN stays NaN.
+__device__ __forceinline__ float glu(float g, float u, float nlog) {   // nlog = -a log2(e)
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * nlog));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+  return g * r * u;
 }
+
+__device__ __forceinline__ uint16_t bf16_bits(float f) { return __bfloat16_as_ushort(__float2bfloat16_rn(f)); }
 
 template <int BN>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -233,6 +234,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t tq = tmem + (static_cast<uint32_t>(q * 32) << 16);
     float* xs = reinterpret_cast<float*>(sbase + p.x_off);   // [2 tiles][row scales BN | row weights BN]
     const bool is_gate = lane < 16;
+    const float nlog = -1.44269504f * (p.epi == kEpiClampF32 ? p.alpha : 1.f);
     int tc = 0;
     for (int t = blockIdx.x; t < total; t += gridDim.x) {
       const Tile tl = decode_tile<BN>(t, prefix, p);
@@ -261,22 +263,47 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int j = 0; j < 16; ++j)
           d[j] = fmaf(static_cast<float>(static_cast<int>(v[j])), sa[c0 + j] * ws, bias);
+        const bool whole = c0 + 16 <= tl.nrows;
         if (p.gated) {
+          // gate lanes take the even columns, up lanes the odd ones
+          float g[8], u[8];
 #pragma unroll
-          for (int j = 0; j < 16; j += 2) {
-            // gate lanes keep column j, up lanes column j + 1
-            const float got = __shfl_xor_sync(kFull, is_gate ? d[j + 1] : d[j], 16);
-            const float y = is_gate ? gated(p, d[j], got) : gated(p, got, d[j + 1]);
-            const int n = c0 + j + (is_gate ? 0 : 1);
-            if (n < tl.nrows && f < p.n_feat)
-              out[(long long)n * p.ldo] = static_cast<uint16_t>(__bfloat16_as_ushort(__float2bfloat16_rn(y)));
+          for (int j = 0; j < 8; ++j) {
+            const float got = __shfl_xor_sync(kFull, is_gate ? d[2 * j + 1] : d[2 * j], 16);
+            g[j] = is_gate ? d[2 * j] : got;
+            u[j] = is_gate ? got : d[2 * j + 1];
+          }
+          if (p.epi == kEpiClampF32) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              g[j] = g[j] > p.limit ? p.limit : g[j];
+              u[j] = (u[j] < -p.limit ? -p.limit : (u[j] > p.limit ? p.limit : u[j])) + 1.f;
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j) g[j] = glu(g[j], u[j], nlog);
+          const int n0 = c0 + (is_gate ? 0 : 1);
+          uint16_t* o = out + n0 * p.ldo;
+          if (f < p.n_feat) {
+            if (whole) {
+#pragma unroll
+              for (int j = 0; j < 8; ++j) o[2 * j * p.ldo] = bf16_bits(g[j]);
+            } else {
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                if (n0 + 2 * j < tl.nrows) o[2 * j * p.ldo] = bf16_bits(g[j]);
+            }
           }
         } else if (f < p.n_feat) {
+          uint16_t* o = out + c0 * p.ldo;
+          if (whole) {
 #pragma unroll
-          for (int j = 0; j < 16; ++j)
-            if (c0 + j < tl.nrows)
-              out[(long long)(c0 + j) * p.ldo] =
-                  static_cast<uint16_t>(__bfloat16_as_ushort(__float2bfloat16_rn(d[j] * rw[c0 + j])));
+            for (int j = 0; j < 16; ++j) o[j * p.ldo] = bf16_bits(d[j] * rw[c0 + j]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              if (c0 + j < tl.nrows) o[j * p.ldo] = bf16_bits(d[j] * rw[c0 + j]);
+          }
         }
       }
       tc_fence_before();
