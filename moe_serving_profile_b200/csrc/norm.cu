@@ -14,7 +14,12 @@
 // infinity: a row that holds one gets a NaN or infinite scale and its products
 // come out NaN instead of plausible.
 //
-// One block per row, the row in registers between the passes.
+// Bound by memory: one block per row holds it in registers between the passes
+// (V vectors of 8 columns per thread), all its loads issued before the first
+// use. Quotients by the row's or group's scale are correctly rounded by
+// Markstein's method (a rounded reciprocal, then two remainder steps): five
+// multiply-adds a value, where a general division took most of the time of
+// an earlier form of these kernels.
 #include "internal.h"
 #include "ptx.cuh"
 
@@ -22,7 +27,6 @@ namespace b200 {
 namespace {
 
 constexpr unsigned kFull = 0xffffffffu;
-constexpr int kVec = 4;   // 16-byte vectors per thread
 
 __device__ __forceinline__ void unpack8(const uint4& v, float (&f)[8]) {
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -33,14 +37,38 @@ __device__ __forceinline__ void unpack8(const uint4& v, float (&f)[8]) {
   }
 }
 
+__device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
+  return make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]),
+                    pack_bf16x2(f[6], f[7]));
+}
+
 __device__ __forceinline__ uint32_t mag(float f) { return __float_as_uint(f) & 0x7fffffffu; }
 
-// amax / top, or 1 where that is zero (a row or group of zeros, or of values
-// so small that the quotient underflows: they quantise to 0).
-__device__ __forceinline__ float scale_of(uint32_t amax, float top) {
-  const float s = __fdiv_rn(__uint_as_float(amax), top);
-  return s == 0.f ? 1.f : s;
+__device__ __forceinline__ uint32_t mag_max(const float (&f)[8], uint32_t m) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) m = max(m, mag(f[j]));
+  return m;
 }
+
+// Division by one scale: s = amax / top, or 1 where that is zero (a row or
+// group of zeros, or of values so small that the quotient underflows: they
+// quantise to 0).
+struct Divider {
+  float s, r, top;
+  bool plain;   // magnitudes at which the remainder steps could underflow, infinity and NaN
+  __device__ __forceinline__ Divider(uint32_t amax, float top_) : top(top_) {
+    s = __fdiv_rn(__uint_as_float(amax), top);
+    s = s == 0.f ? 1.f : s;
+    r = __frcp_rn(s);
+    plain = !(s > 0x1p-80f && s < 0x1p125f);
+  }
+  __device__ __forceinline__ float operator()(float x) const {
+    if (plain) return fminf(fmaxf(__fdiv_rn(x, s), -top), top);   // a subnormal scale may be short of amax / top
+    float t = x * r;
+    t = fmaf(fmaf(-t, s, x), r, t);
+    return fmaf(fmaf(-t, s, x), r, t);
+  }
+};
 
 __device__ __forceinline__ uint32_t e4m3x2_rn(float x0, float x1) {
   uint16_t r;
@@ -48,23 +76,26 @@ __device__ __forceinline__ uint32_t e4m3x2_rn(float x0, float x1) {
   return r;
 }
 
-__device__ __forceinline__ uint32_t s8_rn(float x) {
-  int r;
-  asm("cvt.rni.sat.s8.f32 %0, %1;" : "=r"(r) : "f"(x));
-  return static_cast<uint32_t>(r) & 0xffu;
+__device__ __forceinline__ uint2 pack_e4m3(const float (&y)[8], const Divider& d) {
+  return make_uint2(e4m3x2_rn(d(y[0]), d(y[1])) | (e4m3x2_rn(d(y[2]), d(y[3])) << 16),
+                    e4m3x2_rn(d(y[4]), d(y[5])) | (e4m3x2_rn(d(y[6]), d(y[7])) << 16));
 }
 
-__device__ __forceinline__ uint2 pack_s8(const float (&y)[8], float s) {
-  uint2 o;
-  o.x = s8_rn(__fdiv_rn(y[0], s)) | (s8_rn(__fdiv_rn(y[1], s)) << 8) | (s8_rn(__fdiv_rn(y[2], s)) << 16) |
-        (s8_rn(__fdiv_rn(y[3], s)) << 24);
-  o.y = s8_rn(__fdiv_rn(y[4], s)) | (s8_rn(__fdiv_rn(y[5], s)) << 8) | (s8_rn(__fdiv_rn(y[6], s)) << 16) |
-        (s8_rn(__fdiv_rn(y[7], s)) << 24);
-  return o;
+// Four values of at most 127 in magnitude to int8, nearest even: adding
+// 1.5 * 2^23 leaves the integer in the sum's low byte.
+__device__ __forceinline__ uint32_t s8x4(float a, float b, float c, float e) {
+  constexpr float kMagic = 12582912.f;
+  const uint32_t ab = __byte_perm(__float_as_uint(a + kMagic), __float_as_uint(b + kMagic), 0x0040);
+  const uint32_t ce = __byte_perm(__float_as_uint(c + kMagic), __float_as_uint(e + kMagic), 0x0040);
+  return __byte_perm(ab, ce, 0x5410);
 }
 
-// Sum / maximum over the block; every thread gets the result. `buf` holds 33
-// words and is free again after the call's last barrier.
+__device__ __forceinline__ uint2 pack_s8(const float (&y)[8], const Divider& d) {
+  return make_uint2(s8x4(d(y[0]), d(y[1]), d(y[2]), d(y[3])), s8x4(d(y[4]), d(y[5]), d(y[6]), d(y[7])));
+}
+
+// Sum / maximum over the block; every thread gets the result. `buf` (32 words)
+// serves one call.
 __device__ __forceinline__ float block_sum(float v, float* buf) {
 #pragma unroll
   for (int o = 16; o >= 1; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
@@ -87,32 +118,39 @@ __device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t* buf) {
   return __reduce_max_sync(kFull, (threadIdx.x & 31) < nw ? buf[threadIdx.x & 31] : 0u);
 }
 
-__global__ void __launch_bounds__(1024) add_rmsnorm_kernel(const NormParams p) {
+template <int V>
+__global__ void __launch_bounds__(V == 4 ? 1024 : 256) add_rmsnorm_kernel(const NormParams p) {
   __shared__ float sum_buf[32];
   __shared__ uint32_t max_buf[32];
   const long long t = blockIdx.x;
   const int nvec = p.H >> 3;
   const uint4* x = reinterpret_cast<const uint4*>(p.x + t * p.ldx);
   const uint4* r = p.res ? reinterpret_cast<const uint4*>(p.res + t * p.ldr) : nullptr;
-  uint4 h[kVec];
+  uint4 h[V], add[V], wv[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int v = threadIdx.x + i * blockDim.x;
+    h[i] = add[i] = wv[i] = make_uint4(0, 0, 0, 0);
+    if (v < nvec) {
+      h[i] = x[v];
+      if (r) add[i] = r[v];
+      if (!p.weight_f32) wv[i] = __ldg(reinterpret_cast<const uint4*>(p.weight) + v);
+    }
+  }
   float sq = 0.f;
 #pragma unroll
-  for (int i = 0; i < kVec; ++i) {
+  for (int i = 0; i < V; ++i) {
     const int v = threadIdx.x + i * blockDim.x;
-    h[i] = make_uint4(0, 0, 0, 0);
-    if (v >= nvec) continue;
-    h[i] = x[v];
     float f[8];
     unpack8(h[i], f);
     if (r) {
       float g[8];
-      unpack8(r[v], g);
+      unpack8(add[i], g);
 #pragma unroll
       for (int j = 0; j < 8; ++j) f[j] += g[j];
-      h[i] = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]),
-                        pack_bf16x2(f[6], f[7]));
+      h[i] = pack8(f);
       unpack8(h[i], f);
-      if (p.res_out) reinterpret_cast<uint4*>(p.res_out + t * p.ldro)[v] = h[i];
+      if (p.res_out && v < nvec) reinterpret_cast<uint4*>(p.res_out + t * p.ldro)[v] = h[i];
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) sq = fmaf(f[j], f[j], sq);
@@ -120,129 +158,128 @@ __global__ void __launch_bounds__(1024) add_rmsnorm_kernel(const NormParams p) {
   const float mean = block_sum(sq, sum_buf) / static_cast<float>(p.H);
   const float rstd = 1.f / sqrtf(mean + p.eps);
 
-  uint32_t amax = 0;
-  float y[kVec][8];
-#pragma unroll
-  for (int i = 0; i < kVec; ++i) {
+  auto normed = [&](int i, float (&y)[8]) {   // zeros past the row's end
     const int v = threadIdx.x + i * blockDim.x;
-    unpack8(h[i], y[i]);
-    if (v < nvec) {
-      float w[8];
-      if (p.weight_f32) {
-        const float4 a = reinterpret_cast<const float4*>(p.weight)[2 * v];
-        const float4 b = reinterpret_cast<const float4*>(p.weight)[2 * v + 1];
-        w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
-        w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
-      } else {
-        unpack8(reinterpret_cast<const uint4*>(p.weight)[v], w);
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        y[i][j] = y[i][j] * rstd * w[j];
-        amax = max(amax, mag(y[i][j]));
-      }
-      if (p.out)
-        reinterpret_cast<uint4*>(p.out + t * p.ldo)[v] =
-            make_uint4(pack_bf16x2(y[i][0], y[i][1]), pack_bf16x2(y[i][2], y[i][3]), pack_bf16x2(y[i][4], y[i][5]),
-                       pack_bf16x2(y[i][6], y[i][7]));
+    float w[8];
+    unpack8(h[i], y);
+    if (p.weight_f32) {
+      if (v >= nvec) return;
+      const float4 a = __ldg(reinterpret_cast<const float4*>(p.weight) + 2 * v);
+      const float4 b = __ldg(reinterpret_cast<const float4*>(p.weight) + 2 * v + 1);
+      w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
+      w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
+    } else {
+      unpack8(wv[i], w);
     }
-  }
-  if (p.quant == 0) return;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) y[j] = y[j] * rstd * w[j];
+  };
   uint2* q = reinterpret_cast<uint2*>(p.q + t * p.k_pad);
   const int npad = p.k_pad >> 3;
-  if (p.quant == 2) {   // int8, one scale per row
-    amax = block_max(amax, max_buf);
-    const float s = scale_of(amax, 127.f);
-    if (threadIdx.x == 0) p.scale[t] = s;
+  if (p.quant != 2) {
+    // e4m3, one scale per 128 columns: 16 neighbouring threads hold a group
+    const int groups = (p.k_pad + 127) >> 7;
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) {
+    for (int i = 0; i < V; ++i) {
       const int v = threadIdx.x + i * blockDim.x;
-      if (v < nvec) q[v] = pack_s8(y[i], s);
+      float y[8];
+      normed(i, y);
+      if (p.out && v < nvec) reinterpret_cast<uint4*>(p.out + t * p.ldo)[v] = pack8(y);
+      if (p.quant == 0) continue;
+      uint32_t m = v < nvec ? mag_max(y, 0) : 0u;
+#pragma unroll
+      for (int o = 8; o >= 1; o >>= 1) m = max(m, __shfl_xor_sync(kFull, m, o));
+      const Divider d(m, 448.f);
+      if (v < nvec) q[v] = pack_e4m3(y, d);
+      else if (v < npad) q[v] = make_uint2(0, 0);
+      if ((v & 15) == 0 && (v >> 4) < groups) p.scale[t * groups + (v >> 4)] = d.s;
     }
-    for (int v = nvec + threadIdx.x; v < npad; v += blockDim.x) q[v] = make_uint2(0, 0);
+    if (p.quant == 0) return;
+    // columns and groups past the vectors that the threads hold
+    for (int v = V * blockDim.x + threadIdx.x; v < npad; v += blockDim.x) {
+      q[v] = make_uint2(0, 0);
+      if ((v & 15) == 0) p.scale[t * groups + (v >> 4)] = 1.f;
+    }
     return;
   }
-  // e4m3, one scale per 128 columns: 16 neighbouring threads hold a group
-  const int groups = (p.k_pad + 127) >> 7;
+  // int8, one scale per row
+  uint32_t amax = 0;
+  float y[V][8];
 #pragma unroll
-  for (int i = 0; i < kVec; ++i) {
+  for (int i = 0; i < V; ++i) {
     const int v = threadIdx.x + i * blockDim.x;
-    uint32_t m = 0;
+    normed(i, y[i]);
     if (v < nvec) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) m = max(m, mag(y[i][j]));
+      amax = mag_max(y[i], amax);
+      if (p.out) reinterpret_cast<uint4*>(p.out + t * p.ldo)[v] = pack8(y[i]);
     }
+  }
+  const Divider d(block_max(amax, max_buf), 127.f);
+  if (threadIdx.x == 0) p.scale[t] = d.s;
 #pragma unroll
-    for (int o = 8; o >= 1; o >>= 1) m = max(m, __shfl_xor_sync(kFull, m, o));
-    const float s = scale_of(m, 448.f);
-    if (v < nvec) {
-      q[v] = make_uint2(e4m3x2_rn(__fdiv_rn(y[i][0], s), __fdiv_rn(y[i][1], s)) |
-                            (e4m3x2_rn(__fdiv_rn(y[i][2], s), __fdiv_rn(y[i][3], s)) << 16),
-                        e4m3x2_rn(__fdiv_rn(y[i][4], s), __fdiv_rn(y[i][5], s)) |
-                            (e4m3x2_rn(__fdiv_rn(y[i][6], s), __fdiv_rn(y[i][7], s)) << 16));
-    } else if (v < npad) {
-      q[v] = make_uint2(0, 0);
-    }
-    if ((v & 15) == 0 && (v >> 4) < groups) p.scale[t * groups + (v >> 4)] = s;
+  for (int i = 0; i < V; ++i) {
+    const int v = threadIdx.x + i * blockDim.x;
+    if (v < nvec) q[v] = pack_s8(y[i], d);
   }
-  // columns and groups past the vectors that the threads hold
-  for (int v = kVec * blockDim.x + threadIdx.x; v < npad; v += blockDim.x) {
-    q[v] = make_uint2(0, 0);
-    if ((v & 15) == 0) p.scale[t * groups + (v >> 4)] = 1.f;
-  }
+  for (int v = nvec + threadIdx.x; v < npad; v += blockDim.x) q[v] = make_uint2(0, 0);
 }
 
-// Where row t's copies go: r itself, or its `copies` places in the permuted
-// order, those of the launch's experts only.
-__device__ __forceinline__ int dest_row(const QuantInt8Params& p, long long t, int c, int lo, int hi) {
-  if (p.inverse == nullptr) return static_cast<int>(t);
-  const int d = p.inverse[t * p.copies + c];
+// The places in the permuted order of 32 copies of row t, from copy c0 on: lane
+// c holds that of copy c0 + c, -1 for a place outside [lo, hi).
+__device__ __forceinline__ int dest_rows(const int* inverse, long long t, int c0, int copies, int lo, int hi) {
+  const int c = c0 + (threadIdx.x & 31);
+  const int d = c < copies ? inverse[t * copies + c] : -1;
   return d >= lo && d < hi ? d : -1;
 }
 
-__global__ void __launch_bounds__(1024) act_quant_int8_kernel(const QuantInt8Params p) {
+template <int V>
+__global__ void __launch_bounds__(V == 4 ? 1024 : 256) act_quant_int8_kernel(const QuantInt8Params p) {
   __shared__ uint32_t max_buf[32];
   const long long t = blockIdx.x;
   const int nvec = p.k_valid >> 3, npad = p.k_pad >> 3;
+  const uint4* x = reinterpret_cast<const uint4*>(p.x + t * p.ldx);
+  uint4 h[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int v = threadIdx.x + i * blockDim.x;
+    h[i] = v < nvec ? x[v] : make_uint4(0, 0, 0, 0);
+  }
   int lo = 0, hi = p.rows_out;
   if (p.range) {
     lo = p.range[p.expert_lo];
     hi = min(hi, p.range[p.expert_hi]);
   }
-  if (p.inverse == nullptr && (t < lo || t >= hi)) return;
-  const uint4* x = reinterpret_cast<const uint4*>(p.x + t * p.ldx);
-  uint4 h[kVec];
+  int dest = t >= lo && t < hi ? static_cast<int>(t) : -1;
+  if (p.inverse) dest = dest_rows(p.inverse, t, 0, p.copies, lo, hi);
   uint32_t amax = 0;
 #pragma unroll
-  for (int i = 0; i < kVec; ++i) {
-    const int v = threadIdx.x + i * blockDim.x;
-    h[i] = make_uint4(0, 0, 0, 0);
-    if (v < nvec) h[i] = x[v];
+  for (int i = 0; i < V; ++i) {
     float f[8];
     unpack8(h[i], f);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) amax = max(amax, mag(f[j]));
+    amax = mag_max(f, amax);
   }
-  amax = block_max(amax, max_buf);
-  const float s = scale_of(amax, 127.f);
-  uint2 o[kVec];
+  const Divider d(block_max(amax, max_buf), 127.f);
+  uint2 o[V];
 #pragma unroll
-  for (int i = 0; i < kVec; ++i) {
+  for (int i = 0; i < V; ++i) {
     float f[8];
     unpack8(h[i], f);
-    o[i] = pack_s8(f, s);
+    o[i] = pack_s8(f, d);
   }
-  for (int c = 0; c < p.copies; ++c) {
-    const int d = dest_row(p, t, c, lo, hi);
-    if (d < 0) continue;
-    uint2* q = reinterpret_cast<uint2*>(p.q + (long long)d * p.k_pad);
+  for (int c0 = 0; c0 < p.copies; c0 += 32) {
+    if (c0) dest = dest_rows(p.inverse, t, c0, p.copies, lo, hi);
+    for (int c = 0; c < min(32, p.copies - c0); ++c) {
+      const int at = __shfl_sync(kFull, dest, c);
+      if (at < 0) continue;
+      uint2* q = reinterpret_cast<uint2*>(p.q + (long long)at * p.k_pad);
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) {
-      const int v = threadIdx.x + i * blockDim.x;
-      if (v < nvec) q[v] = o[i];
+      for (int i = 0; i < V; ++i) {
+        const int v = threadIdx.x + i * blockDim.x;
+        if (v < nvec) q[v] = o[i];
+      }
+      for (int v = nvec + threadIdx.x; v < npad; v += blockDim.x) q[v] = make_uint2(0, 0);
+      if (threadIdx.x == 0) p.scale[at] = d.s;
     }
-    for (int v = nvec + threadIdx.x; v < npad; v += blockDim.x) q[v] = make_uint2(0, 0);
-    if (threadIdx.x == 0) p.scale[d] = s;
   }
 }
 
@@ -257,34 +294,45 @@ __global__ void __launch_bounds__(128) scatter_rows_8bit_kernel(const ScatterRow
     hi = min(hi, p.range[p.expert_hi]);
   }
   const uint4* src = reinterpret_cast<const uint4*>(p.q + t * p.row_bytes);
-  for (int c = 0; c < p.copies; ++c) {
-    const int d = p.inverse[t * p.copies + c];
-    if (d < lo || d >= hi) continue;
-    uint4* dst = reinterpret_cast<uint4*>(p.out + (long long)d * p.row_bytes);
-    for (int v = threadIdx.x; v < nvec; v += blockDim.x) dst[v] = src[v];
-    for (int g = threadIdx.x; g < p.groups; g += blockDim.x)
-      p.out_scale[(long long)d * p.groups + g] = p.scale[t * p.groups + g];
+  for (int c0 = 0; c0 < p.copies; c0 += 32) {
+    const int dest = dest_rows(p.inverse, t, c0, p.copies, lo, hi);
+    const int n = min(32, p.copies - c0);
+    for (int v = threadIdx.x; v < (nvec + 31) / 32 * 32; v += blockDim.x) {   // whole warps: the copies are traded
+      const uint4 val = v < nvec ? __ldg(src + v) : make_uint4(0, 0, 0, 0);
+      for (int c = 0; c < n; ++c) {
+        const int at = __shfl_sync(kFull, dest, c);
+        if (at >= 0 && v < nvec) reinterpret_cast<uint4*>(p.out + (long long)at * p.row_bytes)[v] = val;
+      }
+    }
+    for (int c = 0; c < n; ++c) {
+      const int at = __shfl_sync(kFull, dest, c);
+      if (at < 0) continue;
+      for (int g = threadIdx.x; g < p.groups; g += blockDim.x)
+        p.out_scale[(long long)at * p.groups + g] = p.scale[t * p.groups + g];
+    }
   }
 }
 
-// Threads of a block that holds nvec vectors, kVec per thread at most, a
-// multiple of 32.
-int row_threads(int nvec) {
-  const int per = (nvec + kVec - 1) / kVec;
-  const int want = nvec <= 512 ? (nvec + 1) / 2 : per;   // short rows: two vectors a thread
-  const int t = ((want > per ? want : per) + 31) / 32 * 32;
-  return t < 32 ? 32 : t;
-}
+// Vectors per thread: one for rows of up to 128 vectors, two up to 512, so
+// that a block stays at 256 threads and several share an SM; four beyond.
+int row_vecs(int nvec) { return nvec <= 128 ? 1 : (nvec <= 512 ? 2 : 4); }
+int row_threads(int nvec, int v) { return ((nvec + v - 1) / v + 31) / 32 * 32; }
 
 }  // namespace
 
 cudaError_t launch_add_rmsnorm(cudaStream_t st, const NormParams& p) {
-  add_rmsnorm_kernel<<<p.T, row_threads(p.H >> 3), 0, st>>>(p);
+  const int v = row_vecs(p.H >> 3), n = row_threads(p.H >> 3, v);
+  if (v == 1) add_rmsnorm_kernel<1><<<p.T, n, 0, st>>>(p);
+  else if (v == 2) add_rmsnorm_kernel<2><<<p.T, n, 0, st>>>(p);
+  else add_rmsnorm_kernel<4><<<p.T, n, 0, st>>>(p);
   return cudaGetLastError();
 }
 
 cudaError_t launch_act_quant_int8(cudaStream_t st, const QuantInt8Params& p) {
-  act_quant_int8_kernel<<<p.rows, row_threads(p.k_valid >> 3), 0, st>>>(p);
+  const int v = row_vecs(p.k_valid >> 3), n = row_threads(p.k_valid >> 3, v);
+  if (v == 1) act_quant_int8_kernel<1><<<p.rows, n, 0, st>>>(p);
+  else if (v == 2) act_quant_int8_kernel<2><<<p.rows, n, 0, st>>>(p);
+  else act_quant_int8_kernel<4><<<p.rows, n, 0, st>>>(p);
   return cudaGetLastError();
 }
 
