@@ -383,6 +383,20 @@ int b200moe_w8a8_gemm(int device, void* stream, const b200moe_gemm_args* args, c
 int b200moe_int8_gemm(int device, void* stream, const b200moe_gemm_args* args, const void* q,
                       const float* q_scale, const float* w_scale, const float* bias);
 
+/* b200moe_act_quant_int8 of x and b200moe_int8_gemm on its rows, in one call:
+ * x holds `rows` bf16 rows of ldx elements whose k_valid columns are quantised
+ * to args->k_pad columns, row r to its `copies` places inverse[r][..] of the
+ * args->b_rows permuted rows (inverse NULL: to r), of the launch's experts
+ * only. The GEMM's first weight tiles load while the rows are quantised.
+ * workspace: b200moe_int8_project_workspace(args->b_rows, args->k_pad) bytes of
+ * device memory the call may overwrite, 256-byte aligned; it must not be in
+ * use by another call that may run at the same time. */
+size_t b200moe_int8_project_workspace(int rows, int k_pad);
+int b200moe_int8_project(int device, void* stream, const b200moe_gemm_args* args, const void* x,
+                         long long ldx, int rows, int k_valid, const int* inverse, int copies,
+                         const float* w_scale, const float* bias, void* workspace,
+                         size_t workspace_bytes);
+
 /* ------------------------------------------------------------ combine
  * out[t, :] = ordered bf16 sum over the slots k of token t of the
  * contribution rows c[inverse[t*K+k], :], starting from bf16 zero and

@@ -44,6 +44,8 @@ EXPORTED = (
     "b200moe_expert_gemm",
     "b200moe_w8a8_gemm",
     "b200moe_int8_gemm",
+    "b200moe_int8_project_workspace",
+    "b200moe_int8_project",
     "b200moe_combine",
     "b200moe_combine_f32",
     "b200moe_append_shared_slot",
@@ -196,6 +198,13 @@ def _load() -> ctypes.CDLL:
     lib.b200moe_w8a8_gemm.argtypes = [c_int, c_void_p, POINTER(GemmArgs), c_void_p, c_void_p]
     lib.b200moe_int8_gemm.restype = c_int
     lib.b200moe_int8_gemm.argtypes = [c_int, c_void_p, POINTER(GemmArgs), c_void_p, c_void_p, c_void_p, c_void_p]
+    lib.b200moe_int8_project_workspace.restype = c_size_t
+    lib.b200moe_int8_project_workspace.argtypes = [c_int, c_int]
+    lib.b200moe_int8_project.restype = c_int
+    lib.b200moe_int8_project.argtypes = [
+        c_int, c_void_p, POINTER(GemmArgs), c_void_p, c_longlong, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p,
+        c_void_p, c_size_t,
+    ]
     lib.b200moe_gemm_args_size.restype = c_size_t
     lib.b200moe_gemm_args_size.argtypes = []
     if lib.b200moe_gemm_args_size() != ctypes.sizeof(GemmArgs):

@@ -81,6 +81,8 @@ struct DeviceScope {
   }
 };
 
+size_t align256(size_t v) { return (v + 255) & ~static_cast<size_t>(255); }
+
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
@@ -208,9 +210,9 @@ int b200moe_route_grouped(int device, void* stream, const void* logits, int logi
   return B200MOE_OK;
 }
 
-int b200moe_act_quant_int8(int device, void* stream, const void* x, long long ldx, int rows,
-                           int k_valid, int k_pad, const int* inverse, int copies, int rows_out,
-                           const int* row_offsets, int expert_lo, int expert_hi, void* q, float* s) {
+// Checks of the int8 quantiser's arguments; fills all but range, q and scale.
+static int act_quant_int8_params(b200::QuantInt8Params& p, const void* x, long long ldx, int rows, int k_valid,
+                                 int k_pad, const int* inverse, int copies, int rows_out) {
   B200_CHECK(rows >= 0 && k_valid >= 1 && k_pad >= k_valid && rows_out >= 0 && copies >= 1,
              "bad sizes rows=%d k_valid=%d k_pad=%d rows_out=%d copies=%d", rows, k_valid, k_pad, rows_out, copies);
   B200_CHECK(k_valid % 8 == 0 && k_pad % 16 == 0 && ldx % 8 == 0 && ldx >= k_valid,
@@ -218,14 +220,7 @@ int b200moe_act_quant_int8(int device, void* stream, const void* x, long long ld
   if (k_pad > 8 * b200::kNormMaxVecs)
     return fail(B200MOE_ERR_UNSUPPORTED, "at most %d columns (k_pad=%d)", 8 * b200::kNormMaxVecs, k_pad);
   B200_CHECK(inverse || (copies == 1 && rows_out >= rows), "without inverse, copies is 1 and rows_out at least rows");
-  B200_CHECK(row_offsets == nullptr || (expert_lo >= 0 && expert_hi >= expert_lo), "bad expert range");
-  if (rows == 0 || rows_out == 0) return B200MOE_OK;
-  B200_CHECK(x && q && s, "x, q and s are required");
-  B200_CHECK(aligned16(x) && aligned16(q), "x and q must be 16-byte aligned");
-  DeviceScope scope;
-  int rc = use_device(device, nullptr);
-  if (rc) return rc;
-  b200::QuantInt8Params p{};
+  B200_CHECK(rows == 0 || rows_out == 0 || (x && aligned16(x)), "x is required, 16-byte aligned");
   p.x = static_cast<const __nv_bfloat16*>(x);
   p.ldx = ldx;
   p.rows = rows;
@@ -234,6 +229,21 @@ int b200moe_act_quant_int8(int device, void* stream, const void* x, long long ld
   p.inverse = inverse;
   p.copies = copies;
   p.rows_out = rows_out;
+  return B200MOE_OK;
+}
+
+int b200moe_act_quant_int8(int device, void* stream, const void* x, long long ldx, int rows,
+                           int k_valid, int k_pad, const int* inverse, int copies, int rows_out,
+                           const int* row_offsets, int expert_lo, int expert_hi, void* q, float* s) {
+  b200::QuantInt8Params p{};
+  int rc = act_quant_int8_params(p, x, ldx, rows, k_valid, k_pad, inverse, copies, rows_out);
+  if (rc) return rc;
+  B200_CHECK(row_offsets == nullptr || (expert_lo >= 0 && expert_hi >= expert_lo), "bad expert range");
+  if (rows == 0 || rows_out == 0) return B200MOE_OK;
+  B200_CHECK(q && s && aligned16(q), "q (16-byte aligned) and s are required");
+  DeviceScope scope;
+  rc = use_device(device, nullptr);
+  if (rc) return rc;
   p.range = row_offsets;
   p.expert_lo = expert_lo;
   p.expert_hi = expert_hi;
@@ -826,11 +836,8 @@ int b200moe_w8a8_gemm(int device, void* stream, const b200moe_gemm_args* a, cons
   return B200MOE_OK;
 }
 
-int b200moe_int8_gemm(int device, void* stream, const b200moe_gemm_args* a, const void* q,
-                      const float* q_scale, const float* w_scale, const float* bias) {
-  B200_CHECK(a != nullptr, "args is NULL");
-  if (a->max_rows <= 0) return B200MOE_OK;
-  B200_CHECK(a->weight && q && q_scale && w_scale && a->out, "weight, q, q_scale, w_scale, out are required");
+static int int8_gemm_check(const b200moe_gemm_args* a, const float* w_scale) {
+  B200_CHECK(a->weight && w_scale && a->out, "weight, w_scale, out are required");
   B200_CHECK(a->offsets || (a->n_experts == 1 && a->expert_begin == 0), "more than one expert needs offsets");
   B200_CHECK(a->wfmt == B200MOE_W_INT8, "the int8 GEMM needs int8 weights");
   B200_CHECK(a->planes == 1 || a->planes == 2, "planes must be 1 or 2");
@@ -848,23 +855,27 @@ int b200moe_int8_gemm(int device, void* stream, const b200moe_gemm_args* a, cons
   if (a->k_pad >= 131072)
     return fail(B200MOE_ERR_UNSUPPORTED, "k_pad must be below 131072, where the int32 sum could overflow");
   B200_CHECK(a->b_rows >= 1 && a->b_rows >= a->max_rows, "q must have at least max_rows rows");
-  B200_CHECK(aligned16(q) && aligned16(a->weight), "q and weight must be 16-byte aligned");
+  B200_CHECK(aligned16(a->weight), "weight must be 16-byte aligned");
   B200_CHECK(a->ldo >= a->n_feat && a->ldo % 8 == 0 && a->n_feat % 8 == 0 && aligned16(a->out),
              "output rows must be 16-byte aligned (ldo %% 8 == 0, n_feat %% 8 == 0)");
   if (a->row_weight) B200_CHECK(a->row_src != nullptr, "row_weight needs row_src");
   B200_CHECK(a->token_tile == 0 || a->token_tile == 16 || a->token_tile == 32 || a->token_tile == 64 ||
                  a->token_tile == 128 || a->token_tile == 256,
              "token_tile must be 0, 16, 32, 64, 128 or 256");
-  DeviceScope scope;
-  int* sp = nullptr;
-  int rc = use_device(device, &sp);
-  if (rc) return rc;
+  return B200MOE_OK;
+}
 
+// after_quant: the stream's previous kernel is this library's quantiser of the
+// same call, which writes q and q_scale only, so that everything else may be
+// read before it has ended.
+static int int8_gemm_launch(int device, int* sp, void* stream, const b200moe_gemm_args* a, const void* q,
+                            const float* q_scale, const float* w_scale, const float* bias, bool after_quant) {
   const bool is_gated = a->planes == 2;
   int bn = a->token_tile;
   if (bn == 0) {
-    // 1.5x the mean rows per expert, so that one tile usually holds an expert's rows
-    const long long avg = (3ll * a->max_rows + 2ll * a->n_experts - 1) / (2ll * a->n_experts);
+    // 1.5x the mean rows per expert, so that one tile usually holds an expert's
+    // rows; without offsets the rows are known
+    const long long avg = a->offsets ? (3ll * a->max_rows + 2ll * a->n_experts - 1) / (2ll * a->n_experts) : a->max_rows;
     bn = std::min(256, std::max(16, pow2_ceil(static_cast<int>(std::min(avg, 1ll << 20)))));
   }
   const int feat_tiles = a->feat_pad / (is_gated ? 64 : 128);
@@ -894,6 +905,7 @@ int b200moe_int8_gemm(int device, void* stream, const b200moe_gemm_args* a, cons
   p.ldo = a->ldo;
   p.status = sp;
   p.box = std::min(bn, 64);
+  p.early = after_quant ? 1 : 0;
   // shared memory: stages of a 16 KB weight image and bn x 128 B token rows,
   // the epilogue's scales, barriers and the tile prefix
   const uint32_t budget = 232448u - 2048u;
@@ -935,9 +947,64 @@ int b200moe_int8_gemm(int device, void* stream, const b200moe_gemm_args* a, cons
   cfg.blockDim = dim3(b200::kInt8Threads, 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = static_cast<cudaStream_t>(stream);
+  // the launch may begin before the stream's previous kernel has ended; the
+  // kernel waits for that end itself
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
   void* args[] = {&qmap, &p};
   B200_CUDA(cudaLaunchKernelExC(&cfg, kern, args));
   return B200MOE_OK;
+}
+
+int b200moe_int8_gemm(int device, void* stream, const b200moe_gemm_args* a, const void* q,
+                      const float* q_scale, const float* w_scale, const float* bias) {
+  B200_CHECK(a != nullptr, "args is NULL");
+  if (a->max_rows <= 0) return B200MOE_OK;
+  int rc = int8_gemm_check(a, w_scale);
+  if (rc) return rc;
+  B200_CHECK(q && q_scale && aligned16(q), "q (16-byte aligned) and q_scale are required");
+  DeviceScope scope;
+  int* sp = nullptr;
+  rc = use_device(device, &sp);
+  if (rc) return rc;
+  return int8_gemm_launch(device, sp, stream, a, q, q_scale, w_scale, bias, false);
+}
+
+size_t b200moe_int8_project_workspace(int rows, int k_pad) {
+  if (rows <= 0 || k_pad <= 0) return 0;
+  return align256((size_t)rows * k_pad) + align256((size_t)rows * sizeof(float));
+}
+
+int b200moe_int8_project(int device, void* stream, const b200moe_gemm_args* a, const void* x, long long ldx,
+                         int rows, int k_valid, const int* inverse, int copies, const float* w_scale,
+                         const float* bias, void* workspace, size_t workspace_bytes) {
+  B200_CHECK(a != nullptr, "args is NULL");
+  if (a->max_rows <= 0) return B200MOE_OK;
+  int rc = int8_gemm_check(a, w_scale);
+  if (rc) return rc;
+  b200::QuantInt8Params p{};
+  rc = act_quant_int8_params(p, x, ldx, rows, k_valid, a->k_pad, inverse, copies, a->b_rows);
+  if (rc) return rc;
+  B200_CHECK(workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0 &&
+                 workspace_bytes >= b200moe_int8_project_workspace(a->b_rows, a->k_pad),
+             "workspace must be 256-byte aligned and hold %zu bytes (got %zu)",
+             b200moe_int8_project_workspace(a->b_rows, a->k_pad), workspace_bytes);
+  p.q = static_cast<uint8_t*>(workspace);
+  p.scale = reinterpret_cast<float*>(p.q + align256((size_t)a->b_rows * a->k_pad));
+  if (a->offsets) {
+    p.range = a->offsets;
+    p.expert_lo = a->expert_begin;
+    p.expert_hi = a->expert_begin + a->n_experts;
+  }
+  DeviceScope scope;
+  int* sp = nullptr;
+  rc = use_device(device, &sp);
+  if (rc) return rc;
+  if (rows > 0) B200_CUDA(b200::launch_act_quant_int8(static_cast<cudaStream_t>(stream), p));
+  return int8_gemm_launch(device, sp, stream, a, p.q, p.scale, w_scale, bias, rows > 0);
 }
 
 int b200moe_combine(int device, void* stream, const void* rows, long long ld_rows,
@@ -1132,7 +1199,6 @@ struct LayerPlan {
   bool gather;
 };
 
-size_t align256(size_t v) { return (v + 255) & ~static_cast<size_t>(255); }
 
 // Token tile of the separate-call path (experts.tile_policy): the smallest
 // power of two from 16 covering 1.5x the mean rows per expert, capped at

@@ -119,6 +119,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   int* prefix = s_total + 1;            // [n_experts + 1]: row chunks of the experts before
 
   if (warp == 0) {
+    // what the row chunks are counted from may come from the previous kernel
+    if (!p.early) grid_dep_wait();
     const int bad = *reinterpret_cast<volatile int*>(p.status) & kStatusWaitTimeout;
     int acc = 0;
     if (lane == 0) prefix[0] = 0;
@@ -168,25 +170,42 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (lane == 0) {
       Ring ring(p.ns);
       int issued = 0;
-      bool ok = true;
+      bool ok = true, waited = !p.early;
       for (int t = blockIdx.x; ok && t < total; t += gridDim.x) {
         const Tile tl = decode_tile<BN>(t, prefix, p);
         if (tl.nrows <= 0) continue;
         const uint8_t* wt = p.wtiles + (long long)(tl.e * p.feat_tiles + tl.ft) * p.nkb * kAStage;
         const int boxes = (tl.nrows + p.box - 1) / p.box;
-        for (int k = 0; k < p.nkb; ++k, ring.next(), ++issued) {
+        auto arm = [&](int s, int k) {   // both operands' bytes, and the weights' copy
+          mbar_arrive_expect_tx(&full[s], kAStage + boxes * p.box * 128);
+          bulk_load(sbase + s * p.stage_bytes, wt + (long long)k * kAStage, kAStage, &full[s]);
+        };
+        auto rows = [&](int s, int k) {
+          for (int b = 0; b < boxes; ++b)
+            tma_load_2d(sbase + s * p.stage_bytes + kAStage + b * p.box * 128, &qmap, &full[s], k * 128,
+                        tl.row0 + b * p.box);
+        };
+        int k = 0;
+        if (!waited) {
+          // the ring is empty: fill it with weights, then wait for the rows
+          const int pre = min(p.ns, p.nkb);
+          for (int i = 0; i < pre; ++i) arm(i, i);
+          grid_dep_wait();
+          waited = true;
+          for (; k < pre; ++k, ring.next(), ++issued) rows(k, k);
+        }
+        for (; k < p.nkb; ++k, ring.next(), ++issued) {
           const int s = ring.idx;
           if (!wait_bounded(&empty[s], ring.phase ^ 1u, p.status)) {
             ok = false;
             break;
           }
-          uint8_t* st = sbase + s * p.stage_bytes;
-          mbar_arrive_expect_tx(&full[s], kAStage + boxes * p.box * 128);
-          bulk_load(st, wt + (long long)k * kAStage, kAStage, &full[s]);
-          for (int b = 0; b < boxes; ++b)
-            tma_load_2d(st + kAStage + b * p.box * 128, &qmap, &full[s], k * 128, tl.row0 + b * p.box);
+          arm(s, k);
+          rows(s, k);
         }
       }
+      // also without a tile: this grid must not end before the previous one
+      if (!waited) grid_dep_wait();
       // every issued copy has landed before the CTA may exit
       for (int i = max(0, issued - p.ns); i < issued; ++i)
         wait_bounded(&full[i % p.ns], (i / p.ns) & 1, p.status, 32);
@@ -236,6 +255,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const bool is_gate = lane < 16;
     const float nlog = -1.44269504f * (p.epi == kEpiClampF32 ? p.alpha : 1.f);
     int tc = 0;
+    grid_dep_wait();   // row scales and routing weights are read, and rows written, below
     for (int t = blockIdx.x; t < total; t += gridDim.x) {
       const Tile tl = decode_tile<BN>(t, prefix, p);
       if (tl.nrows <= 0) continue;

@@ -133,6 +133,7 @@ struct Int8Params {
   long long ldo;
   int* status;
   int ns, box;                 // pipeline stages, token rows per copy
+  int early;                   // only q and qs depend on the stream's previous kernel
   uint32_t stage_bytes, x_off, bar_off, tmem_cols;
 };
 constexpr int kInt8Threads = 320;    // copy warp, MMA warp, 8 epilogue warps

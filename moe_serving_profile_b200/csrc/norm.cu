@@ -122,6 +122,7 @@ template <int V>
 __global__ void __launch_bounds__(V == 4 ? 1024 : 256) add_rmsnorm_kernel(const NormParams p) {
   __shared__ float sum_buf[32];
   __shared__ uint32_t max_buf[32];
+  grid_dep_launch();
   const long long t = blockIdx.x;
   const int nvec = p.H >> 3;
   const uint4* x = reinterpret_cast<const uint4*>(p.x + t * p.ldx);
@@ -235,6 +236,7 @@ __device__ __forceinline__ int dest_rows(const int* inverse, long long t, int c0
 template <int V>
 __global__ void __launch_bounds__(V == 4 ? 1024 : 256) act_quant_int8_kernel(const QuantInt8Params p) {
   __shared__ uint32_t max_buf[32];
+  grid_dep_launch();
   const long long t = blockIdx.x;
   const int nvec = p.k_valid >> 3, npad = p.k_pad >> 3;
   const uint4* x = reinterpret_cast<const uint4*>(p.x + t * p.ldx);
@@ -286,6 +288,7 @@ __global__ void __launch_bounds__(V == 4 ? 1024 : 256) act_quant_int8_kernel(con
 // Rows of 8-bit values with `groups` scales each, copied to their places in
 // the permuted order.
 __global__ void __launch_bounds__(128) scatter_rows_8bit_kernel(const ScatterRowsParams p) {
+  grid_dep_launch();
   const long long t = blockIdx.x;
   const int nvec = p.row_bytes >> 4;
   int lo = 0, hi = p.rows_out;

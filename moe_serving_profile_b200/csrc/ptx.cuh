@@ -434,6 +434,14 @@ B200_DEVI void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
 }
 B200_DEVI void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// ---------------------------------------------------------------- dependent launch
+// Let the stream's next kernel begin, where its launch allows that; its
+// grid_dep_wait still waits until this grid has ended.
+B200_DEVI void grid_dep_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+// Wait until the stream's previous kernel has ended and its writes are visible
+// (at once for a launch that does not overlap it).
+B200_DEVI void grid_dep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // ---------------------------------------------------------------- cluster
 B200_DEVI uint32_t cluster_ctarank() {
   uint32_t r;

@@ -131,6 +131,23 @@ def _local_range(w: ExpertWeights, perm: ops.Permutation, num_experts: int, expe
     return dict(offsets=perm.offsets, expert_lo=lo, expert_hi=hi) if (lo, hi) != (0, num_experts) else {}
 
 
+def _int8_tile(rows: int, experts: int) -> int:
+    """tile_policy's tile of an int8 launch, in integers (exact sums: the tile
+    changes no result)."""
+    want = -(-3 * rows // (2 * experts))
+    return 16 if want <= 16 else min(256, 1 << (want - 1).bit_length())
+
+
+def _w1(w: ExpertWeights) -> dict:
+    return dict(planes=2, feat_pad=w.i_pad, n_feat=w.inter, k_pad=w.h_k, weight=w.w1, weight_scale=w.s1, bias=w.b1,
+                epilogue=w.gated_epilogue, alpha=w.alpha, limit=w.limit, n_experts=w.n_experts)
+
+
+def _w2(w: ExpertWeights) -> dict:
+    return dict(planes=1, feat_pad=w.h_f, n_feat=w.hidden, k_pad=w.i_pad, weight=w.w2, weight_scale=w.s2, bias=w.b2,
+                epilogue=_lib.EPI_DOWN_ONCE, n_experts=w.n_experts)
+
+
 def int8_gate_up(w: ExpertWeights, hidden: torch.Tensor | ops.QuantRows, perm: ops.Permutation, *, K: int,
                  num_experts: int, expert_begin: int, copies: int | None = None,
                  out: torch.Tensor | None = None) -> torch.Tensor:
@@ -139,22 +156,19 @@ def int8_gate_up(w: ExpertWeights, hidden: torch.Tensor | ops.QuantRows, perm: o
     token rows a norm already quantised (ops.QuantRows)."""
     if w.fmt != _lib.W_INT8:
         raise ValueError("int8_gate_up needs int8 expert weights")
-    local = _local_range(w, perm, num_experts, expert_begin)
     copies = K if copies is None else copies
     R = perm.perm_src.numel()
-    if isinstance(hidden, ops.QuantRows):
-        T = hidden.q.shape[0]
-        rows = ops.scatter_rows_8bit(hidden.checked(torch.int8, w.h_k, w.w1.device), perm.inverse, copies, **local)
-    else:
-        T = hidden.shape[0]
-        if hidden.shape[1] != w.hidden:
-            raise ValueError(f"hidden size {hidden.shape[1]} does not match the experts' {w.hidden}")
-        rows = ops.act_quant_int8(hidden, k_pad=w.h_k, inverse=perm.inverse, copies=copies, **local)
     act = torch.empty(R, w.i_pad, device=w.w1.device, dtype=torch.bfloat16) if out is None else out
-    return ops.int8_gemm(offsets=perm.offsets, expert_begin=expert_begin, n_experts=w.n_experts, max_rows=R,
-                         planes=2, feat_pad=w.i_pad, n_feat=w.inter, k_pad=w.h_k, weight=w.w1, weight_scale=w.s1,
-                         rows=rows, epilogue=w.gated_epilogue, bias=w.b1, alpha=w.alpha, limit=w.limit, out=act,
-                         token_tile=tile_policy(T, copies, num_experts))
+    tile = _int8_tile(R, num_experts)
+    if isinstance(hidden, ops.QuantRows):
+        rows = ops.scatter_rows_8bit(hidden.checked(torch.int8, w.h_k, w.w1.device), perm.inverse, copies,
+                                     **_local_range(w, perm, num_experts, expert_begin))
+        return ops.int8_gemm(offsets=perm.offsets, expert_begin=expert_begin, max_rows=R, rows=rows, out=act,
+                             token_tile=tile, **_w1(w))
+    if hidden.shape[1] != w.hidden:
+        raise ValueError(f"hidden size {hidden.shape[1]} does not match the experts' {w.hidden}")
+    return ops.int8_project(hidden, offsets=perm.offsets, expert_begin=expert_begin, inverse=perm.inverse,
+                            copies=copies, out=act, token_tile=tile, **_w1(w))
 
 
 def int8_down(w: ExpertWeights, act: torch.Tensor, perm: ops.Permutation, weights: torch.Tensor | None, *, K: int,
@@ -164,17 +178,15 @@ def int8_down(w: ExpertWeights, act: torch.Tensor, perm: ops.Permutation, weight
     [T, K] when given: contribution rows [T*K, H] bf16."""
     if w.fmt != _lib.W_INT8:
         raise ValueError("int8_down needs int8 expert weights")
-    local = _local_range(w, perm, num_experts, expert_begin)
     R = perm.perm_src.numel()
-    rows = ops.act_quant_int8(act[:, :w.inter], k_pad=w.i_pad, **local)
+    if act.shape[0] != R or act.shape[1] < w.inter:
+        raise ValueError(f"act must be [{R}, {w.inter} or more], got {tuple(act.shape)}")
     if contrib is None:
         contrib = torch.empty(R, w.hidden, device=act.device, dtype=torch.bfloat16)
-    return ops.int8_gemm(offsets=perm.offsets, expert_begin=expert_begin, n_experts=w.n_experts, max_rows=R,
-                         planes=1, feat_pad=w.h_f, n_feat=w.hidden, k_pad=w.i_pad, weight=w.w2, weight_scale=w.s2,
-                         rows=rows, epilogue=_lib.EPI_DOWN_ONCE, bias=w.b2,
-                         row_weight=None if weights is None else weights.reshape(-1),
-                         row_src=None if weights is None else perm.perm_src, out=contrib,
-                         token_tile=tile_policy(R, 1, num_experts))
+    return ops.int8_project(act if act.shape[1] == w.inter else act[:, :w.inter], offsets=perm.offsets,
+                            expert_begin=expert_begin, row_weight=weights,
+                            row_src=None if weights is None else perm.perm_src, out=contrib,
+                            token_tile=_int8_tile(R, num_experts), **_w2(w))
 
 
 def run_experts_int8(w: ExpertWeights, hidden: torch.Tensor | ops.QuantRows, perm: ops.Permutation,
@@ -195,18 +207,11 @@ def run_experts_int8_placed(w: ExpertWeights, x: torch.Tensor, offsets: torch.Te
     last segment are neither read nor written. ``tokens``: the rows expected,
     for the token tile."""
     R = x.shape[0]
-    bn = tile_policy(tokens, 1, w.n_experts)
-    local = dict(offsets=offsets, expert_lo=0, expert_hi=w.n_experts)
+    kw = dict(offsets=offsets, expert_begin=0, token_tile=_int8_tile(tokens, w.n_experts))
     act = torch.empty(R, w.i_pad, device=x.device, dtype=torch.bfloat16)
-    ops.int8_gemm(offsets=offsets, expert_begin=0, n_experts=w.n_experts, max_rows=R, planes=2, feat_pad=w.i_pad,
-                  n_feat=w.inter, k_pad=w.h_k, weight=w.w1, weight_scale=w.s1,
-                  rows=ops.act_quant_int8(x, k_pad=w.h_k, **local), epilogue=w.gated_epilogue, bias=w.b1,
-                  alpha=w.alpha, limit=w.limit, out=act, token_tile=bn)
+    ops.int8_project(x, out=act, **kw, **_w1(w))
     y = torch.empty(R, w.hidden, device=x.device, dtype=torch.bfloat16)
-    return ops.int8_gemm(offsets=offsets, expert_begin=0, n_experts=w.n_experts, max_rows=R, planes=1,
-                         feat_pad=w.h_f, n_feat=w.hidden, k_pad=w.i_pad, weight=w.w2, weight_scale=w.s2,
-                         rows=ops.act_quant_int8(act[:, :w.inter], k_pad=w.i_pad, **local),
-                         epilogue=_lib.EPI_DOWN_ONCE, bias=w.b2, out=y, token_tile=bn)
+    return ops.int8_project(act[:, :w.inter], out=y, **kw, **_w2(w))
 
 
 def int8_swiglu(w: ExpertWeights, x: torch.Tensor) -> torch.Tensor:
@@ -214,32 +219,24 @@ def int8_swiglu(w: ExpertWeights, x: torch.Tensor) -> torch.Tensor:
     if w.fmt != _lib.W_INT8 or w.n_experts != 1:
         raise ValueError("int8_swiglu needs the int8 weights of one expert")
     T = x.shape[0]
-    bn = tile_policy(T, 1, 1, cover=1.0)
     act = torch.empty(T, w.i_pad, device=x.device, dtype=torch.bfloat16)
-    ops.int8_gemm(offsets=None, expert_begin=0, n_experts=1, max_rows=T, planes=2, feat_pad=w.i_pad, n_feat=w.inter,
-                  k_pad=w.h_k, weight=w.w1, weight_scale=w.s1, rows=ops.act_quant_int8(x, k_pad=w.h_k),
-                  epilogue=w.gated_epilogue, bias=w.b1, alpha=w.alpha, limit=w.limit, out=act, token_tile=bn)
+    ops.int8_project(x, offsets=None, expert_begin=0, out=act, **_w1(w))
     y = torch.empty(T, w.hidden, device=x.device, dtype=torch.bfloat16)
-    return ops.int8_gemm(offsets=None, expert_begin=0, n_experts=1, max_rows=T, planes=1, feat_pad=w.h_f,
-                         n_feat=w.hidden, k_pad=w.i_pad, weight=w.w2, weight_scale=w.s2,
-                         rows=ops.act_quant_int8(act[:, :w.inter], k_pad=w.i_pad), epilogue=_lib.EPI_DOWN_ONCE,
-                         bias=w.b2, out=y, token_tile=bn)
+    return ops.int8_project(act[:, :w.inter], offsets=None, expert_begin=0, out=y, **_w2(w))
 
 
 def int8_linear(w: Int8Linear, x: torch.Tensor | ops.QuantRows, out: torch.Tensor | None = None) -> torch.Tensor:
     """Dense int8 projection of bf16 rows ``x`` [T, K], or of rows a norm
     already quantised: bf16 [T, N]."""
-    rows = x if isinstance(x, ops.QuantRows) else None
-    if rows is None:
-        if x.shape[-1] != w.in_features:
-            raise ValueError(f"x has {x.shape[-1]} columns, the projection takes {w.in_features}")
-        rows = ops.act_quant_int8(x, k_pad=w.k_pad)
-    T = rows.q.shape[0]
+    quantised = isinstance(x, ops.QuantRows)
+    T = (x.q if quantised else x).shape[0]
+    if not quantised and x.shape[-1] != w.in_features:
+        raise ValueError(f"x has {x.shape[-1]} columns, the projection takes {w.in_features}")
     if out is None:
         out = torch.empty(T, w.out_features, device=w.w.device, dtype=torch.bfloat16)
-    return ops.int8_gemm(offsets=None, expert_begin=0, n_experts=1, max_rows=T, planes=1, feat_pad=w.n_pad,
-                         n_feat=w.out_features, k_pad=w.k_pad, weight=w.w, weight_scale=w.scale, rows=rows,
-                         epilogue=_lib.EPI_DOWN_ONCE, bias=w.bias, out=out, token_tile=tile_policy(T, 1, 1, cover=1.0))
+    kw = dict(offsets=None, expert_begin=0, n_experts=1, planes=1, feat_pad=w.n_pad, n_feat=w.out_features,
+              k_pad=w.k_pad, weight=w.w, weight_scale=w.scale, epilogue=_lib.EPI_DOWN_ONCE, bias=w.bias, out=out)
+    return ops.int8_gemm(max_rows=T, rows=x, **kw) if quantised else ops.int8_project(x, **kw)
 
 
 def run_experts_w8a8(w: ExpertWeights, hidden: torch.Tensor, perm: ops.Permutation,

@@ -23,8 +23,8 @@ def _dev(t: torch.Tensor, what: str) -> int:
     return t.device.index
 
 
-def _stream(device: int) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+# the current stream's handle, without building a torch.cuda.Stream around it
+_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _ptr(t: torch.Tensor | None) -> int | None:
@@ -301,6 +301,16 @@ class NormOut:
 QUANT = {None: _lib.QUANT_NONE, "fp8": _lib.QUANT_FP8, "int8": _lib.QUANT_INT8}
 
 
+def _residual_rows(t: torch.Tensor, x: torch.Tensor, device: int, what: str) -> int:
+    """The row stride of a residual, checked against ``x``."""
+    _bf16_rows(t, what)
+    if t.get_device() != device:
+        raise ValueError(f"{what} must be on cuda:{device}, got {t.device}")
+    if t.shape != x.shape:
+        raise ValueError(f"{what} must have x's shape {tuple(x.shape)}, got {tuple(t.shape)}")
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
 def add_rmsnorm(x: torch.Tensor, weight: torch.Tensor, eps: float, *, residual: torch.Tensor | None = None,
                 residual_out: torch.Tensor | None = None, quant: str | None = None, k_pad: int | None = None,
                 normed: bool = True) -> NormOut:
@@ -320,34 +330,35 @@ def add_rmsnorm(x: torch.Tensor, weight: torch.Tensor, eps: float, *, residual: 
     _same_device(weight, device, "weight")
     if quant is None and not normed:
         raise ValueError("nothing to compute: no quantised rows and no bf16 output")
-    for t, what in ((residual, "residual"), (residual_out, "residual_out")):
-        if t is not None:
-            _bf16_rows(t, what)
-            _same_device(t, device, what)
-            if t.shape != x.shape:
-                raise ValueError(f"{what} must have x's shape {tuple(x.shape)}, got {tuple(t.shape)}")
-    if residual is None and residual_out is not None:
+    dev = x.device
+    ldr = ldro = 0
+    if residual is not None:
+        ldr = _residual_rows(residual, x, device, "residual")
+        if residual_out is None:
+            residual_out, ldro = torch.empty((T, H), device=dev, dtype=torch.bfloat16), H
+        else:
+            ldro = _residual_rows(residual_out, x, device, "residual_out")
+    elif residual_out is not None:
         raise ValueError("residual_out needs a residual")
-    if residual is not None and residual_out is None:
-        residual_out = torch.empty(T, H, device=x.device, dtype=torch.bfloat16)
-    out = torch.empty(T, H, device=x.device, dtype=torch.bfloat16) if normed else None
-    rows = None
-    if quant is not None:
-        if k_pad is None:
-            k_pad = -(-H // 64) * 64 if quant == "fp8" else -(-H // 128) * 128
-        dtype = torch.float8_e4m3fn if quant == "fp8" else torch.int8
-        shape = (T, -(-k_pad // 128)) if quant == "fp8" else (T,)
-        rows = QuantRows(torch.empty((T, k_pad), device=x.device, dtype=dtype),
-                         torch.empty(shape, device=x.device, dtype=torch.float32))
-
-    def ld(t):
-        return 0 if t is None else (t.stride(0) if T > 1 else H)
-
+    out = torch.empty((T, H), device=dev, dtype=torch.bfloat16) if normed else None
+    rows = q = scale = None
+    if quant is None:
+        k_pad = 0
+    elif quant == "fp8":
+        k_pad = -(-H // 64) * 64 if k_pad is None else k_pad
+        q = torch.empty((T, k_pad), device=dev, dtype=torch.float8_e4m3fn)
+        scale = torch.empty((T, -(-k_pad // 128)), device=dev, dtype=torch.float32)
+        rows = QuantRows(q, scale)
+    else:
+        k_pad = -(-H // 128) * 128 if k_pad is None else k_pad
+        q = torch.empty((T, k_pad), device=dev, dtype=torch.int8)
+        scale = torch.empty((T,), device=dev, dtype=torch.float32)
+        rows = QuantRows(q, scale)
     check(
         lib.b200moe_add_rmsnorm(
-            device, _stream(device), _ptr(x), ld(x), _ptr(residual), ld(residual), _ptr(residual_out),
-            ld(residual_out), _ptr(weight), int(weight.dtype == torch.float32), float(eps), T, H, _ptr(out), ld(out),
-            QUANT[quant], _ptr(rows.q) if rows else None, k_pad if rows else 0, _ptr(rows.scale) if rows else None,
+            device, _stream(device), x.data_ptr(), x.stride(0) if T > 1 else H, _ptr(residual), ldr,
+            _ptr(residual_out), ldro, weight.data_ptr(), int(weight.dtype == torch.float32), eps, T, H, _ptr(out), H,
+            QUANT[quant], _ptr(q), k_pad, _ptr(scale),
         ),
         "add_rmsnorm",
     )
@@ -541,6 +552,41 @@ def w8a8_gemm(*, offsets: torch.Tensor, expert_begin: int, n_experts: int, max_r
     return out
 
 
+def _int8_args(*, offsets, expert_begin, n_experts, max_rows, planes, feat_pad, n_feat, k_pad, weight, weight_scale,
+               b_rows, epilogue, bias, alpha, limit, row_weight, row_src, out, token_tile, device):
+    """The checked GemmArgs of an int8 launch (positional: the fields of
+    b200moe_gemm_args in order)."""
+    tiles = n_experts * (feat_pad // (64 if planes == 2 else 128))
+    if weight.dtype != torch.int8 or not weight.is_contiguous() or weight.numel() != tiles * 128 * k_pad:
+        raise ValueError(f"weight must be contiguous int8 tiles of {tiles * 128 * k_pad} elements")
+    for t, what in ((weight_scale, "weight_scale"), (bias, "bias")):
+        if t is not None and (t.dtype != torch.float32 or not t.is_contiguous() or t.numel() != tiles * 128
+                              or t.get_device() != device):
+            raise ValueError(f"{what} must be contiguous float32 of {tiles * 128} elements on {weight.device}")
+    if out.dtype != torch.bfloat16 or out.dim() != 2 or out.stride(1) != 1:
+        raise ValueError("output must be a 2D bfloat16 tensor with contiguous rows")
+    rows_out, cols_out = out.shape
+    if out.get_device() != device or rows_out < max_rows or cols_out < n_feat:
+        raise ValueError(f"output must hold {max_rows} rows of {n_feat} columns on {weight.device}")
+    if offsets is not None and (offsets.get_device() != device or offsets.dtype != torch.int32
+                                or not offsets.is_contiguous() or offsets.numel() <= expert_begin + n_experts):
+        raise ValueError(f"offsets must be contiguous int32 covering the experts, on {weight.device}")
+    rw = rs = None
+    if row_weight is not None:
+        if (row_weight.dtype not in (torch.float32, torch.bfloat16) or not row_weight.is_contiguous()
+                or row_weight.get_device() != device or row_weight.numel() < max_rows):
+            raise ValueError(f"row_weight must be contiguous float32 or bfloat16, one per row, on {weight.device}")
+        if (row_src is None or row_src.dtype != torch.int32 or row_src.numel() < max_rows
+                or not row_src.is_contiguous() or row_src.get_device() != device):
+            raise ValueError(f"row_weight needs row_src (contiguous int32, one entry per row) on {weight.device}")
+        rw, rs = row_weight.data_ptr(), row_src.data_ptr()
+    return _lib.GemmArgs(
+        None if offsets is None else offsets.data_ptr(), expert_begin, n_experts, max_rows, token_tile, 0,
+        _lib.W_INT8, planes, feat_pad, n_feat, k_pad, weight.data_ptr(), 0, 0, None, 0, b_rows, 0, None, 1,
+        epilogue, None, alpha, limit, rw, int(row_weight is not None and row_weight.dtype == torch.bfloat16), rs,
+        out.data_ptr(), out.stride(0) if rows_out > 1 else cols_out)
+
+
 def int8_gemm(*, offsets: torch.Tensor | None, expert_begin: int, n_experts: int, max_rows: int, planes: int,
               feat_pad: int, n_feat: int, k_pad: int, weight: torch.Tensor, weight_scale: torch.Tensor,
               rows: QuantRows, epilogue: int, bias: torch.Tensor | None = None, alpha: float = 1.702,
@@ -551,52 +597,44 @@ def int8_gemm(*, offsets: torch.Tensor | None, expert_begin: int, n_experts: int
     (``act_quant_int8``'s outputs). ``offsets`` None: one expert holds all
     ``max_rows`` rows."""
     device = _dev(weight, "weight")
-    _bf16_rows(out, "output")
-    rows = rows.checked(torch.int8, k_pad, weight.device)
-    tiles = n_experts * (feat_pad // (64 if planes == 2 else 128))
-    if weight.dtype != torch.int8 or not weight.is_contiguous() or weight.numel() != tiles * 128 * k_pad:
-        raise ValueError(f"weight must be contiguous int8 tiles of {tiles * 128 * k_pad} elements")
-    for t, what in ((weight_scale, "weight_scale"), (bias, "bias")):
-        if t is not None and (t.dtype != torch.float32 or not t.is_contiguous() or t.numel() != tiles * 128
-                              or t.device != weight.device):
-            raise ValueError(f"{what} must be contiguous float32 of {tiles * 128} elements on {weight.device}")
-    if out.device != weight.device or out.shape[0] < max_rows or out.shape[1] < n_feat:
-        raise ValueError(f"output must hold {max_rows} rows of {n_feat} columns on {weight.device}")
-    if offsets is not None:
-        _same_device(offsets, device, "offsets")
-        if offsets.dtype != torch.int32 or not offsets.is_contiguous() or offsets.numel() <= expert_begin + n_experts:
-            raise ValueError("offsets must be contiguous int32 covering the experts")
-    a = _lib.GemmArgs()
-    a.offsets = _ptr(offsets)
-    a.expert_begin = expert_begin
-    a.n_experts = n_experts
-    a.max_rows = max_rows
-    a.token_tile = token_tile
-    a.wfmt = _lib.W_INT8
-    a.planes = planes
-    a.feat_pad = feat_pad
-    a.n_feat = n_feat
-    a.k_pad = k_pad
-    a.weight = _ptr(weight)
-    a.b_rows = rows.q.shape[0]
-    a.b_div = 1
-    a.epilogue = epilogue
-    a.alpha = alpha
-    a.limit = limit
-    if row_weight is not None:
-        _same_device(row_weight, device, "row_weight")
-        _same_device(row_src, device, "row_src")
-        if row_weight.dtype not in (torch.float32, torch.bfloat16) or not row_weight.is_contiguous():
-            raise ValueError("row_weight must be contiguous float32 or bfloat16")
-        if row_src is None or row_src.dtype != torch.int32 or row_src.numel() < max_rows:
-            raise ValueError("row_weight needs row_src (int32, one entry per row)")
-        a.row_weight = _ptr(row_weight)
-        a.row_weight_bf16 = int(row_weight.dtype == torch.bfloat16)
-        a.row_src = _ptr(row_src)
-    a.out = _ptr(out)
-    a.ldo = out.stride(0) if out.shape[0] > 1 else out.shape[1]
-    check(lib.b200moe_int8_gemm(device, _stream(device), ctypes.byref(a), _ptr(rows.q), _ptr(rows.scale),
-                                _ptr(weight_scale), _ptr(bias)), "int8_gemm")
+    rows.checked(torch.int8, k_pad, weight.device)
+    a = _int8_args(offsets=offsets, expert_begin=expert_begin, n_experts=n_experts, max_rows=max_rows, planes=planes,
+                   feat_pad=feat_pad, n_feat=n_feat, k_pad=k_pad, weight=weight, weight_scale=weight_scale,
+                   b_rows=rows.q.shape[0], epilogue=epilogue, bias=bias, alpha=alpha, limit=limit,
+                   row_weight=row_weight, row_src=row_src, out=out, token_tile=token_tile, device=device)
+    check(lib.b200moe_int8_gemm(device, _stream(device), ctypes.byref(a), rows.q.data_ptr(), rows.scale.data_ptr(),
+                                weight_scale.data_ptr(), _ptr(bias)), "int8_gemm")
+    return out
+
+
+def int8_project(x: torch.Tensor, *, offsets: torch.Tensor | None, expert_begin: int, n_experts: int, planes: int,
+                 feat_pad: int, n_feat: int, k_pad: int, weight: torch.Tensor, weight_scale: torch.Tensor,
+                 epilogue: int, bias: torch.Tensor | None = None, alpha: float = 1.702, limit: float = 7.0,
+                 inverse: torch.Tensor | None = None, copies: int = 1, row_weight: torch.Tensor | None = None,
+                 row_src: torch.Tensor | None = None, out: torch.Tensor, token_tile: int = 0) -> torch.Tensor:
+    """``act_quant_int8`` of bf16 rows ``x`` (each to its ``copies`` places
+    ``inverse`` of the permuted order) and ``int8_gemm`` on them, in one
+    library call (b200moe_int8_project): the weights' first tiles load while
+    the rows are quantised."""
+    device = _dev(weight, "weight")
+    if x.dtype != torch.bfloat16 or x.dim() != 2 or x.stride(1) != 1 or x.get_device() != device:
+        raise ValueError(f"x must be a 2-D bfloat16 tensor with unit column stride on {weight.device}")
+    rows, k_valid = x.shape
+    R = rows
+    if inverse is not None:
+        _inverse_rows(inverse, rows, copies, device)
+        R = rows * copies
+    elif copies != 1:
+        raise ValueError("copies need inverse")
+    a = _int8_args(offsets=offsets, expert_begin=expert_begin, n_experts=n_experts, max_rows=R, planes=planes,
+                   feat_pad=feat_pad, n_feat=n_feat, k_pad=k_pad, weight=weight, weight_scale=weight_scale,
+                   b_rows=R, epilogue=epilogue, bias=bias, alpha=alpha, limit=limit, row_weight=row_weight,
+                   row_src=row_src, out=out, token_tile=token_tile, device=device)
+    nbytes = lib.b200moe_int8_project_workspace(R, k_pad)
+    ws = torch.empty(nbytes, device=weight.device, dtype=torch.uint8)
+    check(lib.b200moe_int8_project(device, _stream(device), ctypes.byref(a), x.data_ptr(),
+                                   x.stride(0) if rows > 1 else k_valid, rows, k_valid, _ptr(inverse), copies,
+                                   weight_scale.data_ptr(), _ptr(bias), ws.data_ptr(), nbytes), "int8_project")
     return out
 
 
