@@ -20,7 +20,7 @@ from functools import lru_cache
 import torch
 
 from moe_serving_profile_b200 import _lib, ops
-from moe_serving_profile_b200.layout import ExpertWeights, Int8Linear
+from moe_serving_profile_b200.layout import ExpertWeights
 
 
 @lru_cache(maxsize=None)
@@ -138,16 +138,6 @@ def _int8_tile(rows: int, experts: int) -> int:
     return 16 if want <= 16 else min(256, 1 << (want - 1).bit_length())
 
 
-def _w1(w: ExpertWeights) -> dict:
-    return dict(planes=2, feat_pad=w.i_pad, n_feat=w.inter, k_pad=w.h_k, weight=w.w1, weight_scale=w.s1, bias=w.b1,
-                epilogue=w.gated_epilogue, alpha=w.alpha, limit=w.limit, n_experts=w.n_experts)
-
-
-def _w2(w: ExpertWeights) -> dict:
-    return dict(planes=1, feat_pad=w.h_f, n_feat=w.hidden, k_pad=w.i_pad, weight=w.w2, weight_scale=w.s2, bias=w.b2,
-                epilogue=_lib.EPI_DOWN_ONCE, n_experts=w.n_experts)
-
-
 def int8_gate_up(w: ExpertWeights, hidden: torch.Tensor | ops.QuantRows, perm: ops.Permutation, *, K: int,
                  num_experts: int, expert_begin: int, copies: int | None = None,
                  out: torch.Tensor | None = None) -> torch.Tensor:
@@ -163,12 +153,11 @@ def int8_gate_up(w: ExpertWeights, hidden: torch.Tensor | ops.QuantRows, perm: o
     if isinstance(hidden, ops.QuantRows):
         rows = ops.scatter_rows_8bit(hidden.checked(torch.int8, w.h_k, w.w1.device), perm.inverse, copies,
                                      **_local_range(w, perm, num_experts, expert_begin))
-        return ops.int8_gemm(offsets=perm.offsets, expert_begin=expert_begin, max_rows=R, rows=rows, out=act,
-                             token_tile=tile, **_w1(w))
+        return ops.int8_gemm(w.m1, rows, offsets=perm.offsets, expert_begin=expert_begin, out=act, token_tile=tile)
     if hidden.shape[1] != w.hidden:
         raise ValueError(f"hidden size {hidden.shape[1]} does not match the experts' {w.hidden}")
-    return ops.int8_project(hidden, offsets=perm.offsets, expert_begin=expert_begin, inverse=perm.inverse,
-                            copies=copies, out=act, token_tile=tile, **_w1(w))
+    return ops.int8_project(w.m1, hidden, offsets=perm.offsets, expert_begin=expert_begin, inverse=perm.inverse,
+                            copies=copies, out=act, token_tile=tile)
 
 
 def int8_down(w: ExpertWeights, act: torch.Tensor, perm: ops.Permutation, weights: torch.Tensor | None, *, K: int,
@@ -179,14 +168,13 @@ def int8_down(w: ExpertWeights, act: torch.Tensor, perm: ops.Permutation, weight
     if w.fmt != _lib.W_INT8:
         raise ValueError("int8_down needs int8 expert weights")
     R = perm.perm_src.numel()
-    if act.shape[0] != R or act.shape[1] < w.inter:
-        raise ValueError(f"act must be [{R}, {w.inter} or more], got {tuple(act.shape)}")
+    if act.shape[0] != R:
+        raise ValueError(f"act must have a row for each of the {R} assignments, got {act.shape[0]}")
     if contrib is None:
         contrib = torch.empty(R, w.hidden, device=act.device, dtype=torch.bfloat16)
-    return ops.int8_project(act if act.shape[1] == w.inter else act[:, :w.inter], offsets=perm.offsets,
-                            expert_begin=expert_begin, row_weight=weights,
+    return ops.int8_project(w.m2, act, offsets=perm.offsets, expert_begin=expert_begin, row_weight=weights,
                             row_src=None if weights is None else perm.perm_src, out=contrib,
-                            token_tile=_int8_tile(R, num_experts), **_w2(w))
+                            token_tile=_int8_tile(R, num_experts))
 
 
 def run_experts_int8(w: ExpertWeights, hidden: torch.Tensor | ops.QuantRows, perm: ops.Permutation,
@@ -209,9 +197,9 @@ def run_experts_int8_placed(w: ExpertWeights, x: torch.Tensor, offsets: torch.Te
     R = x.shape[0]
     kw = dict(offsets=offsets, expert_begin=0, token_tile=_int8_tile(tokens, w.n_experts))
     act = torch.empty(R, w.i_pad, device=x.device, dtype=torch.bfloat16)
-    ops.int8_project(x, out=act, **kw, **_w1(w))
+    ops.int8_project(w.m1, x, out=act, **kw)
     y = torch.empty(R, w.hidden, device=x.device, dtype=torch.bfloat16)
-    return ops.int8_project(act[:, :w.inter], out=y, **kw, **_w2(w))
+    return ops.int8_project(w.m2, act, out=y, **kw)
 
 
 def int8_swiglu(w: ExpertWeights, x: torch.Tensor) -> torch.Tensor:
@@ -220,23 +208,25 @@ def int8_swiglu(w: ExpertWeights, x: torch.Tensor) -> torch.Tensor:
         raise ValueError("int8_swiglu needs the int8 weights of one expert")
     T = x.shape[0]
     act = torch.empty(T, w.i_pad, device=x.device, dtype=torch.bfloat16)
-    ops.int8_project(x, offsets=None, expert_begin=0, out=act, **_w1(w))
+    ops.int8_project(w.m1, x, out=act)
     y = torch.empty(T, w.hidden, device=x.device, dtype=torch.bfloat16)
-    return ops.int8_project(act[:, :w.inter], offsets=None, expert_begin=0, out=y, **_w2(w))
+    return ops.int8_project(w.m2, act, out=y)
 
 
-def int8_linear(w: Int8Linear, x: torch.Tensor | ops.QuantRows, out: torch.Tensor | None = None) -> torch.Tensor:
-    """Dense int8 projection of bf16 rows ``x`` [T, K], or of rows a norm
-    already quantised: bf16 [T, N]."""
-    quantised = isinstance(x, ops.QuantRows)
-    T = (x.q if quantised else x).shape[0]
-    if not quantised and x.shape[-1] != w.in_features:
-        raise ValueError(f"x has {x.shape[-1]} columns, the projection takes {w.in_features}")
+def int8_linear(w: ops.Int8Matrix, x: torch.Tensor | ops.QuantRows, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Dense int8 projection (layout.int8_linear's weights) of bf16 rows ``x``
+    [T, K], or of rows a norm already quantised: bf16 [T, N]."""
+    if w.n_experts != 1 or w.planes != 1:
+        raise ValueError("int8_linear needs the weights of layout.int8_linear")
+    if isinstance(x, ops.QuantRows):
+        if out is None:
+            out = torch.empty(x.q.shape[0], w.n_feat, device=w.weight.device, dtype=torch.bfloat16)
+        return ops.int8_gemm(w, x, out=out)
+    if x.shape[-1] != w.k_valid:
+        raise ValueError(f"x has {x.shape[-1]} columns, the projection takes {w.k_valid}")
     if out is None:
-        out = torch.empty(T, w.out_features, device=w.w.device, dtype=torch.bfloat16)
-    kw = dict(offsets=None, expert_begin=0, n_experts=1, planes=1, feat_pad=w.n_pad, n_feat=w.out_features,
-              k_pad=w.k_pad, weight=w.w, weight_scale=w.scale, epilogue=_lib.EPI_DOWN_ONCE, bias=w.bias, out=out)
-    return ops.int8_gemm(max_rows=T, rows=x, **kw) if quantised else ops.int8_project(x, **kw)
+        out = torch.empty(x.shape[0], w.n_feat, device=w.weight.device, dtype=torch.bfloat16)
+    return ops.int8_project(w, x, out=out)
 
 
 def run_experts_w8a8(w: ExpertWeights, hidden: torch.Tensor, perm: ops.Permutation,

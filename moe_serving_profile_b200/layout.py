@@ -39,6 +39,7 @@ from dataclasses import dataclass
 import torch
 
 from moe_serving_profile_b200 import _lib
+from moe_serving_profile_b200.ops import Int8Matrix
 
 
 def _ceil(v: int, m: int) -> int:
@@ -48,8 +49,9 @@ def _ceil(v: int, m: int) -> int:
 @dataclass
 class ExpertWeights:
     """One layer's local experts in device layout: w1 (gate/up) and w2 (down)
-    are bf16 [E, planes, F_p, K_p] for BF16 weights and packed blobs
-    [E, feature tiles, K_p / 64, blob bytes] for FP8 / MXFP4 (scales inside)."""
+    are bf16 [E, planes, F_p, K_p] for BF16 weights, packed blobs [E, feature
+    tiles, K_p / 64, blob bytes] for FP8 / MXFP4 (scales inside) and tiles for
+    int8 (m1 / m2 describe them, s1 / s2 and b1 / b2 are their scales and biases)."""
 
     fmt: int
     n_experts: int
@@ -65,6 +67,8 @@ class ExpertWeights:
     gated_epilogue: int = _lib.EPI_SWIGLU
     alpha: float = 1.702
     limit: float = 7.0
+    m1: Int8Matrix | None = None
+    m2: Int8Matrix | None = None
 
     @property
     def i_pad(self) -> int:
@@ -215,28 +219,32 @@ def quantize_int8(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 
 
 def _int8_rows(t: torch.Tensor) -> torch.Tensor:
-    """[planes, F_p, ...] -> [feat_tiles, 128, ...] in the int8 tiles' row
+    """[E, planes, F_p, ...] -> [E, feat_tiles, 128, ...] in the int8 tiles' row
     order (two planes: 16 gate rows, then the 16 up rows of the same features)."""
-    P, F = t.shape[:2]
-    rest = tuple(t.shape[2:])
+    E, P, F = t.shape[:3]
+    rest = tuple(t.shape[3:])
     if P == 2:
-        return t.reshape(2, F // 16, 16, *rest).transpose(0, 1).reshape(F // 64, 128, *rest)
-    return t.reshape(F // 128, 128, *rest)
+        return t.reshape(E, 2, F // 16, 16, *rest).transpose(1, 2).reshape(E, F // 64, 128, *rest)
+    return t.reshape(E, F // 128, 128, *rest)
 
 
 def _int8_tiles(w: torch.Tensor, feat_pad: int, k_pad: int) -> torch.Tensor:
     """int8 [E, planes, F, K] -> [E, feat_tiles, k_pad / 128, 128, 128] images."""
     E, P, F, K = w.shape
-    ft = feat_pad // (64 if P == 2 else 128)
-    out = torch.empty(E, ft, k_pad // 128, 128, 128, device=w.device, dtype=torch.int8)
+    ft, nkb = feat_pad // (64 if P == 2 else 128), k_pad // 128
+    out = torch.empty(E, ft, nkb, 128, 128, device=w.device, dtype=torch.int8)
+    words = out.view(torch.int64).view(E, ft, nkb, 16, 8, 8, 2)     # [.., row / 8, row % 8, 16-byte chunk, word]
     chunk = torch.arange(8, device=w.device)
-    for e in range(E):   # one expert at a time bounds the scratch memory
-        full = torch.zeros(P, feat_pad, k_pad, device=w.device, dtype=torch.int8)
-        full[:, :F, :K] = w[e]
-        rows = _int8_rows(full).reshape(ft, 16, 8, k_pad // 128, 8, 16)   # [tile, row / 8, row % 8, block, chunk, 16]
-        dst = out[e].view(ft, k_pad // 128, 16, 8, 8, 16)
+    step = max(1, (256 << 20) // (P * feat_pad * k_pad))            # experts at a time: bounds the scratch memory
+    for e in range(0, E, step):
+        part = w[e:e + step]
+        if (F, K) != (feat_pad, k_pad) or not part.is_contiguous() or part.data_ptr() % 8:
+            full = torch.zeros(part.shape[0], P, feat_pad, k_pad, device=w.device, dtype=torch.int8)
+            full[:, :, :F, :K] = part
+            part = full
+        rows = _int8_rows(part.view(torch.int64)).view(-1, ft, 16, 8, nkb, 8, 2)
         for r in range(8):
-            dst[:, :, :, r] = rows[:, :, r].index_select(3, chunk ^ r).transpose(1, 2)
+            words[e:e + step, :, :, :, r] = rows[:, :, :, r].index_select(4, chunk ^ r).transpose(2, 3)
     return out
 
 
@@ -247,7 +255,7 @@ def _int8_channels(v: torch.Tensor | None, feat_pad: int) -> torch.Tensor | None
     E, P, F = v.shape
     full = torch.zeros(E, P, feat_pad, device=v.device, dtype=torch.float32)
     full[:, :, :F] = v
-    return torch.stack([_int8_rows(full[e]) for e in range(E)])
+    return _int8_rows(full).contiguous()
 
 
 def _check_int8(w: torch.Tensor, scale: torch.Tensor, what: str) -> None:
@@ -255,6 +263,16 @@ def _check_int8(w: torch.Tensor, scale: torch.Tensor, what: str) -> None:
         raise ValueError(f"{what} weights must be int8, got {w.dtype}")
     if scale.shape != w.shape[:-1]:
         raise ValueError(f"{what} needs one scale per channel {tuple(w.shape[:-1])}, got {tuple(scale.shape)}")
+
+
+def _planes(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
+    """[E, 2, I, H] of the two; no copy where they already lie so in memory."""
+    E, inter, hidden = gate.shape
+    size = inter * hidden
+    if (gate.stride() == up.stride() == (2 * size, hidden, 1) and up.data_ptr() == gate.data_ptr() + size
+            and gate.untyped_storage().data_ptr() == up.untyped_storage().data_ptr()):
+        return gate.as_strided((E, 2, inter, hidden), (2 * size, size, hidden, 1))
+    return torch.stack([gate, up], dim=1)
 
 
 def int8_experts(gate: torch.Tensor, gate_scale: torch.Tensor, up: torch.Tensor, up_scale: torch.Tensor,
@@ -277,13 +295,13 @@ def int8_experts(gate: torch.Tensor, gate_scale: torch.Tensor, up: torch.Tensor,
     I_p, H_p = _ceil(inter, 128), _ceil(hidden, 128)
     b1 = None if gate_bias is None else torch.stack([gate_bias.float(), up_bias.float()], dim=1)
     b2 = None if down_bias is None else down_bias.float()[:, None]
-    return ExpertWeights(_lib.W_INT8, E, hidden, inter,
-                         _int8_tiles(torch.stack([gate, up], dim=1), I_p, H_p),
-                         _int8_tiles(down[:, None], H_p, I_p),
-                         s1=_int8_channels(torch.stack([gate_scale.float(), up_scale.float()], dim=1), I_p),
-                         s2=_int8_channels(down_scale.float()[:, None], H_p),
-                         b1=_int8_channels(b1, I_p), b2=_int8_channels(b2, H_p),
-                         gated_epilogue=gated_epilogue, alpha=alpha, limit=limit)
+    m1 = Int8Matrix(E, 2, inter, hidden, I_p, H_p, _int8_tiles(_planes(gate, up), I_p, H_p),
+                    _int8_channels(torch.stack([gate_scale.float(), up_scale.float()], dim=1), I_p),
+                    _int8_channels(b1, I_p), gated_epilogue, alpha, limit)
+    m2 = Int8Matrix(E, 1, hidden, inter, H_p, I_p, _int8_tiles(down[:, None], H_p, I_p),
+                    _int8_channels(down_scale.float()[:, None], H_p), _int8_channels(b2, H_p), _lib.EPI_DOWN_ONCE)
+    return ExpertWeights(_lib.W_INT8, E, hidden, inter, m1.weight, m2.weight, s1=m1.scale, s2=m2.scale, b1=m1.bias,
+                         b2=m2.bias, gated_epilogue=gated_epilogue, alpha=alpha, limit=limit, m1=m1, m2=m2)
 
 
 def int8_experts_from(gate: torch.Tensor, up: torch.Tensor, down: torch.Tensor, **more) -> ExpertWeights:
@@ -292,36 +310,18 @@ def int8_experts_from(gate: torch.Tensor, up: torch.Tensor, down: torch.Tensor, 
     return int8_experts(*parts, **more)
 
 
-@dataclass
-class Int8Linear:
-    """A dense int8 projection [out_features, in_features] in tile layout."""
-
-    out_features: int
-    in_features: int
-    w: torch.Tensor
-    scale: torch.Tensor
-    bias: torch.Tensor | None = None
-
-    @property
-    def n_pad(self) -> int:
-        return _ceil(self.out_features, 128)
-
-    @property
-    def k_pad(self) -> int:
-        return _ceil(self.in_features, 128)
-
-
-def int8_linear(weight: torch.Tensor, scale: torch.Tensor, bias: torch.Tensor | None = None) -> Int8Linear:
-    """int8 weight [N, K] with one scale per output channel [N], bias [N]."""
+def int8_linear(weight: torch.Tensor, scale: torch.Tensor, bias: torch.Tensor | None = None) -> Int8Matrix:
+    """A dense projection: int8 weight [N, K] with one scale per output channel
+    [N], bias [N]."""
     if weight.dim() != 2:
         raise ValueError("weight must be [out_features, in_features]")
     _check_int8(weight, scale, "linear")
     N, K = weight.shape
     _check_dims(K, N)
     N_p, K_p = _ceil(N, 128), _ceil(K, 128)
-    return Int8Linear(N, K, _int8_tiles(weight[None, None], N_p, K_p),
+    return Int8Matrix(1, 1, N, K, N_p, K_p, _int8_tiles(weight[None, None], N_p, K_p),
                       _int8_channels(scale.float()[None, None], N_p),
-                      _int8_channels(None if bias is None else bias.float()[None, None], N_p))
+                      _int8_channels(None if bias is None else bias.float()[None, None], N_p), _lib.EPI_DOWN_ONCE)
 
 
 def bf16_experts(gate: torch.Tensor, up: torch.Tensor, down: torch.Tensor,

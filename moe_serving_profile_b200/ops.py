@@ -98,6 +98,7 @@ def _same_device(t: torch.Tensor | None, device: int, what: str) -> None:
         raise ValueError(f"{what} must be on cuda:{device}, got {t.device}")
 
 
+_BF16_FLAG = {torch.float32: 0, torch.bfloat16: 1}   # the C calls' fp32 / bf16 switch
 SCORING = {"sigmoid": _lib.SCORE_SIGMOID, "softmax": _lib.SCORE_SOFTMAX}
 
 
@@ -112,15 +113,20 @@ def route_grouped(logits: torch.Tensor, bias: torch.Tensor | None, top_k: int, *
     the lower id), their scores renormalised and times ``scale``. scores are
     fp32 [T, K] in descending order of the keys."""
     device = _dev(logits, "logits")
-    if logits.dtype not in (torch.float32, torch.bfloat16) or logits.dim() != 2 or logits.stride(1) != 1:
+    bf = _BF16_FLAG.get(logits.dtype)
+    sl = logits.stride()
+    if bf is None or len(sl) != 2 or sl[1] != 1:
         raise ValueError("logits must be a 2D float32 or bfloat16 tensor with contiguous rows")
-    if scoring not in SCORING:
+    mode = SCORING.get(scoring)
+    if mode is None:
         raise ValueError(f"scoring must be one of {tuple(SCORING)}, got {scoring!r}")
     T, E = logits.shape
+    pb = None
     if bias is not None:
-        _same_device(bias, device, "bias")
-        if bias.dtype != torch.float32 or bias.shape != (E,) or not bias.is_contiguous():
-            raise ValueError(f"bias must be contiguous float32 [{E}]")
+        if (bias.dtype != torch.float32 or bias.shape != (E,) or not bias.is_contiguous()
+                or bias.get_device() != device):
+            raise ValueError(f"bias must be contiguous float32 [{E}] on {logits.device}")
+        pb = bias.data_ptr()
     if not 1 <= top_k <= E:   # before the outputs of that width are allocated
         raise ValueError(f"top_k must be in [1, {E}], got {top_k}")
     dev = logits.device
@@ -129,9 +135,9 @@ def route_grouped(logits: torch.Tensor, bias: torch.Tensor | None, top_k: int, *
     counts = torch.empty(E, device=dev, dtype=torch.int32)
     check(
         lib.b200moe_route_grouped(
-            device, _stream(device), _ptr(logits), int(logits.dtype == torch.bfloat16),
-            logits.stride(0) if T > 1 else E, _ptr(bias), T, E, top_k, n_group, topk_group, group_top,
-            SCORING[scoring], int(normalize), float(scale), _ptr(scores), _ptr(indices), _ptr(counts),
+            device, _stream(device), logits.data_ptr(), bf, sl[0] if T > 1 else E, pb, T, E, top_k, n_group,
+            topk_group, group_top, mode, int(normalize), scale, scores.data_ptr(), indices.data_ptr(),
+            counts.data_ptr(),
         ),
         "route_grouped",
     )
@@ -208,14 +214,14 @@ class QuantRows:
 
     def checked(self, dtype: torch.dtype, k_pad: int, device: torch.device) -> "QuantRows":
         """Self, if these are ``dtype`` rows of width ``k_pad`` on ``device``."""
-        rows = self.q.shape[0]
-        shape = (rows,) if dtype == torch.int8 else (rows, -(-k_pad // 128))
-        if self.q.dtype != dtype or self.q.dim() != 2 or self.q.shape[1] != k_pad or not self.q.is_contiguous():
-            raise ValueError(f"quantised rows must be contiguous {dtype} [rows, {k_pad}], got {self.q.dtype} "
-                             f"{tuple(self.q.shape)}")
-        if self.scale.dtype != torch.float32 or tuple(self.scale.shape) != shape or not self.scale.is_contiguous():
-            raise ValueError(f"row scales must be contiguous float32 {shape}")
-        if self.q.device != device or self.scale.device != device:
+        q, scale = self.q, self.scale
+        if q.dtype != dtype or q.dim() != 2 or q.shape[1] != k_pad or not q.is_contiguous():
+            raise ValueError(f"quantised rows must be contiguous {dtype} [rows, {k_pad}], got {q.dtype} "
+                             f"{tuple(q.shape)}")
+        shape = q.shape[:1] if dtype == torch.int8 else (q.shape[0], -(-k_pad // 128))
+        if scale.dtype != torch.float32 or scale.shape != shape or not scale.is_contiguous():
+            raise ValueError(f"row scales must be contiguous float32 {tuple(shape)}")
+        if q.device != device or scale.device != device:
             raise ValueError(f"quantised rows must be on {device}")
         return self
 
@@ -303,12 +309,11 @@ QUANT = {None: _lib.QUANT_NONE, "fp8": _lib.QUANT_FP8, "int8": _lib.QUANT_INT8}
 
 def _residual_rows(t: torch.Tensor, x: torch.Tensor, device: int, what: str) -> int:
     """The row stride of a residual, checked against ``x``."""
-    _bf16_rows(t, what)
-    if t.get_device() != device:
-        raise ValueError(f"{what} must be on cuda:{device}, got {t.device}")
-    if t.shape != x.shape:
-        raise ValueError(f"{what} must have x's shape {tuple(x.shape)}, got {tuple(t.shape)}")
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    st = t.stride()
+    if t.dtype != torch.bfloat16 or t.shape != x.shape or st[1] != 1 or t.get_device() != device:
+        raise ValueError(f"{what} must be bfloat16 {tuple(x.shape)} with contiguous rows on {x.device}, got {t.dtype} "
+                         f"{tuple(t.shape)} on {t.device}")
+    return st[0] if t.shape[0] > 1 else t.shape[1]
 
 
 def add_rmsnorm(x: torch.Tensor, weight: torch.Tensor, eps: float, *, residual: torch.Tensor | None = None,
@@ -321,45 +326,49 @@ def add_rmsnorm(x: torch.Tensor, weight: torch.Tensor, eps: float, *, residual: 
     FP8 or the int8 experts, padded to ``k_pad`` columns (default: what those
     experts take); ``normed=False`` leaves the bf16 output out."""
     device = _dev(x, "x")
-    _bf16_rows(x, "x")
-    if quant not in QUANT:
+    sx = x.stride()
+    if x.dtype != torch.bfloat16 or len(sx) != 2 or sx[1] != 1:
+        raise ValueError("x must be a 2D bfloat16 tensor with contiguous rows")
+    mode = QUANT.get(quant)
+    if mode is None:
         raise ValueError(f"quant must be one of {tuple(QUANT)}, got {quant!r}")
     T, H = x.shape
-    if weight.dtype not in (torch.bfloat16, torch.float32) or weight.shape != (H,) or not weight.is_contiguous():
+    f32 = weight.dtype == torch.float32
+    if not (f32 or weight.dtype == torch.bfloat16) or weight.shape != (H,) or not weight.is_contiguous():
         raise ValueError(f"weight must be contiguous bfloat16 or float32 [{H}]")
-    _same_device(weight, device, "weight")
-    if quant is None and not normed:
+    if weight.get_device() != device:
+        raise ValueError(f"weight must be on cuda:{device}, got {weight.device}")
+    if not mode and not normed:
         raise ValueError("nothing to compute: no quantised rows and no bf16 output")
     dev = x.device
     ldr = ldro = 0
+    pr = pro = po = pq = ps = None
     if residual is not None:
-        ldr = _residual_rows(residual, x, device, "residual")
+        ldr, pr = _residual_rows(residual, x, device, "residual"), residual.data_ptr()
         if residual_out is None:
-            residual_out, ldro = torch.empty((T, H), device=dev, dtype=torch.bfloat16), H
+            residual_out, ldro = torch.empty(T, H, device=dev, dtype=torch.bfloat16), H
         else:
             ldro = _residual_rows(residual_out, x, device, "residual_out")
+        pro = residual_out.data_ptr()
     elif residual_out is not None:
         raise ValueError("residual_out needs a residual")
-    out = torch.empty((T, H), device=dev, dtype=torch.bfloat16) if normed else None
-    rows = q = scale = None
-    if quant is None:
-        k_pad = 0
-    elif quant == "fp8":
-        k_pad = -(-H // 64) * 64 if k_pad is None else k_pad
-        q = torch.empty((T, k_pad), device=dev, dtype=torch.float8_e4m3fn)
-        scale = torch.empty((T, -(-k_pad // 128)), device=dev, dtype=torch.float32)
-        rows = QuantRows(q, scale)
-    else:
-        k_pad = -(-H // 128) * 128 if k_pad is None else k_pad
-        q = torch.empty((T, k_pad), device=dev, dtype=torch.int8)
-        scale = torch.empty((T,), device=dev, dtype=torch.float32)
-        rows = QuantRows(q, scale)
+    out = rows = None
+    if normed:
+        out = torch.empty(T, H, device=dev, dtype=torch.bfloat16)
+        po = out.data_ptr()
+    if mode:
+        if k_pad is None:   # what the experts of that form take
+            k_pad = -(-H // 64) * 64 if quant == "fp8" else -(-H // 128) * 128
+        if quant == "fp8":
+            q = torch.empty(T, k_pad, device=dev, dtype=torch.float8_e4m3fn)
+            scale = torch.empty(T, -(-k_pad // 128), device=dev, dtype=torch.float32)
+        else:
+            q = torch.empty(T, k_pad, device=dev, dtype=torch.int8)
+            scale = torch.empty(T, device=dev, dtype=torch.float32)
+        rows, pq, ps = QuantRows(q, scale), q.data_ptr(), scale.data_ptr()
     check(
-        lib.b200moe_add_rmsnorm(
-            device, _stream(device), x.data_ptr(), x.stride(0) if T > 1 else H, _ptr(residual), ldr,
-            _ptr(residual_out), ldro, weight.data_ptr(), int(weight.dtype == torch.float32), eps, T, H, _ptr(out), H,
-            QUANT[quant], _ptr(q), k_pad, _ptr(scale),
-        ),
+        lib.b200moe_add_rmsnorm(device, _stream(device), x.data_ptr(), sx[0] if T > 1 else H, pr, ldr, pro, ldro,
+                                weight.data_ptr(), int(f32), eps, T, H, po, H, mode, pq, k_pad or 0, ps),
         "add_rmsnorm",
     )
     return NormOut(out, residual_out, rows)
@@ -552,89 +561,112 @@ def w8a8_gemm(*, offsets: torch.Tensor, expert_begin: int, n_experts: int, max_r
     return out
 
 
-def _int8_args(*, offsets, expert_begin, n_experts, max_rows, planes, feat_pad, n_feat, k_pad, weight, weight_scale,
-               b_rows, epilogue, bias, alpha, limit, row_weight, row_src, out, token_tile, device):
-    """The checked GemmArgs of an int8 launch (positional: the fields of
-    b200moe_gemm_args in order)."""
-    tiles = n_experts * (feat_pad // (64 if planes == 2 else 128))
-    if weight.dtype != torch.int8 or not weight.is_contiguous() or weight.numel() != tiles * 128 * k_pad:
-        raise ValueError(f"weight must be contiguous int8 tiles of {tiles * 128 * k_pad} elements")
-    for t, what in ((weight_scale, "weight_scale"), (bias, "bias")):
-        if t is not None and (t.dtype != torch.float32 or not t.is_contiguous() or t.numel() != tiles * 128
-                              or t.get_device() != device):
-            raise ValueError(f"{what} must be contiguous float32 of {tiles * 128} elements on {weight.device}")
-    if out.dtype != torch.bfloat16 or out.dim() != 2 or out.stride(1) != 1:
-        raise ValueError("output must be a 2D bfloat16 tensor with contiguous rows")
-    rows_out, cols_out = out.shape
-    if out.get_device() != device or rows_out < max_rows or cols_out < n_feat:
-        raise ValueError(f"output must hold {max_rows} rows of {n_feat} columns on {weight.device}")
-    if offsets is not None and (offsets.get_device() != device or offsets.dtype != torch.int32
-                                or not offsets.is_contiguous() or offsets.numel() <= expert_begin + n_experts):
-        raise ValueError(f"offsets must be contiguous int32 covering the experts, on {weight.device}")
-    rw = rs = None
+@dataclass
+class Int8Matrix:
+    """Int8 weights in tile layout (layout.int8_experts / int8_linear) with
+    what the int8 GEMM has to know of them; checked once, here."""
+
+    n_experts: int
+    planes: int              # 2: gate and up, 1: one projection
+    n_feat: int              # output features (of a plane)
+    k_valid: int             # input columns
+    feat_pad: int
+    k_pad: int
+    weight: torch.Tensor     # int8 tiles
+    scale: torch.Tensor      # fp32 per channel, tile row order
+    bias: torch.Tensor | None
+    epilogue: int
+    alpha: float = 1.702
+    limit: float = 7.0
+
+    def __post_init__(self):
+        tiles = self.n_experts * (self.feat_pad // (64 if self.planes == 2 else 128))
+        w = self.weight
+        if w.dtype != torch.int8 or not w.is_contiguous() or w.numel() != tiles * 128 * self.k_pad:
+            raise ValueError(f"weight must be contiguous int8 tiles of {tiles * 128 * self.k_pad} elements")
+        for t, what in ((self.scale, "scale"), (self.bias, "bias")):
+            if t is not None and (t.dtype != torch.float32 or not t.is_contiguous() or t.numel() != tiles * 128
+                                  or t.device != w.device):
+                raise ValueError(f"{what} must be contiguous float32 of {tiles * 128} elements on {w.device}")
+
+
+def _int8_args(m: Int8Matrix, device: int, offsets, expert_begin: int, R: int, b_rows: int, row_weight, row_src, out,
+               token_tile: int):
+    """The GemmArgs of an int8 launch (the fields of b200moe_gemm_args in order)."""
+    so = out.stride()
+    if out.dtype != torch.bfloat16 or len(so) != 2 or so[1] != 1 or out.get_device() != device:
+        raise ValueError(f"output must be a 2D bfloat16 tensor with contiguous rows on {m.weight.device}")
+    ro, co = out.shape
+    if ro < R or co < m.n_feat:
+        raise ValueError(f"output must hold {R} rows of {m.n_feat} columns, got {tuple(out.shape)}")
+    po = prw = prs = None
+    bf = 0
+    if offsets is not None:
+        if (offsets.get_device() != device or offsets.dtype != torch.int32 or not offsets.is_contiguous()
+                or offsets.numel() <= expert_begin + m.n_experts):
+            raise ValueError(f"offsets must be contiguous int32 covering the experts, on {m.weight.device}")
+        po = offsets.data_ptr()
     if row_weight is not None:
-        if (row_weight.dtype not in (torch.float32, torch.bfloat16) or not row_weight.is_contiguous()
-                or row_weight.get_device() != device or row_weight.numel() < max_rows):
-            raise ValueError(f"row_weight must be contiguous float32 or bfloat16, one per row, on {weight.device}")
-        if (row_src is None or row_src.dtype != torch.int32 or row_src.numel() < max_rows
-                or not row_src.is_contiguous() or row_src.get_device() != device):
-            raise ValueError(f"row_weight needs row_src (contiguous int32, one entry per row) on {weight.device}")
-        rw, rs = row_weight.data_ptr(), row_src.data_ptr()
+        bf = _BF16_FLAG.get(row_weight.dtype)
+        if (bf is None or not row_weight.is_contiguous() or row_weight.get_device() != device
+                or row_weight.numel() < R):
+            raise ValueError(f"row_weight must be contiguous float32 or bfloat16, one per row, on {m.weight.device}")
+        if (row_src is None or row_src.dtype != torch.int32 or row_src.numel() < R or not row_src.is_contiguous()
+                or row_src.get_device() != device):
+            raise ValueError(f"row_weight needs row_src (contiguous int32, one entry per row) on {m.weight.device}")
+        prw, prs = row_weight.data_ptr(), row_src.data_ptr()
     return _lib.GemmArgs(
-        None if offsets is None else offsets.data_ptr(), expert_begin, n_experts, max_rows, token_tile, 0,
-        _lib.W_INT8, planes, feat_pad, n_feat, k_pad, weight.data_ptr(), 0, 0, None, 0, b_rows, 0, None, 1,
-        epilogue, None, alpha, limit, rw, int(row_weight is not None and row_weight.dtype == torch.bfloat16), rs,
-        out.data_ptr(), out.stride(0) if rows_out > 1 else cols_out)
+        po, expert_begin, m.n_experts, R, token_tile, 0, _lib.W_INT8, m.planes, m.feat_pad, m.n_feat, m.k_pad,
+        m.weight.data_ptr(), 0, 0, None, 0, b_rows, 0, None, 1, m.epilogue, None, m.alpha, m.limit, prw, bf, prs,
+        out.data_ptr(), so[0] if ro > 1 else co)
 
 
-def int8_gemm(*, offsets: torch.Tensor | None, expert_begin: int, n_experts: int, max_rows: int, planes: int,
-              feat_pad: int, n_feat: int, k_pad: int, weight: torch.Tensor, weight_scale: torch.Tensor,
-              rows: QuantRows, epilogue: int, bias: torch.Tensor | None = None, alpha: float = 1.702,
-              limit: float = 7.0, row_weight: torch.Tensor | None = None, row_src: torch.Tensor | None = None,
-              out: torch.Tensor, token_tile: int = 0) -> torch.Tensor:
-    """Int8 grouped GEMM (b200moe_int8_gemm): int8 weight tiles with one fp32
-    scale per channel times int8 permuted rows with one scale each
-    (``act_quant_int8``'s outputs). ``offsets`` None: one expert holds all
-    ``max_rows`` rows."""
-    device = _dev(weight, "weight")
-    rows.checked(torch.int8, k_pad, weight.device)
-    a = _int8_args(offsets=offsets, expert_begin=expert_begin, n_experts=n_experts, max_rows=max_rows, planes=planes,
-                   feat_pad=feat_pad, n_feat=n_feat, k_pad=k_pad, weight=weight, weight_scale=weight_scale,
-                   b_rows=rows.q.shape[0], epilogue=epilogue, bias=bias, alpha=alpha, limit=limit,
-                   row_weight=row_weight, row_src=row_src, out=out, token_tile=token_tile, device=device)
+def int8_gemm(m: Int8Matrix, rows: QuantRows, *, offsets: torch.Tensor | None = None, expert_begin: int = 0,
+              max_rows: int | None = None, row_weight: torch.Tensor | None = None,
+              row_src: torch.Tensor | None = None, out: torch.Tensor, token_tile: int = 0) -> torch.Tensor:
+    """Int8 grouped GEMM (b200moe_int8_gemm) of int8 permuted rows with one
+    scale each (``act_quant_int8``'s outputs). ``offsets`` None: one expert
+    holds all rows. ``max_rows``: how many of ``rows`` may be an expert's."""
+    device = _dev(m.weight, "weight")
+    rows.checked(torch.int8, m.k_pad, m.weight.device)
+    n = rows.q.shape[0]
+    R = n if max_rows is None else max_rows
+    a = _int8_args(m, device, offsets, expert_begin, R, n, row_weight, row_src, out, token_tile)
     check(lib.b200moe_int8_gemm(device, _stream(device), ctypes.byref(a), rows.q.data_ptr(), rows.scale.data_ptr(),
-                                weight_scale.data_ptr(), _ptr(bias)), "int8_gemm")
+                                m.scale.data_ptr(), None if m.bias is None else m.bias.data_ptr()), "int8_gemm")
     return out
 
 
-def int8_project(x: torch.Tensor, *, offsets: torch.Tensor | None, expert_begin: int, n_experts: int, planes: int,
-                 feat_pad: int, n_feat: int, k_pad: int, weight: torch.Tensor, weight_scale: torch.Tensor,
-                 epilogue: int, bias: torch.Tensor | None = None, alpha: float = 1.702, limit: float = 7.0,
+def int8_project(m: Int8Matrix, x: torch.Tensor, *, offsets: torch.Tensor | None = None, expert_begin: int = 0,
                  inverse: torch.Tensor | None = None, copies: int = 1, row_weight: torch.Tensor | None = None,
                  row_src: torch.Tensor | None = None, out: torch.Tensor, token_tile: int = 0) -> torch.Tensor:
-    """``act_quant_int8`` of bf16 rows ``x`` (each to its ``copies`` places
-    ``inverse`` of the permuted order) and ``int8_gemm`` on them, in one
-    library call (b200moe_int8_project): the weights' first tiles load while
-    the rows are quantised."""
-    device = _dev(weight, "weight")
-    if x.dtype != torch.bfloat16 or x.dim() != 2 or x.stride(1) != 1 or x.get_device() != device:
-        raise ValueError(f"x must be a 2-D bfloat16 tensor with unit column stride on {weight.device}")
-    rows, k_valid = x.shape
-    R = rows
+    """``act_quant_int8`` of the first ``m.k_valid`` columns of bf16 rows ``x``
+    (each to its ``copies`` places ``inverse`` of the permuted order) and
+    ``int8_gemm`` on them, in one library call (b200moe_int8_project): the
+    weights' first tiles load while the rows are quantised."""
+    device = _dev(m.weight, "weight")
+    sx = x.stride()
+    if x.dtype != torch.bfloat16 or len(sx) != 2 or sx[1] != 1 or x.get_device() != device:
+        raise ValueError(f"x must be a 2-D bfloat16 tensor with unit column stride on {m.weight.device}")
+    rows, cols = x.shape
+    if cols < m.k_valid:
+        raise ValueError(f"x has {cols} columns, the weights take {m.k_valid}")
+    R, inv = rows, None
     if inverse is not None:
-        _inverse_rows(inverse, rows, copies, device)
         R = rows * copies
+        if (inverse.dtype != torch.int32 or not inverse.is_contiguous() or inverse.numel() != R
+                or inverse.get_device() != device):
+            raise ValueError(f"inverse must be contiguous int32 of rows * copies = {R} elements on {m.weight.device}")
+        inv = inverse.data_ptr()
     elif copies != 1:
         raise ValueError("copies need inverse")
-    a = _int8_args(offsets=offsets, expert_begin=expert_begin, n_experts=n_experts, max_rows=R, planes=planes,
-                   feat_pad=feat_pad, n_feat=n_feat, k_pad=k_pad, weight=weight, weight_scale=weight_scale,
-                   b_rows=R, epilogue=epilogue, bias=bias, alpha=alpha, limit=limit, row_weight=row_weight,
-                   row_src=row_src, out=out, token_tile=token_tile, device=device)
-    nbytes = lib.b200moe_int8_project_workspace(R, k_pad)
-    ws = torch.empty(nbytes, device=weight.device, dtype=torch.uint8)
+    a = _int8_args(m, device, offsets, expert_begin, R, R, row_weight, row_src, out, token_tile)
+    nbytes = lib.b200moe_int8_project_workspace(R, m.k_pad)
+    ws = torch.empty(nbytes, device=out.device, dtype=torch.uint8)
     check(lib.b200moe_int8_project(device, _stream(device), ctypes.byref(a), x.data_ptr(),
-                                   x.stride(0) if rows > 1 else k_valid, rows, k_valid, _ptr(inverse), copies,
-                                   weight_scale.data_ptr(), _ptr(bias), ws.data_ptr(), nbytes), "int8_project")
+                                   sx[0] if rows > 1 else m.k_valid, rows, m.k_valid, inv, copies,
+                                   m.scale.data_ptr(), None if m.bias is None else m.bias.data_ptr(), ws.data_ptr(),
+                                   nbytes), "int8_project")
     return out
 
 

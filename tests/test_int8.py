@@ -95,7 +95,7 @@ def test_tile_layout_round_trip():
         assert w.w2[e, f // 128, k // 128, r, 16 * (c ^ (r & 7)) + k % 16] == raw["w2"][e, f, k]
         assert w.s2[e, f // 128, r] == raw["s2"][e, f]
     lin = layout.int8_linear(parts[4][0], parts[5][0])
-    assert torch.equal(lin.w[0], w.w2[0]) and torch.equal(lin.scale[0], w.s2[0])
+    assert torch.equal(lin.weight[0], w.w2[0]) and torch.equal(lin.scale[0], w.s2[0])
     q, s = layout.quantize_int8(torch.tensor([[0.0, 0.0], [1.0, -127.0], [2.54, 1.0]]))
     assert q.tolist() == [[0, 0], [1, -127], [127, 50]] and s[0] == 1 and s[1] == 1
 
@@ -123,10 +123,9 @@ def run_gemm(cuda, g, counts, planes, F, K, tile, *, clamp=False, bias=False, fu
     epi = _lib.EPI_DOWN_ONCE if planes == 1 else (_lib.EPI_CLAMP_SWIGLU_F32 if clamp else _lib.EPI_SWIGLU_F32)
     src = torch.randperm(rows, generator=g).int()
     rw = None if row_w is None else torch.rand(rows, generator=g).to(row_w)
-    ops.int8_gemm(offsets=off, expert_begin=begin, n_experts=E, max_rows=rows, planes=planes, feat_pad=fp, n_feat=F,
-                  k_pad=kp, weight=tiles, weight_scale=layout._int8_channels(ws3, fp).to(cuda),
-                  rows=ops.QuantRows(q.to(cuda), s.to(cuda)), epilogue=epi,
-                  bias=None if b is None else layout._int8_channels(b, fp).to(cuda),
+    m = ops.Int8Matrix(E, planes, F, K, fp, kp, tiles, layout._int8_channels(ws3, fp).to(cuda),
+                       None if b is None else layout._int8_channels(b, fp).to(cuda), epi)
+    ops.int8_gemm(m, ops.QuantRows(q.to(cuda), s.to(cuda)), offsets=off, expert_begin=begin,
                   row_weight=None if rw is None else rw.to(cuda), row_src=None if rw is None else src.to(cuda),
                   out=out, token_tile=tile)
     assert _lib.device_status(0) == 0
