@@ -197,7 +197,8 @@ int b200moe_route_grouped(int device, void* stream, const void* logits, int logi
   p.K = K;
   p.S = E / n_group;
   p.G = n_group;
-  p.P = pow2_ceil(n_group);
+  for (p.lsh = 5; (32 >> p.lsh) < n_group; --p.lsh) {
+  }
   p.keep = topk_group;
   p.top = group_top;
   p.softmax = scoring == B200MOE_SCORE_SOFTMAX;

@@ -53,7 +53,7 @@ struct RouteParams {
   int bf16;
   long long ld;
   const float* bias;           // [E] or NULL
-  int T, K, S, G, P;           // S experts in each of G groups, P the power of two >= G
+  int T, K, S, G, lsh;         // S experts in each of G groups; a group has 2^lsh lanes
   int keep, top;               // groups kept, keys in a group's sum (1 or 2)
   int softmax, normalize;
   float scale;

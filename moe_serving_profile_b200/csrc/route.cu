@@ -11,11 +11,16 @@
 // NaN keys and sums rank above every number.
 //
 // The selection is the one of the formula in 64-bit arithmetic. It is made in
-// fp32 with a bound on every key's error, and a token whose order that bound
-// does not settle (two neighbours of the selection, the last selected and the
-// first left out, the last kept and the first dropped group) is selected again
-// in 64 bits; so is every token with NaN. Of random tokens that is less than
-// one in a hundred.
+// fp32 with a bound on every key's error. A token whose order that bound does
+// not settle (two neighbours of the selection, the last selected and the first
+// left out, the last kept and the first dropped group), or that has a NaN key,
+// is put aside and selected in 64 bits when its warp is through: about two of
+// a thousand tokens of random logits. bf16 logits tie often; without a bias and
+// without sums of two keys their order is that of the scores, so they are the
+// keys (LOGIT), in words that hold them and the expert exactly, and nothing is
+// put aside but scores that 64 bits round together (sigmoid of logits above
+// 16, exponentials below e^-600). 4001 tokens, 160 experts: 18 us with scores
+// as keys, one token in ten put aside.
 //
 // One warp per token. Each group has L = 32 / P lanes, P the power of two >= G;
 // lane `sub` of a group holds its experts 4 (sub + L j) .. + 3, j = 0, 1, ...,
@@ -50,65 +55,89 @@ __device__ __forceinline__ unsigned long long order64(double v) {
   return b < 0 ? ~static_cast<unsigned long long>(b) : (static_cast<unsigned long long>(b) | (1ull << 63));
 }
 
-// Score in 64 bits; mx and sum: the row's largest logit and softmax sum.
-__device__ __forceinline__ double score64(const RouteParams& p, float x, double mx, double sum) {
-  const double v = static_cast<double>(x);
-  return p.softmax ? exp(v - mx) / sum : 1.0 / (1.0 + exp(-v));
+// 1 / x for x >= 1: the hardware's estimate and Newton's iteration.
+__device__ __forceinline__ double rcp64(double x) {
+  double y;
+  asm("rcp.approx.ftz.f64 %0, %1;" : "=d"(y) : "d"(x));
+  if (y == 0.0) return y;   // x is infinite (or its reciprocal subnormal)
+#pragma unroll
+  for (int i = 0; i < 3; ++i) y = fma(fma(-x, y, 1.0), y, y);
+  return y;
 }
 
-// Lane k < K gets the k-th selected expert. Only the keys stay in registers:
-// the call is rare, and its registers bound the kernel's.
+// The selection of one token, in lane k < K the k-th expert, with the row's
+// largest logit and the reciprocal of its softmax sum (0 and 1 with sigmoid).
+struct Selected {
+  int e;
+  float mx, inv;
+};
+
+// In 64 bits throughout: the lane's experts side by side, since a 64-bit chain
+// is slow (10 us when its parts ran one after another, 4 us so).
 template <int NL>
-__device__ __noinline__ int select64(const RouteParams& p, int t) {
-  const int lane = threadIdx.x & 31;
-  const int L = 32 / p.P;
-  const int g = lane / L, sub = lane % L;
-  auto holds = [&](int i) { return g < p.G && slot_offset(sub, L, i) < p.S; };
-  auto expert = [&](int i) { return g * p.S + slot_offset(sub, L, i); };
-  double mx = -INFINITY, sum = 0;
-  if (p.softmax) {
-#pragma unroll 1
-    for (int i = 0; i < NL; ++i)
-      if (holds(i)) {
-        const double v = static_cast<double>(load_logit(p, t, expert(i)));
-        mx = v > mx ? v : mx;
-      }
+__device__ __noinline__ Selected select64(const RouteParams& p, int t) {
+  const int lane = threadIdx.x & 31, L = 1 << p.lsh, g = lane >> p.lsh, sub = lane & (L - 1);
+  Selected out{0, 0.f, 1.f};
+  float x[NL], bias[NL];
+  uint32_t live = 0;
 #pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) {
-      const double m2 = __shfl_xor_sync(kFull, mx, o);
-      mx = m2 > mx ? m2 : mx;
-    }
-#pragma unroll 1
-    for (int i = 0; i < NL; ++i)
-      if (holds(i)) sum += exp(static_cast<double>(load_logit(p, t, expert(i))) - mx);
+  for (int i = 0; i < NL; ++i) {
+    const int o = slot_offset(sub, L, i);
+    const bool in = g < p.G && o < p.S;
+    live |= in ? 1u << i : 0u;
+    x[i] = in ? load_logit(p, t, g * p.S + o) : -INFINITY;
+    bias[i] = in && p.bias ? __ldg(p.bias + g * p.S + o) : 0.f;
+  }
+  double v[NL];
+  double mx = 0, sum = 0;
+  if (p.softmax) {
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < NL; ++i) top = fmaxf(top, x[i]);   // not NaN: that comes out of the sum
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, o));
+    out.mx = top;
+    mx = static_cast<double>(top);
+  }
+#pragma unroll 2
+  for (int i = 0; i < NL; ++i) {
+    const double a = static_cast<double>(x[i]) - mx;
+    double e = exp(p.softmax ? a : -a);
+    if (!p.softmax) e = rcp64(1.0 + e);
+    v[i] = e;
+    sum += ((live >> i) & 1u) ? e : 0.0;
+  }
+  if (p.softmax) {
 #pragma unroll
     for (int o = 16; o >= 1; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
+    const double inv = rcp64(sum);
+#pragma unroll
+    for (int i = 0; i < NL; ++i) v[i] *= inv;
+    out.inv = static_cast<float>(inv);
   }
-  unsigned long long key[NL];          // 0: no expert, or none that may still be selected
-  unsigned long long b1 = 0, b2 = 0;   // the lane's best keys
-  double v1 = 0, v2 = 0;
-  auto put = [&](unsigned long long k, double v) {
+  unsigned long long key[NL];   // 0: no expert, or none that may still be selected
+  unsigned long long b1 = 0, b2 = 0;
+  double v1 = 0, v2 = 0;        // the best two
+  auto put = [&](unsigned long long k, double f) {
     if (k > b1) {
       b2 = b1;
       v2 = v1;
       b1 = k;
-      v1 = v;
+      v1 = f;
     } else if (k > b2) {
       b2 = k;
-      v2 = v;
+      v2 = f;
     }
   };
 #pragma unroll
   for (int i = 0; i < NL; ++i) {
-    key[i] = 0;
-    if (holds(i)) {
-      double v = score64(p, load_logit(p, t, expert(i)), mx, sum);
-      if (p.bias) v += static_cast<double>(p.bias[expert(i)]);
-      key[i] = order64(v);
-      put(key[i], v);
-    }
+    const bool in = (live >> i) & 1u;
+    v[i] += static_cast<double>(bias[i]);
+    key[i] = in ? order64(v[i]) : 0ull;
+    put(key[i], v[i]);
   }
   if (p.keep < p.G) {
+#pragma unroll 1
     for (int o = 1; o < L; o <<= 1) {
       const unsigned long long c1 = __shfl_xor_sync(kFull, b1, o), c2 = __shfl_xor_sync(kFull, b2, o);
       const double w1 = __shfl_xor_sync(kFull, v1, o), w2 = __shfl_xor_sync(kFull, v2, o);
@@ -117,8 +146,9 @@ __device__ __noinline__ int select64(const RouteParams& p, int t) {
     }
     const unsigned long long mine = order64(v1 + ((p.top == 2 && p.S > 1) ? v2 : 0.0));
     int rank = 0;
+#pragma unroll 4
     for (int h = 0; h < p.G; ++h) {
-      const unsigned long long other = __shfl_sync(kFull, mine, h * L);
+      const unsigned long long other = __shfl_sync(kFull, mine, h << p.lsh);
       if (other > mine || (other == mine && h < g)) ++rank;
     }
     if (rank >= p.keep) {
@@ -126,40 +156,47 @@ __device__ __noinline__ int select64(const RouteParams& p, int t) {
       for (int i = 0; i < NL; ++i) key[i] = 0;
     }
   }
-  int sel = 0;
+  // the lane's keys in descending order, equal ones by slot (a stable sort)
+  int id[NL];
+#pragma unroll
+  for (int i = 0; i < NL; ++i) id[i] = g * p.S + slot_offset(sub, L, i);
+#pragma unroll
+  for (int j = 0; j < NL; ++j)
+#pragma unroll
+    for (int i = j & 1; i + 1 < NL; i += 2) {
+      const bool swap = key[i + 1] > key[i];
+      const unsigned long long ka = key[i], kb = key[i + 1];
+      const int ia = id[i], ib = id[i + 1];
+      key[i] = swap ? kb : ka;
+      key[i + 1] = swap ? ka : kb;
+      id[i] = swap ? ib : ia;
+      id[i + 1] = swap ? ia : ib;
+    }
 #pragma unroll 1
   for (int k = 0; k < p.K; ++k) {
-    unsigned long long bk = 0;
-    int bi = 0x7fffffff;
+    const uint32_t hi = static_cast<uint32_t>(key[0] >> 32), lo = static_cast<uint32_t>(key[0]);
+    const bool top = hi == __reduce_max_sync(kFull, hi);
+    const uint32_t most = __reduce_max_sync(kFull, top ? lo : 0u);
+    const bool mine = top && lo == most;
+    const int best = __reduce_min_sync(kFull, mine ? id[0] : 0x7fffffff);
+    if (lane == k) out.e = best;
+    if (mine && id[0] == best) {
 #pragma unroll
-    for (int i = 0; i < NL; ++i)
-      if (key[i] > bk) {
-        bk = key[i];
-        bi = expert(i);
+      for (int i = 0; i + 1 < NL; ++i) {
+        key[i] = key[i + 1];
+        id[i] = id[i + 1];
       }
-#pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) {
-      const unsigned long long k2 = __shfl_xor_sync(kFull, bk, o);
-      const int i2 = __shfl_xor_sync(kFull, bi, o);
-      if (k2 > bk || (k2 == bk && i2 < bi)) {
-        bk = k2;
-        bi = i2;
-      }
+      key[NL - 1] = 0;
     }
-#pragma unroll
-    for (int i = 0; i < NL; ++i)
-      if (bi == expert(i) && holds(i)) key[i] = 0;
-    if (lane == k) sel = bi;
   }
-  return sel;
+  return out;
 }
 
 // ------------------------------------------------------------ fp32 selection
-// Monotone map float -> uint32 and back; NaN above every number.
+// Monotone map float -> uint32 (not for NaN) and back.
 __device__ __forceinline__ uint32_t order32(float f) {
   const uint32_t b = __float_as_uint(f);
-  const uint32_t u = b ^ (static_cast<uint32_t>(static_cast<int32_t>(b) >> 31) | 0x80000000u);
-  return f != f ? 0xffffffffu : u;
+  return b ^ (static_cast<uint32_t>(static_cast<int32_t>(b) >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float unorder32(uint32_t u) {
   return __uint_as_float((u & 0x80000000u) ? (u ^ 0x80000000u) : ~u);
@@ -194,9 +231,9 @@ __device__ __forceinline__ void sort_desc(uint32_t (&k)[N]) {
           }
 }
 
-// A selected expert's full-precision values in lane k, and the bound on its
-// key's distance from the formula's: s (the exp's argument is rounded once,
-// 2^-24 of it; exp, sum and quotient a few units) and the sum with the bias.
+// An expert's full-precision values, and a bound on its key's distance from
+// the formula's: expf (2 units of 2^-23; softmax: its rounded argument as
+// well), sum and quotient, and the sum with the bias.
 struct Pick {
   float x, b, s, key, err;
 };
@@ -206,20 +243,21 @@ __device__ __forceinline__ Pick eval(const RouteParams& p, int t, int e, float m
   r.x = load_logit(p, t, e);
   r.b = p.bias ? p.bias[e] : 0.f;
   const float a = p.softmax ? r.x - mx : r.x;
-  r.s = p.softmax ? expf(a) * inv : 1.f / (1.f + expf(-a));
+  r.s = p.softmax ? expf(a) * inv : rcp(1.f + expf(-a));
   r.key = r.s + r.b;
-  r.err = (r.s * (16.f + fmaxf(-a, 0.f)) + fabsf(r.key)) * kUlp + 1e-37f;
+  // below -104 the exp is zero, and so is the first term (-inf as well)
+  r.err = (r.s * (8.f + (p.softmax ? fminf(-a, 128.f) : 0.f)) + fabsf(r.key)) * kUlp + 1e-37f;
   return r;
 }
 
-template <int NL, bool VEC>
+template <int NL, bool VEC, bool LOGIT>
 __global__ void __launch_bounds__(kThreads, NL <= 8 ? 2 : 1)
     route_grouped_kernel(const __grid_constant__ RouteParams p) {
   constexpr uint32_t kSlots = NL - 1;   // low bits of a word: NL - 1 - slot
   __shared__ int hist[512];
   const int lane = threadIdx.x & 31;
-  const int L = 32 / p.P;
-  const int g = lane / L, sub = lane & (L - 1);
+  const int lsh = p.lsh, L = 1 << lsh;
+  const int g = lane >> lsh, sub = lane & (L - 1);
   const int E = p.S * p.G;
   if (p.counts) {
     for (int e = threadIdx.x; e < E; e += kThreads) hist[e] = 0;
@@ -232,18 +270,16 @@ __global__ void __launch_bounds__(kThreads, NL <= 8 ? 2 : 1)
     const int o = slot_offset(sub, L, i);
     const bool in = g < p.G && o < p.S;
     live |= in ? 1u << i : 0u;
-    bias[i] = in && p.bias ? p.bias[g * p.S + o] : 0.f;
+    bias[i] = !LOGIT && in && p.bias ? p.bias[g * p.S + o] : 0.f;
   }
-  const int warps = gridDim.x * (kThreads / 32);
-  for (int t = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); t < p.T; t += warps) {
-    // ---- keys
-    float x[NL];
-    if (VEC) {   // S % 4 == 0: the four slots of a vector are live together
+  auto fetch = [&](int t, float (&x)[NL]) {
+    const long long row = (long long)t * p.ld + g * p.S + 4 * sub;
 #pragma unroll
-      for (int i = 0; i < NL; i += 4) {
-        x[i] = x[i + 1] = x[i + 2] = x[i + 3] = -INFINITY;
+    for (int i = 0; i < NL; i += 4) {
+      x[i] = x[i + 1] = x[i + 2] = x[i + 3] = -INFINITY;
+      const long long at = row + L * i;
+      if (VEC) {   // S % 4 == 0: the four slots of a vector are live together
         if ((live >> i) & 1u) {
-          const long long at = (long long)t * p.ld + g * p.S + slot_offset(sub, L, i);
           if (p.bf16) {
             const uint2 v = __ldg(reinterpret_cast<const uint2*>(reinterpret_cast<const __nv_bfloat16*>(p.logits) + at));
             x[i] = __uint_as_float(v.x << 16);
@@ -258,151 +294,176 @@ __global__ void __launch_bounds__(kThreads, NL <= 8 ? 2 : 1)
             x[i + 3] = v.w;
           }
         }
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < NL; ++i)
-        x[i] = ((live >> i) & 1u) ? load_logit(p, t, g * p.S + slot_offset(sub, L, i)) : -INFINITY;
-    }
-    constexpr float kLog2e = 1.44269504f;
-    float mx = 0.f, inv = 1.f;
-    if (p.softmax) {
-      mx = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < NL; ++i) mx = fmaxf(mx, x[i]);
-      mx = unorder32(__reduce_max_sync(kFull, order32(mx)));
-      float sum = 0.f;
-#pragma unroll
-      for (int i = 0; i < NL; ++i) {
-        x[i] = ex2((x[i] - mx) * kLog2e);
-        sum += ((live >> i) & 1u) ? x[i] : 0.f;
-      }
-#pragma unroll
-      for (int o = 16; o >= 1; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
-      inv = 1.f / sum;
-#pragma unroll
-      for (int i = 0; i < NL; ++i) x[i] *= inv;
-    } else {
-#pragma unroll
-      for (int i = 0; i < NL; ++i) x[i] = rcp(1.f + ex2(-kLog2e * x[i]));
-    }
-    uint32_t key[NL];
-#pragma unroll
-    for (int i = 0; i < NL; ++i)
-      key[i] = ((live >> i) & 1u) ? (order32(x[i] + bias[i]) & ~kSlots) | (kSlots - i) : 0u;
-    sort_desc(key);
-    bool sure = true;
-
-    // ---- groups: a key is off by at most 2^-19 of the row's largest score
-    // (its approximations) and 2^-23 NL of itself (its low bits)
-    if (p.keep < p.G) {
-      uint32_t k1 = key[0], k2 = key[1];
-      for (int o = 1; o < L; o <<= 1) {
-        const uint32_t c1 = __shfl_xor_sync(kFull, k1, o), c2 = __shfl_xor_sync(kFull, k2, o);
-        k2 = max(min(k1, c1), max(k2, c2));
-        k1 = max(k1, c1);
-      }
-      const float f1 = unorder32(k1 & ~kSlots);
-      const float f2 = p.top == 2 && p.S > 1 ? unorder32(k2 & ~kSlots) : 0.f;
-      const float total = f1 + f2;
-      const float off = (fabsf(f1) + fabsf(f2)) * ((NL + 2) * kUlp) + inv * (32.f * kUlp);
-      int rank = 0;
-      for (int h = 0; h < p.G; ++h) {
-        const float other = __shfl_sync(kFull, total, h * L);
-        rank += other > total || (other == total && h < g) ? 1 : 0;
-      }
-      const bool kept = rank < p.keep, real = g < p.G;
-      const uint32_t low = __reduce_min_sync(kFull, real && kept ? order32(total - off) : 0xffffffffu);
-      const uint32_t high = __reduce_max_sync(kFull, real && !kept ? order32(total + off) : 0u);
-      // NaN and infinite sums are compared in 64 bits
-      sure = low > high && !__any_sync(kFull, real && !(fabsf(total) + off < INFINITY));
-      if (!kept) key[0] = 0;
-    }
-
-    // ---- K rounds of the best word, and the first one left out
-    int sel = 0, border = -1;
-#pragma unroll 1
-    for (int k = 0; k <= p.K; ++k) {
-      const uint32_t m = __reduce_max_sync(kFull, key[0]);
-      if (m == 0) break;   // every expert of the kept groups is selected
-      const int src = __ffs(__ballot_sync(kFull, key[0] == m)) - 1;
-      const int slot = kSlots - (m & kSlots);
-      const int e = (src / L) * p.S + slot_offset(src & (L - 1), L, slot);
-      if (k == p.K) {
-        border = e;
-        break;
-      }
-      if (lane == k) sel = e;   // equal words of several lanes have one slot: the first lane's expert is the lowest
-      if (lane == src) {
-#pragma unroll
-        for (int i = 0; i + 1 < NL; ++i) key[i] = key[i + 1];
-        key[NL - 1] = 0;
-      }
-    }
-
-    // ---- full-precision keys of the selected, and whether their order is sure
-    Pick c = eval(p, t, lane < p.K ? sel : (border >= 0 ? border : sel), mx, inv);
-    auto ordered = [&]() {
-      const float nk = __shfl_down_sync(kFull, c.key, 1), ne = __shfl_down_sync(kFull, c.err, 1);
-      const float nx = __shfl_down_sync(kFull, c.x, 1), nb = __shfl_down_sync(kFull, c.b, 1);
-      const int ni = __shfl_down_sync(kFull, sel, 1);
-      bool ok = c.key - nk > c.err + ne || (c.x == nx && c.b == nb && sel < ni);
-      return __all_sync(kFull, ok || lane >= p.K - 1);
-    };
-    if (!ordered()) {
-      // the low bits that the words lack: rank the selected by their keys
-      int rank = 0;
-      for (int j = 0; j < p.K; ++j) {
-        const float kj = __shfl_sync(kFull, c.key, j);
-        const int ij = __shfl_sync(kFull, sel, j);
-        rank += kj > c.key || (kj == c.key && ij < sel) ? 1 : 0;
-      }
-      int from = lane;
-      for (int j = 0; j < p.K; ++j) {
-        const int rj = __shfl_sync(kFull, rank, j);
-        if (rj == lane && lane < p.K) from = j;
-      }
-      sel = __shfl_sync(kFull, sel, from);
-      c.x = __shfl_sync(kFull, c.x, from);
-      c.b = __shfl_sync(kFull, c.b, from);
-      c.s = __shfl_sync(kFull, c.s, from);
-      c.key = __shfl_sync(kFull, c.key, from);
-      c.err = __shfl_sync(kFull, c.err, from);
-      sure = ordered() && sure;
-    }
-    if (border >= 0) {
-      // the first one left out stands for all of them: their words are not
-      // above its word, their keys at most its low bits above its key
-      Pick n;
-      if (p.K < 32) {
-        n.key = __shfl_sync(kFull, c.key, p.K);
-        n.err = __shfl_sync(kFull, c.err, p.K);
       } else {
-        n = eval(p, t, border, mx, inv);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if ((live >> (i + j)) & 1u)
+            x[i + j] = p.bf16 ? __bfloat162float(__ldg(reinterpret_cast<const __nv_bfloat16*>(p.logits) + at + j))
+                              : __ldg(reinterpret_cast<const float*>(p.logits) + at + j);
       }
-      const float last = __shfl_sync(kFull, c.key, p.K - 1), le = __shfl_sync(kFull, c.err, p.K - 1);
-      sure = sure && last - n.key > le + n.err + fabsf(n.key) * (2 * NL * kUlp) + inv * (32.f * kUlp);
-    } else {
-      sure = sure && __all_sync(kFull, c.key == c.key);
     }
-    if (!sure) {
-      sel = select64<NL>(p, t);
-      c = eval(p, t, sel, mx, inv);
-    }
-    float w = c.s;
+  };
 
+  auto write = [&](int t, int sel, float w) {   // lane k < K: the k-th expert and its score
     const bool mine = lane < p.K;
     if (p.normalize) {
       float sum = mine ? w : 0.f;
 #pragma unroll
       for (int o = 16; o >= 1; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
-      w /= sum + 1e-20f;
+      w *= rcp(sum + 1e-20f);
     }
     if (mine) {
-      p.scores[(long long)t * p.K + lane] = w * p.scale;
-      p.indices[(long long)t * p.K + lane] = sel;
+      const long long at = (long long)t * p.K + lane;
+      p.scores[at] = w * p.scale;
+      p.indices[at] = sel;
       if (p.counts) atomicAdd(&hist[sel], 1);
     }
+  };
+
+  const int warps = gridDim.x * (kThreads / 32);
+  int first = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
+  float next[NL];
+  if (first < p.T) fetch(first, next);
+  while (first < p.T) {   // 32 tokens of the warp at a time
+    uint32_t aside = 0;   // those to select in 64 bits
+    int t = first;
+#pragma unroll 1
+    for (int turn = 0; turn < 32 && t < p.T; ++turn, t += warps) {
+      float x[NL];
+#pragma unroll
+      for (int i = 0; i < NL; ++i) x[i] = next[i];
+      if (t + warps < p.T) fetch(t + warps, next);   // in flight while this token is selected
+
+      // ---- keys
+      constexpr float kLog2e = 1.44269504f;
+      float mx = 0.f, inv = 1.f, total = 0.f;
+      uint32_t key[NL];
+      if (LOGIT) {
+#pragma unroll
+        for (int i = 0; i < NL; ++i) {
+          const uint32_t tag = 0xffffu - (g * p.S + slot_offset(sub, L, i));   // equal logits: the lower id first
+          total += x[i];
+          key[i] = ((live >> (VEC ? i & ~3 : i)) & 1u) ? (order32(x[i] + 0.f) & 0xffff0000u) | tag : 0u;   // -0 is 0
+        }
+      }
+      if (p.softmax) {
+        mx = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < NL; ++i) mx = fmaxf(mx, x[i]);
+        mx = unorder32(__reduce_max_sync(kFull, order32(mx)));
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < NL; ++i) {
+          x[i] = ex2((x[i] - mx) * kLog2e);   // 0 in a slot without an expert
+          sum += x[i];
+        }
+#pragma unroll
+        for (int o = 16; o >= 1; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
+        inv = 1.f / sum;
+#pragma unroll
+        for (int i = 0; i < NL; ++i) x[i] *= inv;
+      } else {
+#pragma unroll
+        for (int i = 0; i < NL; ++i) x[i] = rcp(1.f + ex2(-kLog2e * x[i]));
+      }
+      if (!LOGIT) {
+#pragma unroll
+        for (int i = 0; i < NL; ++i) {
+          const float k = x[i] + bias[i];
+          total += k;
+          key[i] = ((live >> (VEC ? i & ~3 : i)) & 1u) ? (order32(k) & ~kSlots) | (kSlots - i) : 0u;
+        }
+      }
+      bool sure = !__any_sync(kFull, total != total);   // no NaN key (nor infinite ones of both signs)
+      sort_desc(key);
+      // whether 64 bits tell the score of logit a (less the largest, softmax) from those of smaller ones
+      auto apart = [&](float a) { return a > -600.f && (p.softmax || a <= 16.f); };
+
+      // ---- groups. A key is off by at most 2^-20 of the row's largest score
+      // (its approximations) and at most NL units above its word; a sum's word
+      // has the group in its low bits
+      if (p.keep < p.G) {
+        uint32_t k1 = key[0], k2 = key[1];
+        for (int o = 1; o < L; o <<= 1) {
+          const uint32_t c1 = __shfl_xor_sync(kFull, k1, o), c2 = __shfl_xor_sync(kFull, k2, o);
+          k2 = max(min(k1, c1), max(k2, c2));
+          k1 = max(k1, c1);
+        }
+        const uint32_t gmask = (32u >> lsh) - 1;
+        const bool real = g < p.G;
+        float off = 0.f;
+        uint32_t word = 0;
+        if (LOGIT) {
+          word = real ? (k1 & 0xffff0000u) | (gmask - g) : 0u;
+        } else if (real) {
+          const float f1 = unorder32(k1 & ~kSlots);
+          const float f2 = p.top == 2 && p.S > 1 ? unorder32(k2 & ~kSlots) : 0.f;
+          off = (fabsf(f1) + fabsf(f2)) * (NL * kUlp) + inv * (32.f * kUlp);
+          word = (order32(f1 + f2) & ~gmask) | (gmask - g);
+        }
+        uint32_t low = 0xffffffffu, high = 0;   // the last kept and the first dropped sum
+        for (int h = 0; h <= p.keep; ++h) {
+          low = high ? high : low;
+          high = __reduce_max_sync(kFull, h == 0 || word < low ? word : 0u);
+        }
+        if (LOGIT) {
+          sure = sure && apart(unorder32(low & 0xffff0000u) - mx);
+        } else {
+          const float most = __uint_as_float(__reduce_max_sync(kFull, __float_as_uint(off)));
+          // (infinite sums are not told apart here)
+          sure = sure && unorder32(low & ~gmask) - unorder32(high | gmask) > most;
+        }
+        if (word < low) key[0] = 0;
+      }
+
+      // ---- K rounds of the best word; lane k keeps the k-th and where it was
+      uint32_t m = 0, wm = 0;
+      int src = 0, ws = 0;
+      auto best = [&]() {
+        m = __reduce_max_sync(kFull, key[0]);   // 0: no expert is left
+        // equal words of several lanes have one slot: the first lane's expert is the lowest
+        src = __ffs(__ballot_sync(kFull, key[0] == m)) - 1;
+      };
+#pragma unroll 1
+      for (int k = 0; k < p.K; ++k) {
+        best();
+        if (lane == k) {
+          wm = m;
+          ws = src;
+        }
+        if (lane == src) {
+#pragma unroll
+          for (int i = 0; i + 1 < NL; ++i) key[i] = key[i + 1];
+          key[NL - 1] = 0;
+        }
+      }
+      // ---- full-precision keys of the selected, and whether the selection is sure
+      const int sel = lane >= p.K ? 0
+                      : LOGIT     ? static_cast<int>(0xffffu - (wm & 0xffffu))
+                                  : (ws >> lsh) * p.S + slot_offset(ws & (L - 1), L, static_cast<int>(kSlots - (wm & kSlots)));
+      const Pick c = eval(p, t, sel, mx, inv);
+      if (LOGIT) {
+        sure = sure && (lane >= p.K || apart(c.x - mx));
+      } else {
+        const float nk = __shfl_down_sync(kFull, c.key, 1), ne = __shfl_down_sync(kFull, c.err, 1);
+        const float nx = __shfl_down_sync(kFull, c.x, 1), nb = __shfl_down_sync(kFull, c.b, 1);
+        const int ni = __shfl_down_sync(kFull, sel, 1);
+        const bool ordered = c.key - nk > c.err + ne || (c.x == nx && c.b == nb && sel < ni) || lane >= p.K - 1;
+        // the first one left out: no key left is above its word's range
+        m = __reduce_max_sync(kFull, key[0]);
+        const uint32_t high = m ? order32(unorder32(m | kSlots) + inv * (8.f * kUlp)) : 0u;
+        sure = sure && ordered && (lane >= p.K || order32(c.key - c.err) > high);
+      }
+      if (__all_sync(kFull, sure)) write(t, sel, c.s);
+      else aside |= 1u << turn;
+    }
+    while (aside) {
+      const int at = first + (__ffs(aside) - 1) * warps;
+      aside &= aside - 1;
+      const Selected r = select64<NL>(p, at);
+      write(at, r.e, eval(p, at, r.e, r.mx, r.inv).s);
+    }
+    first = t;
   }
   if (p.counts) {
     __syncthreads();
@@ -422,14 +483,17 @@ int route_grouped_blocks(int T, int sm_count) {
 }
 
 cudaError_t launch_route_grouped(cudaStream_t st, const RouteParams& p, int blocks) {
-  const int L = 32 / p.P;
+  const int L = 1 << p.lsh;
   const int per_lane = 4 * ((p.S + 4 * L - 1) / (4 * L));   // slots of a lane, in fours
   const uintptr_t item = p.bf16 ? 2 : 4;
   const bool vec = p.S % 4 == 0 && p.ld % 4 == 0 && reinterpret_cast<uintptr_t>(p.logits) % (4 * item) == 0;
-#define B200_ROUTE(NL_)                                                    \
-  do {                                                                     \
-    if (vec) route_grouped_kernel<NL_, true><<<blocks, kThreads, 0, st>>>(p); \
-    else route_grouped_kernel<NL_, false><<<blocks, kThreads, 0, st>>>(p);    \
+  const bool logit = p.bf16 && p.bias == nullptr && (p.keep == p.G || p.top == 1 || p.S == 1);
+#define B200_ROUTE(NL_)                                                                 \
+  do {                                                                                  \
+    if (vec && logit) route_grouped_kernel<NL_, true, true><<<blocks, kThreads, 0, st>>>(p);   \
+    else if (vec) route_grouped_kernel<NL_, true, false><<<blocks, kThreads, 0, st>>>(p);      \
+    else if (logit) route_grouped_kernel<NL_, false, true><<<blocks, kThreads, 0, st>>>(p);    \
+    else route_grouped_kernel<NL_, false, false><<<blocks, kThreads, 0, st>>>(p);              \
   } while (0)
   if (per_lane <= 4) B200_ROUTE(4);
   else if (per_lane <= 8) B200_ROUTE(8);
