@@ -1,8 +1,10 @@
-"""Build the sm_100a shared library ``libb200moe.so`` next to this file.
+"""Build the sm_100a shared library ``libb200moe.so`` and the torch binding
+``_ext.so`` next to this file.
 
 nvcc compiles every kernel for ``sm_100a`` only (no PTX fallback, no other
 architecture). The library links the CUDA runtime statically and exports the
-C ABI declared in ``include/b200moe.h``. Run ``python -m
+C ABI declared in ``include/b200moe.h``; the binding calls it (g++, no CUDA
+code of its own). Run ``python -m
 moe_serving_profile_b200.build`` or call :func:`build`.
 """
 
@@ -18,6 +20,7 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 INCLUDE = ROOT / "include"
 LIB = PKG / "libb200moe.so"
+EXT = PKG / "_ext.so"
 SOURCES = ["api.cu", "router.cu", "permute.cu", "gemm.cu", "decode.cu", "combine.cu", "a2a.cu", "a2a_p2p.cu", "p2p.cu", "w8a8.cu",
            "route.cu", "norm.cu", "int8.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -37,9 +40,32 @@ def _stale() -> bool:
     return any(p.stat().st_mtime > built for p in deps)
 
 
+def build_ext(force: bool = False) -> Path:
+    """Compile the torch binding if its source or the header is newer."""
+    deps = [CSRC / "ext.cpp", INCLUDE / "b200moe.h"]
+    if not force and EXT.exists() and all(p.stat().st_mtime <= EXT.stat().st_mtime for p in deps):
+        return EXT
+    import sysconfig
+
+    import torch
+
+    root = Path(torch.__file__).resolve().parent
+    tmp = EXT.with_suffix(".so.tmp")
+    subprocess.run([
+        "g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+        "-I", str(root / "include"), "-I", str(root / "include" / "torch" / "csrc" / "api" / "include"),
+        "-I", sysconfig.get_paths()["include"], "-I", str(Path(nvcc()).parents[1] / "include"), "-I", str(INCLUDE),
+        str(CSRC / "ext.cpp"), "-o", str(tmp), "-L", str(root / "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu",
+        "-ltorch_python", "-L", str(PKG), f"-l:{LIB.name}", "-Wl,-rpath,$ORIGIN"], check=True)
+    os.replace(tmp, EXT)
+    return EXT
+
+
 def build(force: bool = False, verbose: bool = False) -> Path:
-    """Compile the library if any source is newer than it; return its path."""
+    """Compile the library if any source is newer than it, then the binding;
+    return the library's path."""
     if not force and not _stale():
+        build_ext()
         return LIB
     objs = []
     build_dir = PKG / "_build"
@@ -58,6 +84,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     subprocess.run([nvcc(), *ARCH, "-shared", "-o", str(tmp), *objs, "-lcudart_static", "-lrt",
                     "-lpthread", "-ldl"], check=True)
     os.replace(tmp, LIB)
+    build_ext(force)
     return LIB
 
 

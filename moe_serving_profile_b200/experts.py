@@ -148,16 +148,15 @@ def int8_gate_up(w: ExpertWeights, hidden: torch.Tensor | ops.QuantRows, perm: o
         raise ValueError("int8_gate_up needs int8 expert weights")
     copies = K if copies is None else copies
     R = perm.perm_src.numel()
-    act = torch.empty(R, w.i_pad, device=w.w1.device, dtype=torch.bfloat16) if out is None else out
     tile = _int8_tile(R, num_experts)
     if isinstance(hidden, ops.QuantRows):
         rows = ops.scatter_rows_8bit(hidden.checked(torch.int8, w.h_k, w.w1.device), perm.inverse, copies,
                                      **_local_range(w, perm, num_experts, expert_begin))
-        return ops.int8_gemm(w.m1, rows, offsets=perm.offsets, expert_begin=expert_begin, out=act, token_tile=tile)
+        return ops.int8_gemm(w.m1, rows, offsets=perm.offsets, expert_begin=expert_begin, out=out, token_tile=tile)
     if hidden.shape[1] != w.hidden:
         raise ValueError(f"hidden size {hidden.shape[1]} does not match the experts' {w.hidden}")
     return ops.int8_project(w.m1, hidden, offsets=perm.offsets, expert_begin=expert_begin, inverse=perm.inverse,
-                            copies=copies, out=act, token_tile=tile)
+                            copies=copies, out=out, token_tile=tile)
 
 
 def int8_down(w: ExpertWeights, act: torch.Tensor, perm: ops.Permutation, weights: torch.Tensor | None, *, K: int,
@@ -170,8 +169,6 @@ def int8_down(w: ExpertWeights, act: torch.Tensor, perm: ops.Permutation, weight
     R = perm.perm_src.numel()
     if act.shape[0] != R:
         raise ValueError(f"act must have a row for each of the {R} assignments, got {act.shape[0]}")
-    if contrib is None:
-        contrib = torch.empty(R, w.hidden, device=act.device, dtype=torch.bfloat16)
     return ops.int8_project(w.m2, act, offsets=perm.offsets, expert_begin=expert_begin, row_weight=weights,
                             row_src=None if weights is None else perm.perm_src, out=contrib,
                             token_tile=_int8_tile(R, num_experts))
@@ -194,23 +191,15 @@ def run_experts_int8_placed(w: ExpertWeights, x: torch.Tensor, offsets: torch.Te
     order, ``offsets`` (int32 [n_experts + 1]) their segments; rows past the
     last segment are neither read nor written. ``tokens``: the rows expected,
     for the token tile."""
-    R = x.shape[0]
-    kw = dict(offsets=offsets, expert_begin=0, token_tile=_int8_tile(tokens, w.n_experts))
-    act = torch.empty(R, w.i_pad, device=x.device, dtype=torch.bfloat16)
-    ops.int8_project(w.m1, x, out=act, **kw)
-    y = torch.empty(R, w.hidden, device=x.device, dtype=torch.bfloat16)
-    return ops.int8_project(w.m2, act, out=y, **kw)
+    kw = dict(offsets=offsets, token_tile=_int8_tile(tokens, w.n_experts))
+    return ops.int8_project(w.m2, ops.int8_project(w.m1, x, **kw), **kw)
 
 
 def int8_swiglu(w: ExpertWeights, x: torch.Tensor) -> torch.Tensor:
     """The one expert of ``w`` on every row of bf16 ``x`` [T, H]."""
     if w.fmt != _lib.W_INT8 or w.n_experts != 1:
         raise ValueError("int8_swiglu needs the int8 weights of one expert")
-    T = x.shape[0]
-    act = torch.empty(T, w.i_pad, device=x.device, dtype=torch.bfloat16)
-    ops.int8_project(w.m1, x, out=act)
-    y = torch.empty(T, w.hidden, device=x.device, dtype=torch.bfloat16)
-    return ops.int8_project(w.m2, act, out=y)
+    return ops.int8_project(w.m2, ops.int8_project(w.m1, x))
 
 
 def int8_linear(w: ops.Int8Matrix, x: torch.Tensor | ops.QuantRows, out: torch.Tensor | None = None) -> torch.Tensor:
@@ -219,13 +208,9 @@ def int8_linear(w: ops.Int8Matrix, x: torch.Tensor | ops.QuantRows, out: torch.T
     if w.n_experts != 1 or w.planes != 1:
         raise ValueError("int8_linear needs the weights of layout.int8_linear")
     if isinstance(x, ops.QuantRows):
-        if out is None:
-            out = torch.empty(x.q.shape[0], w.n_feat, device=w.weight.device, dtype=torch.bfloat16)
         return ops.int8_gemm(w, x, out=out)
     if x.shape[-1] != w.k_valid:
         raise ValueError(f"x has {x.shape[-1]} columns, the projection takes {w.k_valid}")
-    if out is None:
-        out = torch.empty(x.shape[0], w.n_feat, device=w.weight.device, dtype=torch.bfloat16)
     return ops.int8_project(w, x, out=out)
 
 

@@ -3,7 +3,9 @@
 Each function takes CUDA tensors, allocates its outputs with torch's caching
 allocator and enqueues the kernels on the current stream of the tensors'
 device. Nothing here synchronises the host. Tensors on any other device are
-rejected: the library has no CPU implementation.
+rejected: the library has no CPU implementation. The grouped routing, the norm
+and the int8 products go through the compiled binding (csrc/ext.cpp), which
+checks and allocates in C++.
 """
 
 from __future__ import annotations
@@ -14,7 +16,8 @@ from dataclasses import dataclass
 import torch
 
 from moe_serving_profile_b200 import _lib
-from moe_serving_profile_b200._lib import check, lib
+from moe_serving_profile_b200._lib import check, lib   # first: a missing library is its ImportError
+from moe_serving_profile_b200 import _ext
 
 
 def _dev(t: torch.Tensor, what: str) -> int:
@@ -93,12 +96,6 @@ def router(mode: int, hidden: torch.Tensor, weight: torch.Tensor, bias: torch.Te
     return RouterOut(logits_t, probs, scores, indices, counts)
 
 
-def _same_device(t: torch.Tensor | None, device: int, what: str) -> None:
-    if t is not None and (not t.is_cuda or t.device.index != device):
-        raise ValueError(f"{what} must be on cuda:{device}, got {t.device}")
-
-
-_BF16_FLAG = {torch.float32: 0, torch.bfloat16: 1}   # the C calls' fp32 / bf16 switch
 SCORING = {"sigmoid": _lib.SCORE_SIGMOID, "softmax": _lib.SCORE_SOFTMAX}
 
 
@@ -112,35 +109,11 @@ def route_grouped(logits: torch.Tensor, bias: torch.Tensor | None, top_k: int, *
     ``group_top`` keys kept, the ``top_k`` best keys selected (equal keys:
     the lower id), their scores renormalised and times ``scale``. scores are
     fp32 [T, K] in descending order of the keys."""
-    device = _dev(logits, "logits")
-    bf = _BF16_FLAG.get(logits.dtype)
-    sl = logits.stride()
-    if bf is None or len(sl) != 2 or sl[1] != 1:
-        raise ValueError("logits must be a 2D float32 or bfloat16 tensor with contiguous rows")
     mode = SCORING.get(scoring)
     if mode is None:
         raise ValueError(f"scoring must be one of {tuple(SCORING)}, got {scoring!r}")
-    T, E = logits.shape
-    pb = None
-    if bias is not None:
-        if (bias.dtype != torch.float32 or bias.shape != (E,) or not bias.is_contiguous()
-                or bias.get_device() != device):
-            raise ValueError(f"bias must be contiguous float32 [{E}] on {logits.device}")
-        pb = bias.data_ptr()
-    if not 1 <= top_k <= E:   # before the outputs of that width are allocated
-        raise ValueError(f"top_k must be in [1, {E}], got {top_k}")
-    dev = logits.device
-    scores = torch.empty(T, top_k, device=dev, dtype=torch.float32)
-    indices = torch.empty(T, top_k, device=dev, dtype=torch.int64)
-    counts = torch.empty(E, device=dev, dtype=torch.int32)
-    check(
-        lib.b200moe_route_grouped(
-            device, _stream(device), logits.data_ptr(), bf, sl[0] if T > 1 else E, pb, T, E, top_k, n_group,
-            topk_group, group_top, mode, int(normalize), scale, scores.data_ptr(), indices.data_ptr(),
-            counts.data_ptr(),
-        ),
-        "route_grouped",
-    )
+    scores, indices, counts = _ext.route_grouped(logits, bias, top_k, n_group, topk_group, group_top, mode,
+                                                 normalize, scale)
     return RouterOut(logits, None, scores, indices, counts)
 
 
@@ -203,72 +176,18 @@ def act_quant_fp8(x: torch.Tensor, k_pad: int | None = None, rows_src: torch.Ten
     return q, s
 
 
-@dataclass
-class QuantRows:
-    """Rows in 8 bits with their scales: e4m3 ``q`` [rows, k_pad] with fp32
-    ``scale`` [rows, ceil(k_pad / 128)] (W8A8 FP8 experts) or int8 ``q`` with
-    ``scale`` [rows] (int8 experts and products)."""
-
-    q: torch.Tensor
-    scale: torch.Tensor
-
-    def checked(self, dtype: torch.dtype, k_pad: int, device: torch.device) -> "QuantRows":
-        """Self, if these are ``dtype`` rows of width ``k_pad`` on ``device``."""
-        q, scale = self.q, self.scale
-        if q.dtype != dtype or q.dim() != 2 or q.shape[1] != k_pad or not q.is_contiguous():
-            raise ValueError(f"quantised rows must be contiguous {dtype} [rows, {k_pad}], got {q.dtype} "
-                             f"{tuple(q.shape)}")
-        shape = q.shape[:1] if dtype == torch.int8 else (q.shape[0], -(-k_pad // 128))
-        if scale.dtype != torch.float32 or scale.shape != shape or not scale.is_contiguous():
-            raise ValueError(f"row scales must be contiguous float32 {tuple(shape)}")
-        if q.device != device or scale.device != device:
-            raise ValueError(f"quantised rows must be on {device}")
-        return self
-
-
-def _quant_range(offsets, expert_lo: int, expert_hi: int, device: int) -> None:
-    if offsets is not None:
-        _same_device(offsets, device, "offsets")
-        if (offsets.dtype != torch.int32 or not offsets.is_contiguous()
-                or not 0 <= expert_lo <= expert_hi < offsets.numel()):
-            raise ValueError("offsets must be contiguous int32 with 0 <= expert_lo <= expert_hi < offsets.numel()")
-
-
-def _inverse_rows(inverse, rows: int, copies: int, device: int) -> None:
-    _same_device(inverse, device, "inverse")
-    if inverse.dtype != torch.int32 or not inverse.is_contiguous() or inverse.numel() != rows * copies:
-        raise ValueError(f"inverse must be contiguous int32 of rows * copies = {rows * copies} elements")
+QuantRows = _ext.QuantRows
 
 
 def act_quant_int8(x: torch.Tensor, k_pad: int | None = None, inverse: torch.Tensor | None = None,
                    copies: int = 1, offsets: torch.Tensor | None = None, expert_lo: int = 0,
                    expert_hi: int = 0) -> QuantRows:
-    """Int8 rows of bf16 ``x`` with one scale each (amax / 127). With
-    ``inverse`` (a permutation's, int32 [rows * copies]) row r is quantised
-    once and written to each of its ``copies`` places of the permuted order.
-    With ``offsets`` only the places [offsets[expert_lo], offsets[expert_hi])
-    are written."""
-    device = _dev(x, "x")
-    if x.dtype != torch.bfloat16 or x.dim() != 2 or x.stride(1) != 1:
-        raise ValueError("x must be a 2-D bfloat16 tensor with unit column stride")
-    rows, k_valid = x.shape
-    k_pad = -(-k_valid // 128) * 128 if k_pad is None else k_pad
-    rows_out = rows
-    if inverse is not None:
-        _inverse_rows(inverse, rows, copies, device)
-        rows_out = inverse.numel()
-    elif copies != 1:
-        raise ValueError("copies need inverse")
-    _quant_range(offsets, expert_lo, expert_hi, device)
-    q = torch.empty((rows_out, k_pad), device=x.device, dtype=torch.int8)
-    s = torch.empty((rows_out,), device=x.device, dtype=torch.float32)
-    check(
-        lib.b200moe_act_quant_int8(device, _stream(device), _ptr(x), x.stride(0) if rows > 1 else k_valid, rows,
-                                   k_valid, k_pad, _ptr(inverse), copies, rows_out, _ptr(offsets), int(expert_lo),
-                                   int(expert_hi), _ptr(q), _ptr(s)),
-        "act_quant_int8",
-    )
-    return QuantRows(q, s)
+    """Int8 rows of bf16 ``x`` with one scale each (amax / 127), padded to
+    ``k_pad`` columns (default: the next multiple of 128). With ``inverse`` (a
+    permutation's, int32 [rows * copies]) row r is quantised once and written
+    to each of its ``copies`` places of the permuted order. With ``offsets``
+    only the places [offsets[expert_lo], offsets[expert_hi]) are written."""
+    return _ext.act_quant_int8(x, k_pad, inverse, copies, offsets, expert_lo, expert_hi)
 
 
 def scatter_rows_8bit(rows: QuantRows, inverse: torch.Tensor, copies: int, offsets: torch.Tensor | None = None,
@@ -276,24 +195,7 @@ def scatter_rows_8bit(rows: QuantRows, inverse: torch.Tensor, copies: int, offse
     """Quantised token rows at their ``copies`` places each of the permuted
     order (``inverse``: a permutation's); with ``offsets`` only the places
     [offsets[expert_lo], offsets[expert_hi])."""
-    device = _dev(rows.q, "rows")
-    rows = rows.checked(rows.q.dtype, rows.q.shape[1], rows.q.device)
-    if rows.q.dtype not in (torch.int8, torch.float8_e4m3fn):
-        raise ValueError(f"rows must be int8 or float8_e4m3fn, got {rows.q.dtype}")
-    n, width = rows.q.shape
-    _inverse_rows(inverse, n, copies, device)
-    _quant_range(offsets, expert_lo, expert_hi, device)
-    R = inverse.numel()
-    groups = rows.scale.numel() // max(n, 1) or 1
-    q = torch.empty((R, width), device=rows.q.device, dtype=rows.q.dtype)
-    s = torch.empty((R,) + tuple(rows.scale.shape[1:]), device=rows.q.device, dtype=torch.float32)
-    check(
-        lib.b200moe_scatter_rows_8bit(device, _stream(device), _ptr(rows.q), width, _ptr(rows.scale), groups, n,
-                                      _ptr(inverse), copies, R, _ptr(offsets), int(expert_lo), int(expert_hi),
-                                      _ptr(q), _ptr(s)),
-        "scatter_rows_8bit",
-    )
-    return QuantRows(q, s)
+    return _ext.scatter_rows_8bit(rows, inverse, copies, offsets, expert_lo, expert_hi)
 
 
 # --------------------------------------------------------------------------- norm
@@ -307,15 +209,6 @@ class NormOut:
 QUANT = {None: _lib.QUANT_NONE, "fp8": _lib.QUANT_FP8, "int8": _lib.QUANT_INT8}
 
 
-def _residual_rows(t: torch.Tensor, x: torch.Tensor, device: int, what: str) -> int:
-    """The row stride of a residual, checked against ``x``."""
-    st = t.stride()
-    if t.dtype != torch.bfloat16 or t.shape != x.shape or st[1] != 1 or t.get_device() != device:
-        raise ValueError(f"{what} must be bfloat16 {tuple(x.shape)} with contiguous rows on {x.device}, got {t.dtype} "
-                         f"{tuple(t.shape)} on {t.device}")
-    return st[0] if t.shape[0] > 1 else t.shape[1]
-
-
 def add_rmsnorm(x: torch.Tensor, weight: torch.Tensor, eps: float, *, residual: torch.Tensor | None = None,
                 residual_out: torch.Tensor | None = None, quant: str | None = None, k_pad: int | None = None,
                 normed: bool = True) -> NormOut:
@@ -325,53 +218,10 @@ def add_rmsnorm(x: torch.Tensor, weight: torch.Tensor, eps: float, *, residual: 
     "fp8" or "int8" also returns the normed rows in the 8-bit form of the W8A8
     FP8 or the int8 experts, padded to ``k_pad`` columns (default: what those
     experts take); ``normed=False`` leaves the bf16 output out."""
-    device = _dev(x, "x")
-    sx = x.stride()
-    if x.dtype != torch.bfloat16 or len(sx) != 2 or sx[1] != 1:
-        raise ValueError("x must be a 2D bfloat16 tensor with contiguous rows")
     mode = QUANT.get(quant)
     if mode is None:
         raise ValueError(f"quant must be one of {tuple(QUANT)}, got {quant!r}")
-    T, H = x.shape
-    f32 = weight.dtype == torch.float32
-    if not (f32 or weight.dtype == torch.bfloat16) or weight.shape != (H,) or not weight.is_contiguous():
-        raise ValueError(f"weight must be contiguous bfloat16 or float32 [{H}]")
-    if weight.get_device() != device:
-        raise ValueError(f"weight must be on cuda:{device}, got {weight.device}")
-    if not mode and not normed:
-        raise ValueError("nothing to compute: no quantised rows and no bf16 output")
-    dev = x.device
-    ldr = ldro = 0
-    pr = pro = po = pq = ps = None
-    if residual is not None:
-        ldr, pr = _residual_rows(residual, x, device, "residual"), residual.data_ptr()
-        if residual_out is None:
-            residual_out, ldro = torch.empty(T, H, device=dev, dtype=torch.bfloat16), H
-        else:
-            ldro = _residual_rows(residual_out, x, device, "residual_out")
-        pro = residual_out.data_ptr()
-    elif residual_out is not None:
-        raise ValueError("residual_out needs a residual")
-    out = rows = None
-    if normed:
-        out = torch.empty(T, H, device=dev, dtype=torch.bfloat16)
-        po = out.data_ptr()
-    if mode:
-        if k_pad is None:   # what the experts of that form take
-            k_pad = -(-H // 64) * 64 if quant == "fp8" else -(-H // 128) * 128
-        if quant == "fp8":
-            q = torch.empty(T, k_pad, device=dev, dtype=torch.float8_e4m3fn)
-            scale = torch.empty(T, -(-k_pad // 128), device=dev, dtype=torch.float32)
-        else:
-            q = torch.empty(T, k_pad, device=dev, dtype=torch.int8)
-            scale = torch.empty(T, device=dev, dtype=torch.float32)
-        rows, pq, ps = QuantRows(q, scale), q.data_ptr(), scale.data_ptr()
-    check(
-        lib.b200moe_add_rmsnorm(device, _stream(device), x.data_ptr(), sx[0] if T > 1 else H, pr, ldr, pro, ldro,
-                                weight.data_ptr(), int(f32), eps, T, H, po, H, mode, pq, k_pad or 0, ps),
-        "add_rmsnorm",
-    )
-    return NormOut(out, residual_out, rows)
+    return NormOut(*_ext.add_rmsnorm(x, weight, eps, residual, residual_out, mode, k_pad, normed))
 
 
 # --------------------------------------------------------------------------- permutation
@@ -561,113 +411,30 @@ def w8a8_gemm(*, offsets: torch.Tensor, expert_begin: int, n_experts: int, max_r
     return out
 
 
-@dataclass
-class Int8Matrix:
-    """Int8 weights in tile layout (layout.int8_experts / int8_linear) with
-    what the int8 GEMM has to know of them; checked once, here."""
-
-    n_experts: int
-    planes: int              # 2: gate and up, 1: one projection
-    n_feat: int              # output features (of a plane)
-    k_valid: int             # input columns
-    feat_pad: int
-    k_pad: int
-    weight: torch.Tensor     # int8 tiles
-    scale: torch.Tensor      # fp32 per channel, tile row order
-    bias: torch.Tensor | None
-    epilogue: int
-    alpha: float = 1.702
-    limit: float = 7.0
-
-    def __post_init__(self):
-        tiles = self.n_experts * (self.feat_pad // (64 if self.planes == 2 else 128))
-        w = self.weight
-        if w.dtype != torch.int8 or not w.is_contiguous() or w.numel() != tiles * 128 * self.k_pad:
-            raise ValueError(f"weight must be contiguous int8 tiles of {tiles * 128 * self.k_pad} elements")
-        for t, what in ((self.scale, "scale"), (self.bias, "bias")):
-            if t is not None and (t.dtype != torch.float32 or not t.is_contiguous() or t.numel() != tiles * 128
-                                  or t.device != w.device):
-                raise ValueError(f"{what} must be contiguous float32 of {tiles * 128} elements on {w.device}")
-
-
-def _int8_args(m: Int8Matrix, device: int, offsets, expert_begin: int, R: int, b_rows: int, row_weight, row_src, out,
-               token_tile: int):
-    """The GemmArgs of an int8 launch (the fields of b200moe_gemm_args in order)."""
-    so = out.stride()
-    if out.dtype != torch.bfloat16 or len(so) != 2 or so[1] != 1 or out.get_device() != device:
-        raise ValueError(f"output must be a 2D bfloat16 tensor with contiguous rows on {m.weight.device}")
-    ro, co = out.shape
-    if ro < R or co < m.n_feat:
-        raise ValueError(f"output must hold {R} rows of {m.n_feat} columns, got {tuple(out.shape)}")
-    po = prw = prs = None
-    bf = 0
-    if offsets is not None:
-        if (offsets.get_device() != device or offsets.dtype != torch.int32 or not offsets.is_contiguous()
-                or offsets.numel() <= expert_begin + m.n_experts):
-            raise ValueError(f"offsets must be contiguous int32 covering the experts, on {m.weight.device}")
-        po = offsets.data_ptr()
-    if row_weight is not None:
-        bf = _BF16_FLAG.get(row_weight.dtype)
-        if (bf is None or not row_weight.is_contiguous() or row_weight.get_device() != device
-                or row_weight.numel() < R):
-            raise ValueError(f"row_weight must be contiguous float32 or bfloat16, one per row, on {m.weight.device}")
-        if (row_src is None or row_src.dtype != torch.int32 or row_src.numel() < R or not row_src.is_contiguous()
-                or row_src.get_device() != device):
-            raise ValueError(f"row_weight needs row_src (contiguous int32, one entry per row) on {m.weight.device}")
-        prw, prs = row_weight.data_ptr(), row_src.data_ptr()
-    return _lib.GemmArgs(
-        po, expert_begin, m.n_experts, R, token_tile, 0, _lib.W_INT8, m.planes, m.feat_pad, m.n_feat, m.k_pad,
-        m.weight.data_ptr(), 0, 0, None, 0, b_rows, 0, None, 1, m.epilogue, None, m.alpha, m.limit, prw, bf, prs,
-        out.data_ptr(), so[0] if ro > 1 else co)
+Int8Matrix = _ext.Int8Matrix
 
 
 def int8_gemm(m: Int8Matrix, rows: QuantRows, *, offsets: torch.Tensor | None = None, expert_begin: int = 0,
               max_rows: int | None = None, row_weight: torch.Tensor | None = None,
-              row_src: torch.Tensor | None = None, out: torch.Tensor, token_tile: int = 0) -> torch.Tensor:
+              row_src: torch.Tensor | None = None, out: torch.Tensor | None = None,
+              token_tile: int = 0) -> torch.Tensor:
     """Int8 grouped GEMM (b200moe_int8_gemm) of int8 permuted rows with one
     scale each (``act_quant_int8``'s outputs). ``offsets`` None: one expert
-    holds all rows. ``max_rows``: how many of ``rows`` may be an expert's."""
-    device = _dev(m.weight, "weight")
-    rows.checked(torch.int8, m.k_pad, m.weight.device)
-    n = rows.q.shape[0]
-    R = n if max_rows is None else max_rows
-    a = _int8_args(m, device, offsets, expert_begin, R, n, row_weight, row_src, out, token_tile)
-    check(lib.b200moe_int8_gemm(device, _stream(device), ctypes.byref(a), rows.q.data_ptr(), rows.scale.data_ptr(),
-                                m.scale.data_ptr(), None if m.bias is None else m.bias.data_ptr()), "int8_gemm")
-    return out
+    holds all rows. ``max_rows``: how many of ``rows`` may be an expert's.
+    ``out`` (bf16, at least that many rows) is allocated when not given, with
+    ``m.feat_pad`` columns for a gated matrix, ``m.n_feat`` otherwise."""
+    return _ext.int8_gemm(m, rows, offsets, expert_begin, max_rows, row_weight, row_src, out, token_tile)
 
 
 def int8_project(m: Int8Matrix, x: torch.Tensor, *, offsets: torch.Tensor | None = None, expert_begin: int = 0,
                  inverse: torch.Tensor | None = None, copies: int = 1, row_weight: torch.Tensor | None = None,
-                 row_src: torch.Tensor | None = None, out: torch.Tensor, token_tile: int = 0) -> torch.Tensor:
+                 row_src: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                 token_tile: int = 0) -> torch.Tensor:
     """``act_quant_int8`` of the first ``m.k_valid`` columns of bf16 rows ``x``
     (each to its ``copies`` places ``inverse`` of the permuted order) and
     ``int8_gemm`` on them, in one library call (b200moe_int8_project): the
     weights' first tiles load while the rows are quantised."""
-    device = _dev(m.weight, "weight")
-    sx = x.stride()
-    if x.dtype != torch.bfloat16 or len(sx) != 2 or sx[1] != 1 or x.get_device() != device:
-        raise ValueError(f"x must be a 2-D bfloat16 tensor with unit column stride on {m.weight.device}")
-    rows, cols = x.shape
-    if cols < m.k_valid:
-        raise ValueError(f"x has {cols} columns, the weights take {m.k_valid}")
-    R, inv = rows, None
-    if inverse is not None:
-        R = rows * copies
-        if (inverse.dtype != torch.int32 or not inverse.is_contiguous() or inverse.numel() != R
-                or inverse.get_device() != device):
-            raise ValueError(f"inverse must be contiguous int32 of rows * copies = {R} elements on {m.weight.device}")
-        inv = inverse.data_ptr()
-    elif copies != 1:
-        raise ValueError("copies need inverse")
-    a = _int8_args(m, device, offsets, expert_begin, R, R, row_weight, row_src, out, token_tile)
-    nbytes = lib.b200moe_int8_project_workspace(R, m.k_pad)
-    ws = torch.empty(nbytes, device=out.device, dtype=torch.uint8)
-    check(lib.b200moe_int8_project(device, _stream(device), ctypes.byref(a), x.data_ptr(),
-                                   sx[0] if rows > 1 else m.k_valid, rows, m.k_valid, inv, copies,
-                                   m.scale.data_ptr(), None if m.bias is None else m.bias.data_ptr(), ws.data_ptr(),
-                                   nbytes), "int8_project")
-    return out
+    return _ext.int8_project(m, x, offsets, expert_begin, inverse, copies, row_weight, row_src, out, token_tile)
 
 
 # --------------------------------------------------------------------------- combine
