@@ -50,7 +50,7 @@ int* g_status_ptr[kMaxDevices] = {};
 int g_sm_count[kMaxDevices] = {};
 bool g_gemm_attr[kMaxDevices] = {};
 bool g_w8a8_attr[kMaxDevices][4] = {};
-bool g_int8_attr[kMaxDevices][5] = {};
+bool g_int8_attr[kMaxDevices][6] = {};
 void* g_permute_scratch_ptr[kMaxDevices] = {};
 
 int use_device(int device, int** status) {
@@ -905,12 +905,15 @@ static int int8_gemm_launch(int device, int* sp, void* stream, const b200moe_gem
   p.out = static_cast<__nv_bfloat16*>(a->out);
   p.ldo = a->ldo;
   p.status = sp;
-  p.box = std::min(bn, 64);
+  // CTA pairs for the largest tile, where two feature tiles share the token rows
+  const long long wrows = (long long)a->n_experts * feat_tiles * p.nkb * 128;
+  const bool pair = bn == 256 && feat_tiles >= 2 && wrows < 0x7fffffffll;
+  p.box = pair ? 64 : std::min(bn, 128);
   p.early = after_quant ? 1 : 0;
   // shared memory: stages of a 16 KB weight image and bn x 128 B token rows,
   // the epilogue's scales, barriers and the tile prefix
   const uint32_t budget = 232448u - 2048u;
-  p.stage_bytes = 16384u + static_cast<uint32_t>(bn) * 128u;
+  p.stage_bytes = 16384u + static_cast<uint32_t>(pair ? bn / 2 : bn) * 128u;
   const uint32_t xbytes = (b200::int8_epilogue_bytes(bn) + 1023u) & ~1023u;
   const uint32_t barbytes = ((8u * (2u * 16u + 5u) + 8u + 4u * (a->n_experts + 1) + 1023u) / 1024u) * 1024u;
   p.ns = static_cast<int>(std::min<uint32_t>(16u, (budget - xbytes - barbytes) / p.stage_bytes));
@@ -933,8 +936,20 @@ static int int8_gemm_launch(int device, int* sp, void* stream, const b200moe_gem
                       CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (cr != CUDA_SUCCESS) return fail(B200MOE_ERR_CUDA, "activation tensor map failed (%d)", (int)cr);
   }
-  const int ti = bn == 16 ? 0 : bn == 32 ? 1 : bn == 64 ? 2 : bn == 128 ? 3 : 4;
-  const void* kern = b200::int8_kernel_ptr(bn);
+  CUtensorMap wmap;
+  std::memset(&wmap, 0, sizeof(wmap));
+  if (pair) {   // the images as rows of 128 bytes: a copy that may signal the peer CTA is a tensor copy
+    const cuuint64_t dims[2] = {128, static_cast<cuuint64_t>(wrows)};
+    const cuuint64_t strides[1] = {128};
+    const cuuint32_t box[2] = {128, 128};
+    const cuuint32_t estr[2] = {1, 1};
+    CUresult cr = enc(&wmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(a->weight), dims, strides, box, estr,
+                      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (cr != CUDA_SUCCESS) return fail(B200MOE_ERR_CUDA, "weight tensor map failed (%d)", (int)cr);
+  }
+  const int ti = pair ? 5 : bn == 16 ? 0 : bn == 32 ? 1 : bn == 64 ? 2 : bn == 128 ? 3 : 4;
+  const void* kern = pair ? b200::int8_pair_kernel_ptr() : b200::int8_kernel_ptr(bn);
   {
     std::lock_guard<std::mutex> lock(g_mu);
     if (!g_int8_attr[device][ti]) {
@@ -942,7 +957,8 @@ static int int8_gemm_launch(int device, int* sp, void* stream, const b200moe_gem
       g_int8_attr[device][ti] = true;
     }
   }
-  const int grid = static_cast<int>(std::min<long long>(g_sm_count[device], tiles_ub));
+  int grid = static_cast<int>(std::min<long long>(g_sm_count[device], tiles_ub));
+  if (pair) grid = std::max(2, grid & ~1);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid, 1, 1);
   cfg.blockDim = dim3(b200::kInt8Threads, 1, 1);
@@ -950,13 +966,17 @@ static int int8_gemm_launch(int device, int* sp, void* stream, const b200moe_gem
   cfg.stream = static_cast<cudaStream_t>(stream);
   // the launch may begin before the stream's previous kernel has ended; the
   // kernel waits for that end itself
-  cudaLaunchAttribute attr = {};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  void* args[] = {&qmap, &p};
-  B200_CUDA(cudaLaunchKernelExC(&cfg, kern, args));
+  cudaLaunchAttribute attr[2] = {};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 2;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pair ? 2 : 1;
+  void* single_args[] = {&qmap, &p};
+  void* pair_args[] = {&qmap, &wmap, &p};
+  B200_CUDA(cudaLaunchKernelExC(&cfg, kern, pair ? pair_args : single_args));
   return B200MOE_OK;
 }
 

@@ -136,8 +136,9 @@ struct Int8Params {
   int early;                   // only q and qs depend on the stream's previous kernel
   uint32_t stage_bytes, x_off, bar_off, tmem_cols;
 };
-constexpr int kInt8Threads = 320;    // copy warp, MMA warp, 8 epilogue warps
+constexpr int kInt8Threads = 352;    // weight copies, MMAs, 8 epilogue warps, token row copies
 const void* int8_kernel_ptr(int bn); // token tile 16, 32, 64, 128 or 256; else NULL
+const void* int8_pair_kernel_ptr();  // CTA pairs, token tile 256
 uint32_t int8_epilogue_bytes(int bn);
 
 size_t permute_workspace_bytes(int T, int K, int E);
