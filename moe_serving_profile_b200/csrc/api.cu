@@ -921,7 +921,7 @@ static int int8_gemm_launch(int device, int* sp, void* stream, const b200moe_gem
   p.x_off = p.ns * p.stage_bytes;
   p.bar_off = p.x_off + xbytes;
   const uint32_t smem = p.bar_off + barbytes + 1024u;   // + alignment slack
-  p.tmem_cols = static_cast<uint32_t>(std::max(32, 2 * bn));
+  p.tmem_cols = b200::int8_tmem_columns(bn);
 
   PFN_cuTensorMapEncodeTiled_v12000 enc = encode_fn();
   if (!enc) return fail(B200MOE_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");

@@ -37,6 +37,9 @@ constexpr uint32_t kAStage = 16384;   // 128 weight rows x 128 int8
 
 enum { kEpiClampF32 = 3, kEpiSwigluF32 = 5, kEpiDownOnce = 6 };
 
+// Accumulators of a tile: 2 slots x banks x BN columns fit tensor memory.
+__host__ __device__ constexpr int banks(int bn) { return bn <= 64 ? 4 : bn == 128 ? 2 : 1; }
+
 struct Tile {
   int e, ft, row0, nrows;
 };
@@ -127,68 +130,77 @@ __device__ __forceinline__ int count_chunks(const Int8Params& p, int* prefix) {
 }
 
 // Columns first * 16 .. + 15, + 32 .. + 47, ... of one accumulator (this
-// warp's lanes at `acc`): scaled, gated or weighted, and stored as feature f of
-// the rows at `out`.
+// warp's lanes at `acc`, NB banks of BN columns): added, scaled, gated or
+// weighted, and stored as feature f of the rows at `out`.
+template <int BN, int NB>
 __device__ __forceinline__ void epilogue(const Int8Params& p, uint32_t acc, int first, int nrows, int f,
                                          const float* sa, const float* rw, float ws, float bias, float nlog,
                                          uint16_t* out) {
   const bool is_gate = (threadIdx.x & 31) < 16;
-        for (int c0 = first * 16; c0 < nrows; c0 += 32) {
-          uint32_t v[16];
-          tmem_ld16(acc + static_cast<uint32_t>(c0), v);
-          tmem_ld_wait();
-          float d[16];
-  #pragma unroll
-          for (int j = 0; j < 16; ++j)
-            d[j] = fmaf(static_cast<float>(static_cast<int>(v[j])), sa[c0 + j] * ws, bias);
-          const bool whole = c0 + 16 <= nrows;
-          if (p.gated) {
-            // gate lanes take the even columns, up lanes the odd ones
-            float g[8], u[8];
-  #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const float got = __shfl_xor_sync(kFull, is_gate ? d[2 * j + 1] : d[2 * j], 16);
-              g[j] = is_gate ? d[2 * j] : got;
-              u[j] = is_gate ? got : d[2 * j + 1];
-            }
-            if (p.epi == kEpiClampF32) {
-  #pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                g[j] = g[j] > p.limit ? p.limit : g[j];
-                u[j] = (u[j] < -p.limit ? -p.limit : (u[j] > p.limit ? p.limit : u[j])) + 1.f;
-              }
-            }
-  #pragma unroll
-            for (int j = 0; j < 8; ++j) g[j] = glu(g[j], u[j], nlog);
-            const int n0 = c0 + (is_gate ? 0 : 1);
-            uint16_t* o = out + n0 * p.ldo;
-            if (f < p.n_feat) {
-              if (whole) {
-  #pragma unroll
-                for (int j = 0; j < 8; ++j) o[2 * j * p.ldo] = bf16_bits(g[j]);
-              } else {
-  #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                  if (n0 + 2 * j < nrows) o[2 * j * p.ldo] = bf16_bits(g[j]);
-              }
-            }
-          } else if (f < p.n_feat) {
-            uint16_t* o = out + c0 * p.ldo;
-            if (whole) {
-  #pragma unroll
-              for (int j = 0; j < 16; ++j) o[j * p.ldo] = bf16_bits(d[j] * rw[c0 + j]);
-            } else {
-  #pragma unroll
-              for (int j = 0; j < 16; ++j)
-                if (c0 + j < nrows) o[j * p.ldo] = bf16_bits(d[j] * rw[c0 + j]);
-            }
-          }
+  for (int c0 = first * 16; c0 < nrows; c0 += 32) {
+    uint32_t part[NB][16], v[16];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) tmem_ld16(acc + static_cast<uint32_t>(b * BN + c0), part[b]);
+    tmem_ld_wait();
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      v[j] = part[0][j];
+#pragma unroll
+      for (int b = 1; b < NB; ++b) v[j] += part[b][j];
+    }
+    float d[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      d[j] = fmaf(static_cast<float>(static_cast<int>(v[j])), sa[c0 + j] * ws, bias);
+    const bool whole = c0 + 16 <= nrows;
+    if (p.gated) {
+      // gate lanes take the even columns, up lanes the odd ones
+      float g[8], u[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float got = __shfl_xor_sync(kFull, is_gate ? d[2 * j + 1] : d[2 * j], 16);
+        g[j] = is_gate ? d[2 * j] : got;
+        u[j] = is_gate ? got : d[2 * j + 1];
+      }
+      if (p.epi == kEpiClampF32) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          g[j] = g[j] > p.limit ? p.limit : g[j];
+          u[j] = (u[j] < -p.limit ? -p.limit : (u[j] > p.limit ? p.limit : u[j])) + 1.f;
         }
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) g[j] = glu(g[j], u[j], nlog);
+      const int n0 = c0 + (is_gate ? 0 : 1);
+      uint16_t* o = out + n0 * p.ldo;
+      if (f < p.n_feat) {
+        if (whole) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) o[2 * j * p.ldo] = bf16_bits(g[j]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (n0 + 2 * j < nrows) o[2 * j * p.ldo] = bf16_bits(g[j]);
+        }
+      }
+    } else if (f < p.n_feat) {
+      uint16_t* o = out + c0 * p.ldo;
+      if (whole) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) o[j * p.ldo] = bf16_bits(d[j] * rw[c0 + j]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          if (c0 + j < nrows) o[j * p.ldo] = bf16_bits(d[j] * rw[c0 + j]);
+      }
+    }
+  }
 }
 
 template <int BN>
 __global__ void __launch_bounds__(kThreads, 1)
     int8_gemm_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ Int8Params p) {
+  constexpr int NB = banks(BN);
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_u32 = smem_u32(smem_raw);
   const uint32_t base_u32 = (raw_u32 + 1023u) & ~1023u;
@@ -286,37 +298,46 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp == 1) {
     // ------------------------------------------------ MMAs
-    if (lane == 0) {
-      Ring ring(p.ns);
-      int tc = 0;
-      bool ok = true;
-      for (int t = blockIdx.x; ok && t < total; t += gridDim.x) {
-        const Tile tl = decode_tile<16>(t, p.feat_tiles, prefix, p);
-        if (tl.nrows <= 0) continue;
-        const int slot = tc & 1;
-        if (!wait_bounded(&acc_empty[slot], ((tc >> 1) & 1) ^ 1, p.status)) break;
-        const uint32_t idesc = idesc_s8_s32(128, (tl.nrows + 15) & ~15);
-        const uint32_t d = tmem + static_cast<uint32_t>(slot * BN);
-        for (int k = 0; k < p.nkb; ++k, ring.next()) {
-          const int s = ring.idx;
-          if (!wait_bounded(&full[s], ring.phase, p.status)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          const uint32_t st = base_u32 + s * p.stage_bytes;
-          const uint64_t ad = sdesc_k_sw128(st), bd = sdesc_k_sw128(st + kAStage);
+    // The whole warp runs the loop and one lane issues: the descriptors are
+    // then uniform values, where a loop of one lane moved each of them over
+    // (116 cycles an MMA).
+    Ring ring(p.ns);
+    int tc = 0;
+    bool ok = true;
+    const uint32_t acc = __shfl_sync(kFull, tmem, 0);
+    for (int t = blockIdx.x; ok && t < total; t += gridDim.x) {
+      const Tile tl = decode_tile<16>(t, p.feat_tiles, prefix, p);
+      const int nrows = __shfl_sync(kFull, tl.nrows, 0);
+      if (nrows <= 0) continue;
+      const int slot = tc & 1;
+      if (!__all_sync(kFull, wait_bounded(&acc_empty[slot], ((tc >> 1) & 1) ^ 1, p.status))) break;
+      const uint32_t idesc = idesc_s8_s32(128, (nrows + 15) & ~15);
+      const uint32_t d = acc + static_cast<uint32_t>(slot * NB * BN);
+      for (int k = 0; k < p.nkb; ++k, ring.next()) {
+        const int s = ring.idx;
+        if (!__all_sync(kFull, wait_bounded(&full[s], ring.phase, p.status))) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t st = base_u32 + s * p.stage_bytes;
+        const uint64_t ad = sdesc_k_sw128(st), bd = sdesc_k_sw128(st + kAStage);
+        if (elect_one()) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) umma_s8(d, ad + 2 * j, bd + 2 * j, idesc, (k | j) != 0 ? 1u : 0u);
+          for (int j = 0; j < 4; ++j)
+            umma_s8(d + (j % NB) * BN, ad + 2 * j, bd + 2 * j, idesc, k != 0 || j >= NB ? 1u : 0u);
           umma_commit(&empty[s]);
         }
-        umma_commit(&acc_full[slot]);
-        ++tc;
+        __syncwarp();
       }
-      // all issued MMAs have finished before tensor memory is released
-      umma_commit(mma_done);
-      wait_bounded(mma_done, 0, p.status);
+      if (elect_one()) umma_commit(&acc_full[slot]);
+      __syncwarp();
+      ++tc;
     }
+    // all issued MMAs have finished before tensor memory is released
+    if (elect_one()) umma_commit(mma_done);
+    __syncwarp();
+    wait_bounded(mma_done, 0, p.status);
   } else {
     // ------------------------------------------------ epilogue
     // Warp w reads lanes 32 (w % 4) .. + 31 of tensor memory: lane i holds
@@ -348,7 +369,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!named_bar_and(1, kEpi, wait_bounded(&acc_full[slot], (tc >> 1) & 1, p.status))) break;
       tc_fence_after();
       uint16_t* out = reinterpret_cast<uint16_t*>(p.out) + (long long)tl.row0 * p.ldo + f;
-      epilogue(p, tq + static_cast<uint32_t>(slot * BN), first, tl.nrows, f, sa, rw, ws, bias, nlog, out);
+      epilogue<BN, NB>(p, tq + static_cast<uint32_t>(slot * NB * BN), first, tl.nrows, f, sa, rw, ws, bias, nlog, out);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&acc_empty[slot]);
@@ -479,37 +500,44 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp == 1) {
     // ------------------------------------------------ MMAs of the pair
-    if (lane == 0 && rank == 0) {
+    if (rank == 0) {
       Ring ring(p.ns);
       int tc = 0;
       bool ok = true;
+      const uint32_t acc = __shfl_sync(kFull, tmem, 0);
       for (int t = first_tile; ok && t < total; t += step) {
         const Tile tl = decode_tile<32>(t, pairs, prefix, p);
-        if (tl.nrows <= 0) continue;
+        const int nrows = __shfl_sync(kFull, tl.nrows, 0);
+        if (nrows <= 0) continue;
         const int slot = tc & 1;
-        if (!wait_bounded_cluster(&acc_empty[slot], ((tc >> 1) & 1) ^ 1, p.status)) break;
-        const uint32_t idesc = idesc_s8_s32(256, (tl.nrows + 31) & ~31);
-        const uint32_t d = tmem + static_cast<uint32_t>(slot * BN);
+        if (!__all_sync(kFull, wait_bounded_cluster(&acc_empty[slot], ((tc >> 1) & 1) ^ 1, p.status))) break;
+        const uint32_t idesc = idesc_s8_s32(256, (nrows + 31) & ~31);
+        const uint32_t d = acc + static_cast<uint32_t>(slot * BN);
         for (int k = 0; k < p.nkb; ++k, ring.next()) {
           const int s = ring.idx;
-          if (!wait_bounded(&full[s], ring.phase, p.status)) {
+          if (!__all_sync(kFull, wait_bounded(&full[s], ring.phase, p.status))) {
             ok = false;
             break;
           }
           tc_fence_after();
           const uint32_t st = base_u32 + s * p.stage_bytes;
           const uint64_t ad = sdesc_k_sw128(st), bd = sdesc_k_sw128(st + kAStage);
+          if (elect_one()) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) umma_s8_pair(d, ad + 2 * j, bd + 2 * j, idesc, (k | j) != 0 ? 1u : 0u);
-          umma_commit_pair(&empty[s]);
+            for (int j = 0; j < 4; ++j) umma_s8_pair(d, ad + 2 * j, bd + 2 * j, idesc, (k | j) != 0 ? 1u : 0u);
+            umma_commit_pair(&empty[s]);
+          }
+          __syncwarp();
         }
-        umma_commit_pair(&acc_full[slot]);
+        if (elect_one()) umma_commit_pair(&acc_full[slot]);
+        __syncwarp();
         ++tc;
       }
       // all issued MMAs have finished before tensor memory is released
-      umma_commit_pair(mma_done);
+      if (elect_one()) umma_commit_pair(mma_done);
+      __syncwarp();
     }
-    if (lane == 0) wait_bounded(mma_done, 0, p.status);
+    wait_bounded(mma_done, 0, p.status);
   } else {
     // ------------------------------------------------ epilogue of this CTA's feature tile
     const int q = warp & 3, r = q * 32 + lane;
@@ -539,7 +567,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!named_bar_and(1, kEpi, wait_bounded(&acc_full[slot], (tc >> 1) & 1, p.status))) break;
       tc_fence_after();
       uint16_t* out = reinterpret_cast<uint16_t*>(p.out) + (long long)tl.row0 * p.ldo + f;
-      epilogue(p, tq + static_cast<uint32_t>(slot * BN), first, tl.nrows, f, sa, rw, ws, bias, nlog, out);
+      epilogue<BN, 1>(p, tq + static_cast<uint32_t>(slot * BN), first, tl.nrows, f, sa, rw, ws, bias, nlog, out);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&acc_empty[slot]), 0));
@@ -556,6 +584,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 }  // namespace i8
+
+uint32_t int8_tmem_columns(int bn) { return 2u * i8::banks(bn) * static_cast<uint32_t>(bn); }
 
 // Row scales and routing weights of two tiles.
 uint32_t int8_epilogue_bytes(int bn) { return 16u * static_cast<uint32_t>(bn); }

@@ -140,6 +140,7 @@ constexpr int kInt8Threads = 352;    // weight copies, MMAs, 8 epilogue warps, t
 const void* int8_kernel_ptr(int bn); // token tile 16, 32, 64, 128 or 256; else NULL
 const void* int8_pair_kernel_ptr();  // CTA pairs, token tile 256
 uint32_t int8_epilogue_bytes(int bn);
+uint32_t int8_tmem_columns(int bn);  // a power of two from 128 to 512
 
 size_t permute_workspace_bytes(int T, int K, int E);
 cudaError_t launch_permute(cudaStream_t st, const long long* indices, int T, int K, int E,

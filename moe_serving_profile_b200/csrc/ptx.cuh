@@ -169,6 +169,13 @@ B200_DEVI void tma_gather4(void* dst, const CUtensorMap* map, uint64_t* bar, int
       : "memory");
 }
 
+// True in one lane of the (converged) warp.
+B200_DEVI bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(r));
+  return r != 0;
+}
+
 // Barrier among `count` threads (a multiple of 32) on hardware barrier `id`.
 B200_DEVI void named_bar_sync(int id, int count) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(count) : "memory");
