@@ -915,8 +915,10 @@ static int int8_gemm_launch(int device, int* sp, void* stream, const b200moe_gem
   const uint32_t budget = 232448u - 2048u;
   p.stage_bytes = 16384u + static_cast<uint32_t>(pair ? bn / 2 : bn) * 128u;
   const uint32_t xbytes = (b200::int8_epilogue_bytes(bn) + 1023u) & ~1023u;
-  const uint32_t barbytes = ((8u * (2u * 16u + 5u) + 8u + 4u * (a->n_experts + 1) + 1023u) / 1024u) * 1024u;
-  p.ns = static_cast<int>(std::min<uint32_t>(16u, (budget - xbytes - barbytes) / p.stage_bytes));
+  const uint32_t barbytes = ((8u * (2u * 16u + 5u) + 8u + 8u * (a->n_experts + 1) + 1023u) / 1024u) * 1024u;
+  // at most 8 stages: 16-row tiles had room for 11, but streamed weights slower
+  // with them (gate/up at 64 tokens: 8 stages 64 us, 6 66 us, 11 67 us)
+  p.ns = static_cast<int>(std::min<uint32_t>(8u, (budget - xbytes - barbytes) / p.stage_bytes));
   if (p.ns < 2) return fail(B200MOE_ERR_UNSUPPORTED, "shared memory plan does not fit (token_tile=%d)", bn);
   p.x_off = p.ns * p.stage_bytes;
   p.bar_off = p.x_off + xbytes;

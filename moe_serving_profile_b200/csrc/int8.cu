@@ -56,18 +56,12 @@ struct Ring {
   }
 };
 
-// Rows [x, y) of local expert e in the permuted order (no offsets: one expert
-// holds all rows).
-__device__ __forceinline__ int2 expert_rows(const Int8Params& p, int e) {
-  if (p.offsets == nullptr) return make_int2(0, p.dense_rows);
-  return make_int2(p.offsets[p.expert_begin + e], p.offsets[p.expert_begin + e + 1]);
-}
-
 // Tile t: feature tile (or pair of them) t % ftiles of row chunk t / ftiles. An
 // expert's rows are cut into ceil(rows / BN) chunks of equal size rounded up to
 // the MMA's N granule, so that no chunk is nearly empty.
 template <int GRAN>
-__device__ __forceinline__ Tile decode_tile(int t, int ftiles, const int* prefix, const Int8Params& p) {
+__device__ __forceinline__ Tile decode_tile(int t, int ftiles, const int* prefix, const int* starts,
+                                            const Int8Params& p) {
   Tile r;
   const int u = t / ftiles;
   r.ft = t - u * ftiles;
@@ -78,8 +72,7 @@ __device__ __forceinline__ Tile decode_tile(int t, int ftiles, const int* prefix
   }
   r.e = lo;
   const int sub = u - prefix[lo], parts = prefix[lo + 1] - prefix[lo];
-  const int2 rows = expert_rows(p, lo);
-  const int start = rows.x, cnt = rows.y - rows.x;
+  const int start = starts[lo], cnt = starts[lo + 1] - start;
   const int size = ((cnt + parts - 1) / parts + GRAN - 1) / GRAN * GRAN;
   r.row0 = start + sub * size;
   r.nrows = min(size, cnt - sub * size);   // rounding up may leave the last chunk empty
@@ -104,27 +97,43 @@ __device__ __forceinline__ float glu(float g, float u, float nlog) {   // nlog =
 
 __device__ __forceinline__ uint16_t bf16_bits(float f) { return __bfloat16_as_ushort(__float2bfloat16_rn(f)); }
 
-// Exclusive prefix of the experts' row chunks (warp 0); returns their total.
+// starts[e]: the permuted row where local expert e's rows begin (without
+// offsets one expert holds all rows); prefix: exclusive prefix of the experts'
+// row chunks. By warp 0, 128 experts at a time, so that their offsets arrive
+// together. Returns the number of chunks.
 template <int BN>
-__device__ __forceinline__ int count_chunks(const Int8Params& p, int* prefix) {
+__device__ __forceinline__ int count_chunks(const Int8Params& p, int* prefix, int* starts) {
   const int lane = threadIdx.x & 31;
   int acc = 0;
   if (lane == 0) prefix[0] = 0;
-  for (int base = 0; base < p.n_experts; base += 32) {
-    const int e = base + lane;
-    int nt = 0;
-    if (e < p.n_experts) {
-      const int2 rows = expert_rows(p, e);
-      nt = (rows.y - rows.x + BN - 1) / BN;
-    }
-    int incl = nt;
+  for (int base = 0; base < p.n_experts; base += 128) {
+    int at[4];
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(kFull, incl, o);
-      if (lane >= o) incl += v;
+    for (int i = 0; i < 4; ++i) {
+      const int e = min(base + 32 * i + lane, p.n_experts);
+      at[i] = p.offsets ? p.offsets[p.expert_begin + e] : (e ? p.dense_rows : 0);
     }
-    if (e < p.n_experts) prefix[e + 1] = acc + incl;
-    acc += __shfl_sync(kFull, incl, 31);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int e = base + 32 * i + lane;
+      if (e <= p.n_experts) starts[e] = at[i];
+    }
+    const int last = min(base + 128, p.n_experts);   // the next lane's start: from the next vector, or memory
+    const int end = p.offsets ? p.offsets[p.expert_begin + last] : p.dense_rows;
+    if (lane == 0) starts[last] = end;
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int e = base + 32 * i + lane;
+      int incl = e < p.n_experts ? (starts[e + 1] - at[i] + BN - 1) / BN : 0;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(kFull, incl, o);
+        if (lane >= o) incl += v;
+      }
+      if (e < p.n_experts) prefix[e + 1] = acc + incl;
+      acc += __shfl_sync(kFull, incl, 31);
+    }
   }
   return acc;
 }
@@ -216,12 +225,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(mma_done + 1);
   int* s_total = reinterpret_cast<int*>(s_tmem + 1);
   int* prefix = s_total + 1;            // [n_experts + 1]: row chunks of the experts before
+  int* starts = prefix + p.n_experts + 1;   // [n_experts + 1]
 
   if (warp == 0) {
     // what the row chunks are counted from may come from the previous kernel
     if (!p.early) grid_dep_wait();
     const int bad = *reinterpret_cast<volatile int*>(p.status) & kStatusWaitTimeout;
-    const int chunks = count_chunks<BN>(p, prefix);
+    const int chunks = count_chunks<BN>(p, prefix, starts);
     if (lane == 0) {
       *s_total = bad ? 0 : chunks * p.feat_tiles;   // after a wait gave up: nothing to do
       for (int i = 0; i < p.ns; ++i) {
@@ -254,7 +264,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       int issued = 0;
       bool ok = true;
       for (int t = blockIdx.x; ok && t < total; t += gridDim.x) {
-        const Tile tl = decode_tile<16>(t, p.feat_tiles, prefix, p);
+        const Tile tl = decode_tile<16>(t, p.feat_tiles, prefix, starts, p);
         if (tl.nrows <= 0) continue;
         const uint8_t* wt = p.wtiles + (long long)(tl.e * p.feat_tiles + tl.ft) * p.nkb * kAStage;
         const uint32_t bytes = kAStage + (tl.nrows + p.box - 1) / p.box * p.box * 128;   // with the token rows
@@ -281,7 +291,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       Ring ring(p.ns);
       bool ok = true;
       for (int t = blockIdx.x; ok && t < total; t += gridDim.x) {
-        const Tile tl = decode_tile<16>(t, p.feat_tiles, prefix, p);
+        const Tile tl = decode_tile<16>(t, p.feat_tiles, prefix, starts, p);
         if (tl.nrows <= 0) continue;
         const int boxes = (tl.nrows + p.box - 1) / p.box;
         for (int k = 0; k < p.nkb; ++k, ring.next()) {
@@ -306,7 +316,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = true;
     const uint32_t acc = __shfl_sync(kFull, tmem, 0);
     for (int t = blockIdx.x; ok && t < total; t += gridDim.x) {
-      const Tile tl = decode_tile<16>(t, p.feat_tiles, prefix, p);
+      const Tile tl = decode_tile<16>(t, p.feat_tiles, prefix, starts, p);
       const int nrows = __shfl_sync(kFull, tl.nrows, 0);
       if (nrows <= 0) continue;
       const int slot = tc & 1;
@@ -351,7 +361,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     int tc = 0;
     grid_dep_wait();   // row scales and routing weights are read, and rows written, below
     for (int t = blockIdx.x; t < total; t += gridDim.x) {
-      const Tile tl = decode_tile<16>(t, p.feat_tiles, prefix, p);
+      const Tile tl = decode_tile<16>(t, p.feat_tiles, prefix, starts, p);
       if (tl.nrows <= 0) continue;
       const int slot = tc & 1;
       float* sa = xs + (tc & 1) * (2 * BN);
@@ -410,12 +420,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(mma_done + 1);
   int* s_total = reinterpret_cast<int*>(s_tmem + 1);
   int* prefix = s_total + 1;
+  int* starts = prefix + p.n_experts + 1;
   const int pairs = (p.feat_tiles + 1) / 2;
 
   if (warp == 0) {
     if (!p.early) grid_dep_wait();
     const int bad = *reinterpret_cast<volatile int*>(p.status) & kStatusWaitTimeout;
-    const int chunks = count_chunks<BN>(p, prefix);
+    const int chunks = count_chunks<BN>(p, prefix, starts);
     if (lane == 0) {
       *s_total = bad ? 0 : chunks * pairs;
       for (int i = 0; i < p.ns; ++i) {
@@ -453,7 +464,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       int issued = 0;
       bool ok = true;
       for (int t = first_tile; ok && t < total; t += step) {
-        const Tile tl = decode_tile<32>(t, pairs, prefix, p);
+        const Tile tl = decode_tile<32>(t, pairs, prefix, starts, p);
         if (tl.nrows <= 0) continue;
         const int ft = min(2 * tl.ft + static_cast<int>(rank), p.feat_tiles - 1);   // an odd last tile twice
         const int wrow = (tl.e * p.feat_tiles + ft) * p.nkb * 128;
@@ -481,7 +492,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       Ring ring(p.ns);
       bool ok = true;
       for (int t = first_tile; ok && t < total; t += step) {
-        const Tile tl = decode_tile<32>(t, pairs, prefix, p);
+        const Tile tl = decode_tile<32>(t, pairs, prefix, starts, p);
         if (tl.nrows <= 0) continue;
         const int half = ((tl.nrows + 31) & ~31) >> 1;
         const int boxes = (half + p.box - 1) / p.box;
@@ -506,7 +517,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool ok = true;
       const uint32_t acc = __shfl_sync(kFull, tmem, 0);
       for (int t = first_tile; ok && t < total; t += step) {
-        const Tile tl = decode_tile<32>(t, pairs, prefix, p);
+        const Tile tl = decode_tile<32>(t, pairs, prefix, starts, p);
         const int nrows = __shfl_sync(kFull, tl.nrows, 0);
         if (nrows <= 0) continue;
         const int slot = tc & 1;
@@ -549,7 +560,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     int tc = 0;
     grid_dep_wait();
     for (int t = first_tile; t < total; t += step) {
-      const Tile tl = decode_tile<32>(t, pairs, prefix, p);
+      const Tile tl = decode_tile<32>(t, pairs, prefix, starts, p);
       if (tl.nrows <= 0) continue;
       const int slot = tc & 1;
       float* sa = xs + (tc & 1) * (2 * BN);
