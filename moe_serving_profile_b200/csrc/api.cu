@@ -186,8 +186,10 @@ int b200moe_route_grouped(int device, void* stream, const void* logits, int logi
   if (rc) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int blocks = b200::route_grouped_blocks(T, g_sm_count[device]);
-  if (counts && blocks != 1) B200_CUDA(cudaMemsetAsync(counts, 0, sizeof(int) * E, st));
-  if (T == 0) return B200MOE_OK;
+  if (T == 0) {
+    if (counts) B200_CUDA(cudaMemsetAsync(counts, 0, sizeof(int) * E, st));
+    return B200MOE_OK;
+  }
   b200::RouteParams p{};
   p.logits = logits;
   p.bf16 = logits_bf16;

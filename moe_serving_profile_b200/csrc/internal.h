@@ -61,7 +61,6 @@ struct RouteParams {
   long long* indices;
   int* counts;
 };
-// Blocks of a launch; with one, the counts are written and need no zeroing.
 int route_grouped_blocks(int T, int sm_count);
 cudaError_t launch_route_grouped(cudaStream_t st, const RouteParams& p, int blocks);
 

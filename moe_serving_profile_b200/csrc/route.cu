@@ -250,15 +250,26 @@ __device__ __forceinline__ Pick eval(const RouteParams& p, int t, int e, float m
   return r;
 }
 
-template <int NL, bool VEC, bool LOGIT>
+// Zeroes the counts; the selection may begin meanwhile.
+__global__ void __launch_bounds__(512) zero_counts_kernel(int* counts, int E) {
+  grid_dep_launch();
+  if (threadIdx.x < E) counts[threadIdx.x] = 0;
+}
+
+// MODE: 0 loads logits one by one, 1 in vectors of four, 2 also has an expert
+// in every slot of every lane.
+template <int NL, int MODE, bool LOGIT>
 __global__ void __launch_bounds__(kThreads, NL <= 8 ? 2 : 1)
     route_grouped_kernel(const __grid_constant__ RouteParams p) {
   constexpr uint32_t kSlots = NL - 1;   // low bits of a word: NL - 1 - slot
+  constexpr bool VEC = MODE >= 1, FULL = MODE == 2;
   __shared__ int hist[512];
   const int lane = threadIdx.x & 31;
   const int lsh = p.lsh, L = 1 << lsh;
   const int g = lane >> lsh, sub = lane & (L - 1);
   const int E = p.S * p.G;
+  // a block counts in shared memory (16384 tokens adding to one array in global
+  // memory took 20 us longer)
   if (p.counts) {
     for (int e = threadIdx.x; e < E; e += kThreads) hist[e] = 0;
     __syncthreads();
@@ -279,7 +290,7 @@ __global__ void __launch_bounds__(kThreads, NL <= 8 ? 2 : 1)
       x[i] = x[i + 1] = x[i + 2] = x[i + 3] = -INFINITY;
       const long long at = row + L * i;
       if (VEC) {   // S % 4 == 0: the four slots of a vector are live together
-        if ((live >> i) & 1u) {
+        if (FULL || ((live >> i) & 1u)) {
           if (p.bf16) {
             const uint2 v = __ldg(reinterpret_cast<const uint2*>(reinterpret_cast<const __nv_bfloat16*>(p.logits) + at));
             x[i] = __uint_as_float(v.x << 16);
@@ -343,7 +354,7 @@ __global__ void __launch_bounds__(kThreads, NL <= 8 ? 2 : 1)
         for (int i = 0; i < NL; ++i) {
           const uint32_t tag = 0xffffu - (g * p.S + slot_offset(sub, L, i));   // equal logits: the lower id first
           total += x[i];
-          key[i] = ((live >> (VEC ? i & ~3 : i)) & 1u) ? (order32(x[i] + 0.f) & 0xffff0000u) | tag : 0u;   // -0 is 0
+          key[i] = FULL || ((live >> (VEC ? i & ~3 : i)) & 1u) ? (order32(x[i] + 0.f) & 0xffff0000u) | tag : 0u;   // -0 is 0
         }
       }
       if (p.softmax) {
@@ -371,7 +382,7 @@ __global__ void __launch_bounds__(kThreads, NL <= 8 ? 2 : 1)
         for (int i = 0; i < NL; ++i) {
           const float k = x[i] + bias[i];
           total += k;
-          key[i] = ((live >> (VEC ? i & ~3 : i)) & 1u) ? (order32(k) & ~kSlots) | (kSlots - i) : 0u;
+          key[i] = FULL || ((live >> (VEC ? i & ~3 : i)) & 1u) ? (order32(k) & ~kSlots) | (kSlots - i) : 0u;
         }
       }
       bool sure = !__any_sync(kFull, total != total);   // no NaN key (nor infinite ones of both signs)
@@ -467,9 +478,11 @@ __global__ void __launch_bounds__(kThreads, NL <= 8 ? 2 : 1)
   }
   if (p.counts) {
     __syncthreads();
+    const bool alone = gridDim.x == 1;
+    if (!alone) grid_dep_wait();   // the counts are zero
     for (int e = threadIdx.x; e < E; e += kThreads) {
       const int n = hist[e];
-      if (gridDim.x == 1) p.counts[e] = n;
+      if (alone) p.counts[e] = n;
       else if (n) atomicAdd(&p.counts[e], n);
     }
   }
@@ -488,19 +501,37 @@ cudaError_t launch_route_grouped(cudaStream_t st, const RouteParams& p, int bloc
   const uintptr_t item = p.bf16 ? 2 : 4;
   const bool vec = p.S % 4 == 0 && p.ld % 4 == 0 && reinterpret_cast<uintptr_t>(p.logits) % (4 * item) == 0;
   const bool logit = p.bf16 && p.bias == nullptr && (p.keep == p.G || p.top == 1 || p.S == 1);
-#define B200_ROUTE(NL_)                                                                 \
-  do {                                                                                  \
-    if (vec && logit) route_grouped_kernel<NL_, true, true><<<blocks, kThreads, 0, st>>>(p);   \
-    else if (vec) route_grouped_kernel<NL_, true, false><<<blocks, kThreads, 0, st>>>(p);      \
-    else if (logit) route_grouped_kernel<NL_, false, true><<<blocks, kThreads, 0, st>>>(p);    \
-    else route_grouped_kernel<NL_, false, false><<<blocks, kThreads, 0, st>>>(p);              \
+  const bool full = vec && p.S == per_lane * L && p.G * L == 32;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(blocks);
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  if (blocks > 1 && p.counts) {
+    zero_counts_kernel<<<1, 512, 0, st>>>(p.counts, p.S * p.G);
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+  }
+#define B200_ROUTE(NL_)                                                                             \
+  do {                                                                                              \
+    if (logit) {                                                                                    \
+      if (full && per_lane == NL_) return cudaLaunchKernelEx(&cfg, route_grouped_kernel<NL_, 2, true>, p); \
+      if (vec) return cudaLaunchKernelEx(&cfg, route_grouped_kernel<NL_, 1, true>, p);              \
+      return cudaLaunchKernelEx(&cfg, route_grouped_kernel<NL_, 0, true>, p);                       \
+    }                                                                                               \
+    if (full && per_lane == NL_) return cudaLaunchKernelEx(&cfg, route_grouped_kernel<NL_, 2, false>, p);  \
+    if (vec) return cudaLaunchKernelEx(&cfg, route_grouped_kernel<NL_, 1, false>, p);               \
+    return cudaLaunchKernelEx(&cfg, route_grouped_kernel<NL_, 0, false>, p);                        \
   } while (0)
   if (per_lane <= 4) B200_ROUTE(4);
-  else if (per_lane <= 8) B200_ROUTE(8);
-  else if (per_lane <= 16) B200_ROUTE(16);
-  else B200_ROUTE(32);
+  if (per_lane <= 8) B200_ROUTE(8);
+  if (per_lane <= 16) B200_ROUTE(16);
+  B200_ROUTE(32);
 #undef B200_ROUTE
-  return cudaGetLastError();
 }
 
 }  // namespace b200
