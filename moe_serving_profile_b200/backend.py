@@ -12,7 +12,7 @@ from __future__ import annotations
 import torch
 
 NUMERICS = ("reference", "fast", "efficient")
-STORAGE = {"qwen3": ("fp8", "bf16"), "gpt_oss": ("mxfp4", "bf16")}
+STORAGE = {"qwen3": ("fp8", "bf16", "int8"), "gpt_oss": ("mxfp4", "bf16")}
 
 
 def check_runtime(family: str, device, dtype: torch.dtype, storage: str) -> None:

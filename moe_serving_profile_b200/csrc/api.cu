@@ -177,6 +177,7 @@ int b200moe_route_grouped(int device, void* stream, const void* logits, int logi
   if (E > 512 || n_group > 32 || K > 32)
     return fail(B200MOE_ERR_UNSUPPORTED, "grouped routing supports E <= 512, n_group <= 32 and K <= 32 (E=%d "
                 "n_group=%d K=%d)", E, n_group, K);
+  if (T > (1 << 30)) return fail(B200MOE_ERR_UNSUPPORTED, "at most 2^30 tokens (T=%d)", T);
   B200_CHECK(K <= topk_group * (E / n_group), "K=%d exceeds the %d experts of the kept groups", K,
              topk_group * (E / n_group));
   B200_CHECK(ld_logits >= E, "ld_logits must be at least E");

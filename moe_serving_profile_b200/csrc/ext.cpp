@@ -381,7 +381,9 @@ PYBIND11_MODULE(_ext, mod) {
             self.cast<const QuantRows&>().checked(type, k_pad, device);
             return self;
           },
-          "Self, if these are rows of the dtype and width on the device.");
+          "Self, if these are rows of the dtype and width on the device.")
+      .def(py::pickle([](const QuantRows& r) { return py::make_tuple(r.q, r.scale); },
+                      [](py::tuple t) { return QuantRows{t[0].cast<Tensor>(), t[1].cast<Tensor>()}; }));
   py::class_<Int8Matrix>(mod, "Int8Matrix",
                          "Int8 weights in tile layout (layout.int8_experts / int8_linear) with\nwhat the int8 GEMM has "
                          "to know of them; checked once, here.")
@@ -400,7 +402,17 @@ PYBIND11_MODULE(_ext, mod) {
       .def_readonly("bias", &Int8Matrix::bias)
       .def_readonly("epilogue", &Int8Matrix::epilogue)
       .def_readonly("alpha", &Int8Matrix::alpha)
-      .def_readonly("limit", &Int8Matrix::limit);
+      .def_readonly("limit", &Int8Matrix::limit)
+      .def(py::pickle(
+          [](const Int8Matrix& m) {
+            return py::make_tuple(m.n_experts, m.planes, m.n_feat, m.k_valid, m.feat_pad, m.k_pad, m.weight, m.scale,
+                                  m.bias, m.epilogue, m.alpha, m.limit);
+          },
+          [](py::tuple t) {
+            return Int8Matrix(t[0].cast<int>(), t[1].cast<int>(), t[2].cast<int64_t>(), t[3].cast<int64_t>(),
+                              t[4].cast<int64_t>(), t[5].cast<int64_t>(), t[6].cast<Tensor>(), t[7].cast<Tensor>(),
+                              t[8].cast<OptTensor>(), t[9].cast<int>(), t[10].cast<float>(), t[11].cast<float>());
+          }));
   mod.def("route_grouped", &route_grouped);
   mod.def("act_quant_int8", &act_quant_int8);
   mod.def("scatter_rows_8bit", &scatter_rows_8bit);

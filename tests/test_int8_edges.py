@@ -1,0 +1,233 @@
+"""The grouped routing, norm and int8 calls where calls go wrong: offsets past
+32 bits, the same expert twice, signed zeros, two host threads, captured
+replays of long batches, copies of the packed weights."""
+
+from __future__ import annotations
+
+import copy
+import pickle
+import threading
+
+import pytest
+import torch
+
+from moe_serving_profile_b200 import _lib, experts, layout, native, ops
+from tests.test_int8 import distinct, layer64, on, packed, quant
+from tests.test_route_grouped import check, plain
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits(cuda):
+    """Rows behind the 4 GB mark of bf16 inputs and the 2 GB mark of codes equal
+    the same rows alone."""
+    T, H = 600_000, 4096
+    part = torch.randn(64, H, device=cuda).to(torch.bfloat16)
+    x = part.repeat(T // 64, 1)
+    w = torch.rand(H, device=cuda)
+    want = ops.add_rmsnorm(part, w, 1e-6, residual=part, quant="int8")
+    n = ops.add_rmsnorm(x, w, 1e-6, residual=x, quant="int8")
+    for a, b in ((n.out, want.out), (n.residual, want.residual), (n.rows.q, want.rows.q),
+                 (n.rows.scale, want.rows.scale)):
+        assert torch.equal(a[-64:], b) and torch.equal(a[:64], b)
+    lin = layout.int8_linear(*layout.quantize_int8(torch.randn(136, H, device=cuda)))
+    y, y0 = experts.int8_linear(lin, n.rows), experts.int8_linear(lin, want.rows)
+    assert torch.equal(y[-64:], y0) and torch.equal(y[T // 2 // 64 * 64:][:64], y0)
+    del n
+    y = experts.int8_linear(lin, x)
+    assert torch.equal(y[-64:], experts.int8_linear(lin, part))
+    del x, y
+    torch.cuda.empty_cache()
+    logits = torch.randn(64, 512, device=cuda)
+    many = logits.repeat(70_000, 1)                       # 9 GB of fp32 logits
+    r = ops.route_grouped(many, None, 8, n_group=8, topk_group=4)
+    r0 = ops.route_grouped(logits, None, 8, n_group=8, topk_group=4)
+    assert torch.equal(r.indices[-64:], r0.indices) and torch.equal(r.scores[-64:], r0.scores)
+    assert torch.equal(r.counts, r0.counts * 70_000)
+
+
+@pytest.mark.gpu
+def test_one_expert_many_times(cuda):
+    """A token may name an expert twice, and all tokens the same expert."""
+    g = torch.Generator().manual_seed(5)
+    E, H, I, T, K = 8, 128, 64, 90, 3
+    raw, parts, _ = packed(g, E, H, I)
+    w = layout.int8_experts(*on(cuda, *parts)[0])
+    x = torch.randn(T, H, generator=g).to(torch.bfloat16)
+    wt = torch.rand(T, K, generator=g)
+    for idx in (torch.full((T, K), 5), torch.randint(0, E, (T, K), generator=g)):
+        y = experts.layer_forward(w, x.to(cuda), idx.to(cuda), wt.to(cuda), num_experts=E, expert_begin=0,
+                                  numerics="efficient")
+        want = layer64(raw, *quant(x), idx, wt, E)
+        assert float((y.cpu().double() - want).norm() / want.norm()) <= 2.0 ** -8
+
+
+@pytest.mark.gpu
+def test_signed_zero_logits_tie(cuda):
+    for dtype in (torch.float32, torch.bfloat16):
+        x = torch.full((6, 32), -2.0)
+        x[:, 5::7] = 0.0
+        x[:, 3] = -0.0
+        x[1, 20] = -0.0
+        for kw in (dict(), dict(n_group=4, topk_group=2, group_top=1), dict(scoring="softmax")):
+            check(x.to(dtype).to(cuda), None, 4, **kw)
+            check(x.to(dtype).to(cuda), torch.zeros(32, device=cuda), 4, **kw)
+
+
+@pytest.mark.gpu
+def test_saturated_scores_tie(cuda):
+    """Logits whose scores 64 bits round together go by id, others by score."""
+    x = torch.tensor([[40.0, 50.0, 45.0, 38.0, 16.0, 15.5, 17.0, 37.5],
+                      [-800.0, -750.0, -900.0, -600.0, -500.0, -1000.0, -20.0, -700.0]])
+    for dtype in (torch.float32, torch.bfloat16):
+        for scoring in ("sigmoid", "softmax"):
+            for kw in (dict(), dict(n_group=4, topk_group=3, group_top=1)):
+                check(x.to(dtype).to(cuda), None, 6, scoring=scoring, **kw)
+
+
+@pytest.mark.gpu
+def test_calls_of_two_threads(cuda):
+    """Two host threads, each on its own stream, get what one gets."""
+    g = torch.Generator().manual_seed(8)
+    E, H, I, T, K = 16, 256, 128, 500, 4
+    raw, parts, _ = packed(g, E, H, I)
+    w = layout.int8_experts(*on(cuda, *parts)[0])
+    xs = [torch.randn(T, H, generator=g).to(torch.bfloat16).to(cuda) for _ in range(2)]
+    gate = torch.randn(E, H, generator=g).to(cuda)
+    bias = (torch.randn(E, generator=g) * 0.05).to(cuda)
+
+    def block(x):
+        n = ops.add_rmsnorm(x, torch.ones(H, device=cuda), 1e-6, residual=x, quant="int8")
+        r = ops.route_grouped(n.out.float() @ gate.t(), bias, K, n_group=4, topk_group=2)
+        return experts.layer_forward(w, n.out, r.indices, r.scores, num_experts=E, expert_begin=0,
+                                     numerics="efficient", rows=n.rows), r.counts
+
+    want = [block(x) for x in xs]
+    torch.cuda.synchronize()
+    got = [[], []]
+
+    def work(i):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            for _ in range(20):
+                got[i].append(block(xs[i]))
+        s.synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(120)
+    for i in range(2):
+        assert len(got[i]) == 20
+        for y, c in got[i]:
+            assert torch.equal(y, want[i][0]) and torch.equal(c, want[i][1])
+
+
+@pytest.mark.gpu
+def test_captured_long_batches(cuda):
+    """Routing (whose counts a second kernel zeroes), the quantiser and the
+    products of a long batch, replayed on new inputs."""
+    g = torch.Generator().manual_seed(2)
+    T, E, K = 3000, 64, 6
+    logits = [torch.randn(T, E, generator=g).to(cuda) for _ in range(3)]
+    lin = layout.int8_linear(*layout.quantize_int8(torch.randn(520, 328, generator=g).to(cuda)))
+    xs = [torch.randn(T, 328, generator=g).to(torch.bfloat16).to(cuda) for _ in range(3)]
+
+    def step(a, x):
+        r = ops.route_grouped(a, None, K, n_group=8, topk_group=3, scoring="softmax")
+        return r.indices, r.scores, r.counts, experts.int8_linear(lin, x)
+
+    want = [step(a, x) for a, x in zip(logits, xs)]
+    a, x = logits[0].clone(), xs[0].clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(a, x)
+    for i in (1, 2, 0, 0):
+        a.copy_(logits[i])
+        x.copy_(xs[i])
+        graph.replay()
+        torch.cuda.synchronize()
+        for o, w in zip(out, want[i]):
+            assert torch.equal(o, w)
+    idx, _, counts = plain(logits[1].cpu(), None, K, 8, 3, 2, "softmax", True, 1.0)
+    assert torch.equal(want[1][0].cpu(), idx) and torch.equal(want[1][2].cpu().long(), counts)
+
+
+@pytest.mark.gpu
+def test_many_tiles_of_pairs(cuda):
+    """256-row tiles: odd numbers of feature tiles, chunks of all sizes and more
+    tiles than CTA pairs."""
+    from tests.test_int8 import run_gemm
+    g = torch.Generator().manual_seed(12)
+    for planes, F, K in ((1, 1160, 136), (2, 456, 136), (1, 264, 1112)):
+        run_gemm(cuda, g, [1, 31, 32, 33, 255, 256, 257, 0, 511, 700], planes, F, K, 256)
+    run_gemm(cuda, g, [260] * 60, 1, 640, 256, 256, row_w=torch.float32)
+    assert _lib.device_status(0) == 0
+
+
+def test_packed_weights_copy_and_pickle():
+    g = torch.Generator().manual_seed(3)
+    _, parts, _ = packed(g, 2, 64, 16)
+    w = layout.int8_experts(*parts)
+    for other in (copy.deepcopy(w), pickle.loads(pickle.dumps(w))):
+        for m, o in ((w.m1, other.m1), (w.m2, other.m2)):
+            assert torch.equal(m.weight, o.weight) and torch.equal(m.scale, o.scale) and o.bias is None
+            assert m.weight.data_ptr() != o.weight.data_ptr()
+            assert (m.n_experts, m.planes, m.n_feat, m.k_valid, m.feat_pad, m.k_pad, m.epilogue) == (
+                o.n_experts, o.planes, o.n_feat, o.k_valid, o.feat_pad, o.k_pad, o.epilogue)
+    r = pickle.loads(pickle.dumps(ops.QuantRows(torch.zeros(2, 128, dtype=torch.int8), torch.ones(2))))
+    assert r.q.shape == (2, 128) and r.scale.shape == (2,)
+    with pytest.raises(ValueError, match="tiles"):
+        ops.Int8Matrix(2, 2, 16, 64, 128, 128, w.w1[:1], w.s1, None, _lib.EPI_SWIGLU_F32)
+    with pytest.raises(ValueError, match="sizes"):
+        ops.Int8Matrix(2, 2, 200, 64, 128, 128, w.w1, w.s1, None, _lib.EPI_SWIGLU_F32)
+    with pytest.raises(ValueError, match="scale"):
+        ops.Int8Matrix(2, 2, 16, 64, 128, 128, w.w1, w.s1.double(), None, _lib.EPI_SWIGLU_F32)
+
+
+@pytest.mark.gpu
+def test_int8_wrapper_refusals(cuda):
+    g = torch.Generator().manual_seed(0)
+    _, parts, _ = packed(g, 2, 64, 16)
+    w = layout.int8_experts(*on(cuda, *parts)[0])
+    x = torch.zeros(6, 64, dtype=torch.bfloat16, device=cuda)
+    idx = torch.zeros(3, 2, dtype=torch.int64, device=cuda)
+    perm = ops.permute(idx, 2)
+    rows = ops.act_quant_int8(x)
+    kw = dict(offsets=perm.offsets)
+    out = torch.empty(6, 64, dtype=torch.bfloat16, device=cuda)
+    bad = [
+        lambda: ops.int8_gemm(w.m1, rows, offsets=None),                                   # two experts
+        lambda: ops.int8_gemm(w.m1, rows, offsets=perm.offsets[:2]),
+        lambda: ops.int8_gemm(w.m1, rows, offsets=perm.offsets.long()),
+        lambda: ops.int8_gemm(w.m1, rows, offsets=perm.offsets.cpu()),
+        lambda: ops.int8_gemm(w.m1, rows, expert_begin=-1, **kw),
+        lambda: ops.int8_gemm(w.m1, ops.QuantRows(rows.q.cpu(), rows.scale), **kw),
+        lambda: ops.int8_gemm(w.m1, rows, max_rows=7, **kw),
+        lambda: ops.int8_gemm(w.m1, rows, out=out[:5], **kw),
+        lambda: ops.int8_gemm(w.m1, rows, out=out[:, :8], **kw),
+        lambda: ops.int8_gemm(w.m1, rows, out=out.float(), **kw),
+        lambda: ops.int8_gemm(w.m1, rows, out=out.t(), **kw),
+        lambda: ops.int8_gemm(w.m1, rows, out=out[:, 1:], **kw),                           # not 16-byte aligned
+        lambda: ops.int8_gemm(w.m1, rows, token_tile=48, **kw),
+        lambda: ops.int8_gemm(w.m1, rows, row_weight=torch.ones(6, device=cuda), row_src=perm.perm_src, **kw),  # gated
+        lambda: ops.int8_gemm(w.m2, ops.act_quant_int8(x[:, :16], k_pad=128), row_weight=torch.ones(5, device=cuda),
+                              row_src=perm.perm_src, **kw),
+        lambda: ops.int8_gemm(w.m2, ops.act_quant_int8(x[:, :16], k_pad=128), row_weight=torch.ones(6, device=cuda), **kw),
+        lambda: ops.int8_project(w.m1, x.float(), **kw),
+        lambda: ops.int8_project(w.m1, x[:, :32], **kw),
+        lambda: ops.int8_project(w.m1, x[:, 1:], **kw),
+        lambda: ops.int8_project(w.m1, x[:3], inverse=perm.inverse, copies=3, **kw),
+        lambda: ops.int8_project(w.m1, x[:3], copies=2, **kw),
+        lambda: experts.int8_gate_up(w, x[:3, :56], perm, K=2, num_experts=2, expert_begin=0),
+        lambda: experts.int8_down(w, x[:5], perm, None, K=2, num_experts=2, expert_begin=0),
+        lambda: experts.int8_linear(w.m1, x),
+        lambda: experts.int8_swiglu(w, x),
+    ]
+    for i, f in enumerate(bad):
+        with pytest.raises(ValueError):
+            f()
+            pytest.fail(f"call {i} was accepted")
+    e = native.LocalSwiGLUExperts(torch.zeros(2, 32, 64, dtype=torch.bfloat16, device=cuda),
+                                  torch.zeros(2, 64, 16, dtype=torch.bfloat16, device=cuda), storage="int8")
+    assert e(x[:0], idx[:0, 0]).shape == (0, 64) and (e(x, idx.reshape(-1)) == 0).all()
