@@ -876,11 +876,21 @@ static int int8_gemm_launch(int device, int* sp, void* stream, const b200moe_gem
                             const float* q_scale, const float* w_scale, const float* bias, bool after_quant) {
   const bool is_gated = a->planes == 2;
   int bn = a->token_tile;
-  if (bn == 0) {
-    // 1.5x the mean rows per expert, so that one tile usually holds an expert's
-    // rows; without offsets the rows are known
-    const long long avg = a->offsets ? (3ll * a->max_rows + 2ll * a->n_experts - 1) / (2ll * a->n_experts) : a->max_rows;
-    bn = std::min(256, std::max(16, pow2_ceil(static_cast<int>(std::min(avg, 1ll << 20)))));
+  if (bn == 0 && a->offsets) {
+    // Three times the mean rows per expert (16 rows a tile take as long as 128
+    // do, a second tile of an expert its weights' copies again), up to 128; 256
+    // from a mean of 112. Gate/up of 128 experts, us at tiles 64 / 128 / 256:
+    // mean 32 68 / 68 / 69 (skewed load 75 / 70 / 69), mean 62 78 / 71 / 72,
+    // mean 128 129 / 92 / 82; their down projection: mean 32 39 / 39 / 51,
+    // mean 62 52 / 43 / 56.
+    const long long rows = a->max_rows, e = a->n_experts;
+    bn = rows >= 112 * e ? 256 : std::min(128, std::max(16, pow2_ceil(static_cast<int>((3 * rows + e - 1) / e))));
+  } else if (bn == 0) {
+    // one expert: the smallest tile whose tiles fill the SMs at most once, so
+    // that few rows still use most of them (4096 x 4096, 256 rows, us at tiles
+    // 32 / 64 / 128 / 256: 22 / 14 / 15 / 19), else 256
+    const long long ft = a->feat_pad / (is_gated ? 64 : 128);
+    for (bn = a->max_rows <= 16 ? 16 : 32; bn < 256 && (a->max_rows + bn - 1) / bn * ft > g_sm_count[device];) bn *= 2;
   }
   const int feat_tiles = a->feat_pad / (is_gated ? 64 : 128);
   const long long tiles_ub = (long long)(std::min(a->n_experts, a->max_rows) + a->max_rows / bn) * feat_tiles;
@@ -911,7 +921,7 @@ static int int8_gemm_launch(int device, int* sp, void* stream, const b200moe_gem
   // CTA pairs for the largest tile, where two feature tiles share the token rows
   const long long wrows = (long long)a->n_experts * feat_tiles * p.nkb * 128;
   const bool pair = bn == 256 && feat_tiles >= 2 && wrows < 0x7fffffffll;
-  p.box = pair ? 64 : std::min(bn, 128);
+  p.box = std::min(bn, 128);
   p.early = after_quant ? 1 : 0;
   // shared memory: stages of a 16 KB weight image and bn x 128 B token rows,
   // the epilogue's scales, barriers and the tile prefix

@@ -132,10 +132,13 @@ def _local_range(w: ExpertWeights, perm: ops.Permutation, num_experts: int, expe
 
 
 def _int8_tile(rows: int, experts: int) -> int:
-    """tile_policy's tile of an int8 launch, in integers (exact sums: the tile
-    changes no result)."""
-    want = -(-3 * rows // (2 * experts))
-    return 16 if want <= 16 else min(256, 1 << (want - 1).bit_length())
+    """The token tile of an int8 launch over ``rows`` rows of ``experts``
+    experts: the library's own choice (b200moe_int8_gemm), made from the global
+    expert count (exact sums: the tile changes no result)."""
+    if rows >= 112 * experts:
+        return 256
+    want = -(-3 * rows // experts)
+    return 16 if want <= 16 else min(128, 1 << (want - 1).bit_length())
 
 
 def int8_gate_up(w: ExpertWeights, hidden: torch.Tensor | ops.QuantRows, perm: ops.Permutation, *, K: int,
