@@ -59,10 +59,10 @@ __device__ __forceinline__ unsigned long long order64(double v) {
 __device__ __forceinline__ double rcp64(double x) {
   double y;
   asm("rcp.approx.ftz.f64 %0, %1;" : "=d"(y) : "d"(x));
-  if (y == 0.0) return y;   // x is infinite (or its reciprocal subnormal)
+  double r = y;
 #pragma unroll
-  for (int i = 0; i < 3; ++i) y = fma(fma(-x, y, 1.0), y, y);
-  return y;
+  for (int i = 0; i < 3; ++i) r = fma(fma(-x, r, 1.0), r, r);
+  return y == 0.0 ? y : r;   // x is infinite (or its reciprocal subnormal)
 }
 
 // The selection of one token, in lane k < K the k-th expert, with the row's
@@ -72,8 +72,8 @@ struct Selected {
   float mx, inv;
 };
 
-// In 64 bits throughout: the lane's experts side by side, since a 64-bit chain
-// is slow (10 us when its parts ran one after another, 4 us so).
+// In 64 bits throughout: loads and exponentials of the lane's experts side by
+// side, since each is a long chain (one after another they took 10 us a token).
 template <int NL>
 __device__ __noinline__ Selected select64(const RouteParams& p, int t) {
   const int lane = threadIdx.x & 31, L = 1 << p.lsh, g = lane >> p.lsh, sub = lane & (L - 1);
@@ -85,8 +85,21 @@ __device__ __noinline__ Selected select64(const RouteParams& p, int t) {
     const int o = slot_offset(sub, L, i);
     const bool in = g < p.G && o < p.S;
     live |= in ? 1u << i : 0u;
-    x[i] = in ? load_logit(p, t, g * p.S + o) : -INFINITY;
     bias[i] = in && p.bias ? __ldg(p.bias + g * p.S + o) : 0.f;
+  }
+  // (one branch for all loads: they are then under way together)
+  const long long row = (long long)t * p.ld + g * p.S;
+  if (p.bf16) {
+#pragma unroll
+    for (int i = 0; i < NL; ++i)
+      x[i] = ((live >> i) & 1u) ? __bfloat162float(__ldg(reinterpret_cast<const __nv_bfloat16*>(p.logits) + row +
+                                                         slot_offset(sub, L, i)))
+                                : -INFINITY;
+  } else {
+#pragma unroll
+    for (int i = 0; i < NL; ++i)
+      x[i] = ((live >> i) & 1u) ? __ldg(reinterpret_cast<const float*>(p.logits) + row + slot_offset(sub, L, i))
+                                : -INFINITY;
   }
   double v[NL];
   double mx = 0, sum = 0;
@@ -99,14 +112,17 @@ __device__ __noinline__ Selected select64(const RouteParams& p, int t) {
     out.mx = top;
     mx = static_cast<double>(top);
   }
-#pragma unroll 2
+#pragma unroll
   for (int i = 0; i < NL; ++i) {
     const double a = static_cast<double>(x[i]) - mx;
-    double e = exp(p.softmax ? a : -a);
-    if (!p.softmax) e = rcp64(1.0 + e);
-    v[i] = e;
-    sum += ((live >> i) & 1u) ? e : 0.0;
+    v[i] = exp(p.softmax ? a : -a);
   }
+  if (!p.softmax) {
+#pragma unroll
+    for (int i = 0; i < NL; ++i) v[i] = rcp64(1.0 + v[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < NL; ++i) sum += ((live >> i) & 1u) ? v[i] : 0.0;
   if (p.softmax) {
 #pragma unroll
     for (int o = 16; o >= 1; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
@@ -146,7 +162,7 @@ __device__ __noinline__ Selected select64(const RouteParams& p, int t) {
     }
     const unsigned long long mine = order64(v1 + ((p.top == 2 && p.S > 1) ? v2 : 0.0));
     int rank = 0;
-#pragma unroll 4
+#pragma unroll 8
     for (int h = 0; h < p.G; ++h) {
       const unsigned long long other = __shfl_sync(kFull, mine, h << p.lsh);
       if (other > mine || (other == mine && h < g)) ++rank;
