@@ -378,8 +378,10 @@ int b200moe_w8a8_gemm(int device, void* stream, const b200moe_gemm_args* args, c
  * fp32 [b_rows]. wfmt = B200MOE_W_INT8; k_pad % 128 == 0, k_pad < 131072 (the
  * int32 sum cannot overflow); b_src, ldb, k_valid, b_map, b_div, sc_br, sc_bc
  * and the args' bias are unused (b_map and bias NULL). token_tile is 0
- * (choose) or 16, 32, 64, 128, 256. Rows past the last expert's are not
- * written. */
+ * (three times the mean rows per expert, at most 128, or 256 from a mean of
+ * 112; without offsets the smallest whose tiles fill the SMs at most once) or
+ * 16, 32, 64, 128, 256; it changes no result. Rows past the last expert's are
+ * not written. */
 int b200moe_int8_gemm(int device, void* stream, const b200moe_gemm_args* args, const void* q,
                       const float* q_scale, const float* w_scale, const float* bias);
 
