@@ -56,7 +56,7 @@ def build_ext(force: bool = False) -> Path:
         "-I", str(root / "include"), "-I", str(root / "include" / "torch" / "csrc" / "api" / "include"),
         "-I", sysconfig.get_paths()["include"], "-I", str(Path(nvcc()).parents[1] / "include"), "-I", str(INCLUDE),
         str(CSRC / "ext.cpp"), "-o", str(tmp), "-L", str(root / "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu",
-        "-ltorch_python", "-L", str(PKG), f"-l:{LIB.name}", "-Wl,-rpath,$ORIGIN"], check=True)
+        "-ltorch_cuda", "-ltorch_python", "-L", str(PKG), f"-l:{LIB.name}", "-Wl,-rpath,$ORIGIN"], check=True)
     os.replace(tmp, EXT)
     return EXT
 

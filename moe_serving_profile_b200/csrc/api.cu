@@ -55,7 +55,8 @@ void* g_permute_scratch_ptr[kMaxDevices] = {};
 
 int use_device(int device, int** status) {
   B200_CHECK(device >= 0 && device < kMaxDevices, "device %d out of range", device);
-  B200_CUDA(cudaSetDevice(device));
+  int now = -1;
+  if (cudaGetDevice(&now) != cudaSuccess || now != device) B200_CUDA(cudaSetDevice(device));
   std::lock_guard<std::mutex> lock(g_mu);
   if (g_status_ptr[device] == nullptr) {
     void* p = nullptr;
