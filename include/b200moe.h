@@ -381,7 +381,7 @@ int b200moe_w8a8_gemm(int device, void* stream, const b200moe_gemm_args* args, c
  * (three times the mean rows per expert, at most 128, or 256 from a mean of
  * 112; without offsets the smallest whose tiles fill the SMs at most once) or
  * 16, 32, 64, 128, 256; it changes no result. Rows past the last expert's are
- * not written. */
+ * not written; offsets are kept within [0, max_rows]. */
 int b200moe_int8_gemm(int device, void* stream, const b200moe_gemm_args* args, const void* q,
                       const float* q_scale, const float* w_scale, const float* bias);
 

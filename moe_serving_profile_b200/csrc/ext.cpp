@@ -155,6 +155,7 @@ QuantRows act_quant_int8(const Tensor& x, std::optional<int64_t> width, const Op
     check_int32(*inverse, device, out, "inverse");
     need(inverse->numel() == out, "inverse must have rows * copies = ", out, " elements");
   }
+  need(k_pad >= k, "k_pad must be at least ", k, ", got ", k_pad);
   const Range r = expert_range(offsets, expert_lo, expert_hi, device);
   const int n = to_int(rows, "rows"), m = to_int(out, "rows"), kv = to_int(k, "columns"), kp = to_int(k_pad, "k_pad");
   QuantRows q{empty({out, k_pad}, x, at::kChar), empty({out}, x, at::kFloat)};
@@ -282,6 +283,7 @@ struct Placement {   // where an int8 launch's rows are, and what scales them
 // the output where none is given.
 b200moe_gemm_args gemm_args(const Int8Matrix& m, Placement& p, int device, int64_t R, int64_t b_rows) {
   b200moe_gemm_args a{};
+  need(R >= 0, "max_rows must not be negative");
   if (!p.out) p.out = empty({R, m.planes == 2 ? m.feat_pad : m.n_feat}, m.weight, at::kBFloat16);
   check_rows(*p.out, device, "output");
   need(p.out->size(0) >= R && p.out->size(1) >= m.n_feat, "output must hold ", R, " rows of ", m.n_feat,

@@ -100,18 +100,21 @@ __device__ __forceinline__ uint16_t bf16_bits(float f) { return __bfloat16_as_us
 // starts[e]: the permuted row where local expert e's rows begin (without
 // offsets one expert holds all rows); prefix: exclusive prefix of the experts'
 // row chunks. By warp 0, 128 experts at a time, so that their offsets arrive
-// together. Returns the number of chunks.
+// together. Offsets are kept within the launch's rows and a segment that ends
+// before it begins is empty, so that no offset leads outside the row buffers.
+// Returns the number of chunks.
 template <int BN>
 __device__ __forceinline__ int count_chunks(const Int8Params& p, int* prefix, int* starts) {
   const int lane = threadIdx.x & 31;
   int acc = 0;
+  auto in_rows = [&](int v) { return min(max(v, 0), p.dense_rows); };
   if (lane == 0) prefix[0] = 0;
   for (int base = 0; base < p.n_experts; base += 128) {
     int at[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int e = min(base + 32 * i + lane, p.n_experts);
-      at[i] = p.offsets ? p.offsets[p.expert_begin + e] : (e ? p.dense_rows : 0);
+      at[i] = p.offsets ? in_rows(p.offsets[p.expert_begin + e]) : (e ? p.dense_rows : 0);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -119,13 +122,13 @@ __device__ __forceinline__ int count_chunks(const Int8Params& p, int* prefix, in
       if (e <= p.n_experts) starts[e] = at[i];
     }
     const int last = min(base + 128, p.n_experts);   // the next lane's start: from the next vector, or memory
-    const int end = p.offsets ? p.offsets[p.expert_begin + last] : p.dense_rows;
+    const int end = p.offsets ? in_rows(p.offsets[p.expert_begin + last]) : p.dense_rows;
     if (lane == 0) starts[last] = end;
     __syncwarp();
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int e = base + 32 * i + lane;
-      int incl = e < p.n_experts ? (starts[e + 1] - at[i] + BN - 1) / BN : 0;
+      int incl = e < p.n_experts ? (max(0, starts[e + 1] - at[i]) + BN - 1) / BN : 0;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int v = __shfl_up_sync(kFull, incl, o);

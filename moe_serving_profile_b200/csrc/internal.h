@@ -116,7 +116,7 @@ cudaError_t launch_scatter_rows_8bit(cudaStream_t st, const ScatterRowsParams& p
 // Int8 grouped GEMM (int8.cu): kernel parameters, filled by the host.
 struct Int8Params {
   const int* offsets;          // permuted-row offsets of the global experts; NULL: one expert, all dense_rows rows
-  int dense_rows;
+  int dense_rows;              // rows of the launch: the offsets' bound
   int expert_begin, n_experts;
   int gated, feat_tiles, n_feat, nkb;
   const uint8_t* wtiles;       // [n_experts][feat_tiles][nkb][128 rows x 128 bytes, swizzled]

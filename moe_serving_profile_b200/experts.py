@@ -192,7 +192,7 @@ def run_experts_int8_placed(w: ExpertWeights, x: torch.Tensor, offsets: torch.Te
                             tokens: int) -> torch.Tensor:
     """Expert outputs (no routing weight) of bf16 rows already in expert-major
     order, ``offsets`` (int32 [n_experts + 1]) their segments; rows past the
-    last segment are neither read nor written. ``tokens``: the rows expected,
+    last segment may hold anything and their outputs are not written. ``tokens``: the rows expected,
     for the token tile."""
     kw = dict(offsets=offsets, token_tile=_int8_tile(tokens, w.n_experts))
     return ops.int8_project(w.m2, ops.int8_project(w.m1, x, **kw), **kw)

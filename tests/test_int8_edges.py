@@ -231,3 +231,38 @@ def test_int8_wrapper_refusals(cuda):
     e = native.LocalSwiGLUExperts(torch.zeros(2, 32, 64, dtype=torch.bfloat16, device=cuda),
                                   torch.zeros(2, 64, 16, dtype=torch.bfloat16, device=cuda), storage="int8")
     assert e(x[:0], idx[:0, 0]).shape == (0, 64) and (e(x, idx.reshape(-1)) == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tile", [16, 256])
+@pytest.mark.parametrize("offsets", [[0, 40, 100, 260], [-7, 40, 30, 30], [70, 80, 90, 100], [0, 64, 64, 0]])
+def test_offsets_outside_the_rows(cuda, tile, offsets):
+    """Offsets are kept within the launch's rows, a segment that would end
+    before it begins is empty, and rows of no segment are left as they were."""
+    rows, K, N = 64, 256, 136
+    g = torch.Generator().manual_seed(11)
+    w = torch.randint(-127, 128, (3, N, K), generator=g, dtype=torch.int8)
+    lin = [layout.int8_linear(w[e].to(cuda), torch.ones(N, device=cuda)) for e in range(3)]
+    m = ops.Int8Matrix(3, 1, N, K, 256, K, torch.cat([l.weight for l in lin]), torch.cat([l.scale for l in lin]), None,
+                       _lib.EPI_DOWN_ONCE)
+    q = torch.randint(-127, 128, (rows, K), generator=g, dtype=torch.int8)
+    guard = torch.full((rows + 64, N), 7.0, device=cuda, dtype=torch.bfloat16)
+    ops.int8_gemm(m, ops.QuantRows(q.to(cuda), torch.ones(rows, device=cuda)), token_tile=tile, out=guard,
+                  offsets=torch.tensor(offsets, dtype=torch.int32, device=cuda))
+    want = torch.full((rows + 64, N), 7.0, dtype=torch.float64)
+    at = [min(max(o, 0), rows) for o in offsets]
+    for e in range(3):
+        for r in range(at[e], max(at[e], at[e + 1])):
+            want[r] = w[e].double() @ q[r].double()
+    # sums below 2^24 are exact in fp32; one rounding to bf16
+    assert torch.equal(guard.cpu(), want.to(torch.float32).to(torch.bfloat16))
+
+
+@pytest.mark.gpu
+def test_negative_sizes_are_refused(cuda):
+    x = torch.zeros(2, 64, dtype=torch.bfloat16, device=cuda)
+    lin = layout.int8_linear(*layout.quantize_int8(torch.randn(8, 64, device=cuda)))
+    for call in (lambda: ops.act_quant_int8(x, k_pad=-128), lambda: ops.act_quant_int8(x, k_pad=48),
+                 lambda: ops.int8_gemm(lin, ops.act_quant_int8(x), max_rows=-1)):
+        with pytest.raises(ValueError):
+            call()
