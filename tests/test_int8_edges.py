@@ -12,7 +12,7 @@ import pytest
 import torch
 
 from moe_serving_profile_b200 import _lib, experts, layout, native, ops
-from tests.test_int8 import distinct, layer64, on, packed, quant
+from tests.test_int8 import distinct, layer64, on, packed, quant, run_gemm
 from tests.test_route_grouped import check, plain
 
 
@@ -266,3 +266,14 @@ def test_negative_sizes_are_refused(cuda):
                  lambda: ops.int8_gemm(lin, ops.act_quant_int8(x), max_rows=-1)):
         with pytest.raises(ValueError):
             call()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("planes", [1, 2])
+def test_last_chunks_of_every_size(cuda, planes):
+    """Token tile 256: experts whose last chunk of rows comes in each box size,
+    with ragged ends; an odd number of feature tiles; many tiles a CTA."""
+    g = torch.Generator().manual_seed(21 + planes)
+    run_gemm(cuda, g, [0, 1, 31, 64, 65, 128, 129, 255, 256, 257, 320, 321, 385, 513, 1100, 3], planes, 136, 264, 256)
+    run_gemm(cuda, g, [300, 5, 270], planes, 264, 1000, 256, begin=2)
+    run_gemm(cuda, g, [290, 600, 40, 700, 258], planes, 4096, 128, 256)
