@@ -28,6 +28,11 @@
 // is one word: the float's bits made monotone, their low bits replaced by the
 // slot, so that a sort of the lane's keys and the search over the warp move
 // words and the winner's place is known from its word.
+//
+// Bound by instruction issue: about 680 a token, against 1 KB to read. 16384
+// tokens of 256 fp32 logits in 8 groups, K = 8: 23 us (4.2 us for one token).
+// Tokens in 64 bits where they are met, or only their candidates in 64 bits,
+// took 25 us: the hot loop's registers spill.
 #include "internal.h"
 #include "ptx.cuh"
 
