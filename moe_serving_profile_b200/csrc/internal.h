@@ -8,6 +8,24 @@
 
 namespace b200 {
 
+// Launches a kernel that may begin before the stream's previous kernel has
+// ended and waits for that itself (grid_dep_wait). Such a launch also takes
+// less host time than an ordinary one (add_rmsnorm of one row: 6.6 us a
+// call against 7.2).
+template <class... P, class... A>
+cudaError_t launch_dependent(void (*kernel)(P...), int blocks, int threads, cudaStream_t st, const A&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(blocks);
+  cfg.blockDim = dim3(threads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 // Returns a cudaError_t from the launch (cudaSuccess if enqueued).
 cudaError_t launch_router_logits(cudaStream_t st, int mode, const void* hidden, long long ldx,
                                  const void* weight, const void* bias, int T, int H, int E,
@@ -60,9 +78,10 @@ struct RouteParams {
   float* scores;
   long long* indices;
   int* counts;
+  int zeroed;                  // the launch zeroes the counts first (set by launch_route_grouped)
 };
 int route_grouped_blocks(int T, int sm_count);
-cudaError_t launch_route_grouped(cudaStream_t st, const RouteParams& p, int blocks);
+cudaError_t launch_route_grouped(cudaStream_t st, RouteParams p, int blocks);
 
 // RMS norm with residual and 8-bit output, and the 8-bit row movers (norm.cu).
 struct NormParams {

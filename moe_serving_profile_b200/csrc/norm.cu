@@ -126,7 +126,7 @@ template <int V, bool ROW8>
 __global__ void __launch_bounds__(V == 4 ? 1024 : 256) add_rmsnorm_kernel(const NormParams p) {
   __shared__ float sum_buf[32];
   __shared__ uint32_t max_buf[32];
-  grid_dep_launch();
+  grid_dep_begin();
   const long long t = blockIdx.x;
   const int nvec = p.H >> 3;
   const uint4* x = reinterpret_cast<const uint4*>(p.x + t * p.ldx);
@@ -242,7 +242,7 @@ __device__ __forceinline__ int dest_rows(const int* inverse, long long t, int c0
 template <int V>
 __global__ void __launch_bounds__(V == 4 ? 1024 : 256) act_quant_int8_kernel(const QuantInt8Params p) {
   __shared__ uint32_t max_buf[32];
-  grid_dep_launch();
+  grid_dep_begin();
   const long long t = blockIdx.x;
   const int nvec = p.k_valid >> 3, npad = p.k_pad >> 3;
   const uint4* x = reinterpret_cast<const uint4*>(p.x + t * p.ldx);
@@ -294,7 +294,7 @@ __global__ void __launch_bounds__(V == 4 ? 1024 : 256) act_quant_int8_kernel(con
 // Rows of 8-bit values with `groups` scales each, copied to their places in
 // the permuted order.
 __global__ void __launch_bounds__(128) scatter_rows_8bit_kernel(const ScatterRowsParams p) {
-  grid_dep_launch();
+  grid_dep_begin();
   const long long t = blockIdx.x;
   const int nvec = p.row_bytes >> 4;
   int lo = 0, hi = p.rows_out;
@@ -333,28 +333,24 @@ int row_threads(int nvec, int v) { return ((nvec + v - 1) / v + 31) / 32 * 32; }
 cudaError_t launch_add_rmsnorm(cudaStream_t st, const NormParams& p) {
   const int v = row_vecs(p.H >> 3), n = row_threads(p.H >> 3, v);
   if (p.quant == 2) {
-    if (v == 1) add_rmsnorm_kernel<1, true><<<p.T, n, 0, st>>>(p);
-    else if (v == 2) add_rmsnorm_kernel<2, true><<<p.T, n, 0, st>>>(p);
-    else add_rmsnorm_kernel<4, true><<<p.T, n, 0, st>>>(p);
-  } else {
-    if (v == 1) add_rmsnorm_kernel<1, false><<<p.T, n, 0, st>>>(p);
-    else if (v == 2) add_rmsnorm_kernel<2, false><<<p.T, n, 0, st>>>(p);
-    else add_rmsnorm_kernel<4, false><<<p.T, n, 0, st>>>(p);
+    if (v == 1) return launch_dependent(add_rmsnorm_kernel<1, true>, p.T, n, st, p);
+    if (v == 2) return launch_dependent(add_rmsnorm_kernel<2, true>, p.T, n, st, p);
+    return launch_dependent(add_rmsnorm_kernel<4, true>, p.T, n, st, p);
   }
-  return cudaGetLastError();
+  if (v == 1) return launch_dependent(add_rmsnorm_kernel<1, false>, p.T, n, st, p);
+  if (v == 2) return launch_dependent(add_rmsnorm_kernel<2, false>, p.T, n, st, p);
+  return launch_dependent(add_rmsnorm_kernel<4, false>, p.T, n, st, p);
 }
 
 cudaError_t launch_act_quant_int8(cudaStream_t st, const QuantInt8Params& p) {
   const int v = row_vecs(p.k_valid >> 3), n = row_threads(p.k_valid >> 3, v);
-  if (v == 1) act_quant_int8_kernel<1><<<p.rows, n, 0, st>>>(p);
-  else if (v == 2) act_quant_int8_kernel<2><<<p.rows, n, 0, st>>>(p);
-  else act_quant_int8_kernel<4><<<p.rows, n, 0, st>>>(p);
-  return cudaGetLastError();
+  if (v == 1) return launch_dependent(act_quant_int8_kernel<1>, p.rows, n, st, p);
+  if (v == 2) return launch_dependent(act_quant_int8_kernel<2>, p.rows, n, st, p);
+  return launch_dependent(act_quant_int8_kernel<4>, p.rows, n, st, p);
 }
 
 cudaError_t launch_scatter_rows_8bit(cudaStream_t st, const ScatterRowsParams& p) {
-  scatter_rows_8bit_kernel<<<p.rows, 128, 0, st>>>(p);
-  return cudaGetLastError();
+  return launch_dependent(scatter_rows_8bit_kernel, p.rows, 128, st, p);
 }
 
 }  // namespace b200

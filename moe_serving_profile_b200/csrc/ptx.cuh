@@ -511,6 +511,13 @@ B200_DEVI void grid_dep_launch() { asm volatile("griddepcontrol.launch_dependent
 // Wait until the stream's previous kernel has ended and its writes are visible
 // (at once for a launch that does not overlap it).
 B200_DEVI void grid_dep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// The beginning of a kernel whose successor may start early: in this order, so
+// that whatever the successor reads before its own wait was written before
+// this grid.
+B200_DEVI void grid_dep_begin() {
+  grid_dep_wait();
+  grid_dep_launch();
+}
 
 // ---------------------------------------------------------------- cluster
 B200_DEVI uint32_t cluster_ctarank() {

@@ -272,7 +272,7 @@ __device__ __forceinline__ Pick eval(const RouteParams& p, int t, int e, float m
 
 // Zeroes the counts; the selection may begin meanwhile.
 __global__ void __launch_bounds__(512) zero_counts_kernel(int* counts, int E) {
-  grid_dep_launch();
+  grid_dep_begin();
   if (threadIdx.x < E) counts[threadIdx.x] = 0;
 }
 
@@ -288,6 +288,7 @@ __global__ void __launch_bounds__(kThreads, NL <= 8 ? 2 : 1)
   const int lsh = p.lsh, L = 1 << lsh;
   const int g = lane >> lsh, sub = lane & (L - 1);
   const int E = p.S * p.G;
+  if (!p.zeroed) grid_dep_wait();   // zero_counts_kernel has waited for the logits
   // a block counts in shared memory (16384 tokens adding to one array in global
   // memory took 20 us longer)
   if (p.counts) {
@@ -498,11 +499,10 @@ __global__ void __launch_bounds__(kThreads, NL <= 8 ? 2 : 1)
   }
   if (p.counts) {
     __syncthreads();
-    const bool alone = gridDim.x == 1;
-    if (!alone) grid_dep_wait();   // the counts are zero
+    if (p.zeroed) grid_dep_wait();   // the counts are zero
     for (int e = threadIdx.x; e < E; e += kThreads) {
       const int n = hist[e];
-      if (alone) p.counts[e] = n;
+      if (!p.zeroed) p.counts[e] = n;   // the only block
       else if (n) atomicAdd(&p.counts[e], n);
     }
   }
@@ -515,43 +515,33 @@ int route_grouped_blocks(int T, int sm_count) {
   return all < 2 * sm_count ? all : 2 * sm_count;
 }
 
-cudaError_t launch_route_grouped(cudaStream_t st, const RouteParams& p, int blocks) {
+cudaError_t launch_route_grouped(cudaStream_t st, RouteParams p, int blocks) {
   const int L = 1 << p.lsh;
   const int per_lane = 4 * ((p.S + 4 * L - 1) / (4 * L));   // slots of a lane, in fours
   const uintptr_t item = p.bf16 ? 2 : 4;
   const bool vec = p.S % 4 == 0 && p.ld % 4 == 0 && reinterpret_cast<uintptr_t>(p.logits) % (4 * item) == 0;
   const bool logit = p.bf16 && p.bias == nullptr && (p.keep == p.G || p.top == 1 || p.S == 1);
   const bool full = vec && p.S == per_lane * L && p.G * L == 32;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(blocks);
-  cfg.blockDim = dim3(kThreads);
-  cfg.stream = st;
-  cudaLaunchAttribute attr = {};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  if (blocks > 1 && p.counts) {
-    zero_counts_kernel<<<1, 512, 0, st>>>(p.counts, p.S * p.G);
-    cudaError_t e = cudaGetLastError();
+  p.zeroed = blocks > 1 && p.counts;
+  if (p.zeroed) {
+    cudaError_t e = launch_dependent(zero_counts_kernel, 1, 512, st, p.counts, p.S * p.G);
     if (e != cudaSuccess) return e;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
   }
-#define B200_ROUTE(NL_)                                                                             \
-  do {                                                                                              \
-    if (logit) {                                                                                    \
-      if (full && per_lane == NL_) return cudaLaunchKernelEx(&cfg, route_grouped_kernel<NL_, 2, true>, p); \
-      if (vec) return cudaLaunchKernelEx(&cfg, route_grouped_kernel<NL_, 1, true>, p);              \
-      return cudaLaunchKernelEx(&cfg, route_grouped_kernel<NL_, 0, true>, p);                       \
-    }                                                                                               \
-    if (full && per_lane == NL_) return cudaLaunchKernelEx(&cfg, route_grouped_kernel<NL_, 2, false>, p);  \
-    if (vec) return cudaLaunchKernelEx(&cfg, route_grouped_kernel<NL_, 1, false>, p);               \
-    return cudaLaunchKernelEx(&cfg, route_grouped_kernel<NL_, 0, false>, p);                        \
+#define B200_ROUTE_MODE(NL_, MODE_)                                                                        \
+  return logit ? launch_dependent(route_grouped_kernel<NL_, MODE_, true>, blocks, kThreads, st, p)        \
+               : launch_dependent(route_grouped_kernel<NL_, MODE_, false>, blocks, kThreads, st, p)
+#define B200_ROUTE(NL_)                                    \
+  do {                                                     \
+    if (full && per_lane == NL_) B200_ROUTE_MODE(NL_, 2);  \
+    if (vec) B200_ROUTE_MODE(NL_, 1);                      \
+    B200_ROUTE_MODE(NL_, 0);                               \
   } while (0)
   if (per_lane <= 4) B200_ROUTE(4);
   if (per_lane <= 8) B200_ROUTE(8);
   if (per_lane <= 16) B200_ROUTE(16);
   B200_ROUTE(32);
 #undef B200_ROUTE
+#undef B200_ROUTE_MODE
 }
 
 }  // namespace b200

@@ -277,3 +277,51 @@ def test_last_chunks_of_every_size(cuda, planes):
     run_gemm(cuda, g, [0, 1, 31, 64, 65, 128, 129, 255, 256, 257, 320, 321, 385, 513, 1100, 3], planes, 136, 264, 256)
     run_gemm(cuda, g, [300, 5, 270], planes, 264, 1000, 256, begin=2)
     run_gemm(cuda, g, [290, 600, 40, 700, 258], planes, 4096, 128, 256)
+
+
+@pytest.mark.gpu
+def test_calls_back_to_back(cuda):
+    """Kernels that begin before their predecessor ends read nothing too early:
+    buffers rewritten between calls, with and without a wait after every call,
+    and captured."""
+    g = torch.Generator().manual_seed(31)
+    E, K, H, I, T, n = 16, 4, 512, 256, 200, 24
+    _, parts, _ = packed(g, E, H, I)
+    w = layout.int8_experts(*on(cuda, *parts)[0])
+    weight = torch.rand(H, generator=g).to(torch.bfloat16).to(cuda)
+    xs = torch.randn(n, T, H, generator=g).to(torch.bfloat16).to(cuda)
+    ls = torch.randn(n, T, E, generator=g).to(cuda)
+    few = torch.arange(T, device=cuda)[None] < (torch.arange(n, device=cuda) % 3 * 90 + 9)[:, None]
+    xs *= few[:, :, None]
+    x, logits, res = torch.empty_like(xs[0]), torch.empty_like(ls[0]), torch.zeros_like(xs[0])
+    out = torch.empty_like(xs)
+
+    def run(wait):
+        res.zero_()
+        for i in range(n):
+            x.copy_(xs[i])
+            logits.copy_(ls[i])
+            for rows in (T, 10):   # two launches of the router, and one
+                r = ops.route_grouped(logits[:rows], None, K, n_group=4, topk_group=2)
+                wait()
+                norm = ops.add_rmsnorm(x[:rows], weight, 1e-6, residual=res[:rows], residual_out=res[:rows], quant="int8")
+                wait()
+                y = experts.layer_forward(w, norm.out, r.indices, r.scores, num_experts=E, expert_begin=0,
+                                          numerics="efficient", rows=norm.rows)
+                wait()
+                y = y + experts.layer_forward(w, norm.out, r.indices, r.scores, num_experts=E, expert_begin=0,
+                                              numerics="efficient")
+                out[i, :rows] = y
+            wait()
+        return out.clone()
+
+    want = run(torch.cuda.synchronize)
+    got = run(lambda: None)
+    assert torch.equal(got, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run(lambda: None)
+    for _ in range(2):
+        out.zero_()
+        graph.replay()
+        assert torch.equal(out, want)
