@@ -18,9 +18,11 @@
 // a thousand tokens of random logits. bf16 logits tie often; without a bias and
 // without sums of two keys their order is that of the scores, so they are the
 // keys (LOGIT), in words that hold them and the expert exactly, and nothing is
-// put aside but scores that 64 bits round together (sigmoid of logits above
-// 16, exponentials below e^-600). 4001 tokens, 160 experts: 18 us with scores
-// as keys, one token in ten put aside.
+// put aside but what 64 bits may round together: sigmoid of logits above 16,
+// exponentials below e^-600, and rows that hold a logit other than zero below
+// 2^-30 (of its size, the scores of 0 and 1e-20 are one number, and the lower
+// id comes first). 4001 tokens, 160 experts: 18 us with scores as keys, one
+// token in ten put aside.
 //
 // One warp per token. Each group has L = 32 / P lanes, P the power of two >= G;
 // lane `sub` of a group holds its experts 4 (sub + L j) .. + 3, j = 0, 1, ...,
@@ -370,9 +372,15 @@ __global__ void __launch_bounds__(kThreads, NL <= 8 ? 2 : 1)
       constexpr float kLog2e = 1.44269504f;
       float mx = 0.f, inv = 1.f, total = 0.f;
       uint32_t key[NL];
+      // Neighbouring bf16 logits a > b differ by 2^-8 |a| or more. From |a| =
+      // 2^-30 on that is 2^-40 of a sigmoid (slope 1/4), 2^-38 of an exponential,
+      // where 64 bits are off by 2^-51 and (600 + 4) 2^-53. Zeros tie exactly.
+      constexpr uint32_t kTiny = 2u * 0x30800000u - 1u;   // 2^-30
+      uint32_t least = 0xffffffffu;   // twice the least nonzero magnitude's bits, less one
       if (LOGIT) {
 #pragma unroll
         for (int i = 0; i < NL; ++i) {
+          least = min(least, 2u * __float_as_uint(x[i]) - 1u);
           const uint32_t tag = 0xffffu - (g * p.S + slot_offset(sub, L, i));   // equal logits: the lower id first
           total += x[i];
           key[i] = FULL || ((live >> (VEC ? i & ~3 : i)) & 1u) ? (order32(x[i] + 0.f) & 0xffff0000u) | tag : 0u;   // -0 is 0
@@ -406,9 +414,10 @@ __global__ void __launch_bounds__(kThreads, NL <= 8 ? 2 : 1)
           key[i] = FULL || ((live >> (VEC ? i & ~3 : i)) & 1u) ? (order32(k) & ~kSlots) | (kSlots - i) : 0u;
         }
       }
-      bool sure = !__any_sync(kFull, total != total);   // no NaN key (nor infinite ones of both signs)
+      // no NaN key (nor infinite ones of both signs), no tiny logit
+      bool sure = !__any_sync(kFull, total != total || (LOGIT && least < kTiny));
       sort_desc(key);
-      // whether 64 bits tell the score of logit a (less the largest, softmax) from those of smaller ones
+      // whether 64 bits tell the score of logit a (less the largest, softmax; not tiny) from those of smaller ones
       auto apart = [&](float a) { return a > -600.f && (p.softmax || a <= 16.f); };
 
       // ---- groups. A key is off by at most 2^-20 of the row's largest score

@@ -1,0 +1,40 @@
+"""Grouped routing where 64-bit scores meet: logits whose scores are one number
+in 64 bits go by id, others by score, whatever the logits' type."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from tests.test_route_grouped import check
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scoring", ["sigmoid", "softmax"])
+def test_tiny_logits(cuda, scoring):
+    """Around zero: 1e-20 and 0 have one score (0.5, or that of the row's
+    largest), 2^-29 and the numbers beside it have their own."""
+    step = 2.0 ** -29 * (1 + 2.0 ** -7)
+    rows = [
+        [0.0, 1e-20, -1.0, 2e-20, -1e-30, -2.0, 1e-38, -0.0],
+        [1e-20, 2e-20, 1.0, -1e-20, 0.0, -1.0, 0.5, 3e-20],
+        [-1e-20, 0.0, 300.0, 2e-20, 1e-25, -1.0, 5.0, 0.0],
+        [2.0 ** -29, step, -step, 0.0, -2.0 ** -29, 2.0 ** -28, -0.0, -2.0 ** -28],
+        [-3.0, -2.0, -1.0, 2e-20, 1e-20, 0.0, -1e-20, -4.0],
+        [0.0] * 8,
+        [1e-39, 9e-41, 0.0, -9e-41, -1e-39, 2e-39, 1e-45, -2e-39],
+    ]
+    x = torch.tensor(rows)
+    x = torch.cat([x, x.roll(3, 1), x.flip(1)]).to(cuda)
+    for dtype in (torch.bfloat16, torch.float32):
+        for kw in (dict(), dict(n_group=4, topk_group=2, group_top=1), dict(n_group=8, topk_group=5, group_top=2)):
+            for K in (1, 3, 4):
+                check(x.to(dtype), None, K, scoring=scoring, **kw)
+                check(x.to(dtype), torch.zeros(8, device=cuda), K, scoring=scoring, **kw)
+    # among many experts: the tiny one is in no lane's or group's best place
+    g = torch.Generator().manual_seed(4)
+    wide = -torch.rand(40, 160, generator=g) - 0.5
+    wide[:, 7::20], wide[:, 11::20] = 1e-20, 0.0
+    wide[::2, 31] = 3e-20
+    for kw in (dict(), dict(n_group=8, topk_group=3, group_top=1)):
+        check(wide.to(torch.bfloat16).to(cuda), None, 6, scoring=scoring, **kw)
