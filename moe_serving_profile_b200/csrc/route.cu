@@ -61,14 +61,15 @@ __device__ __forceinline__ unsigned long long order64(double v) {
   return b < 0 ? ~static_cast<unsigned long long>(b) : (static_cast<unsigned long long>(b) | (1ull << 63));
 }
 
-// 1 / x for x >= 1: the hardware's estimate and Newton's iteration.
+// 1 / x for x >= 1: the hardware's estimate and Newton's iteration; a division
+// where the estimate is zero (x infinite, or its reciprocal subnormal).
 __device__ __forceinline__ double rcp64(double x) {
   double y;
   asm("rcp.approx.ftz.f64 %0, %1;" : "=d"(y) : "d"(x));
   double r = y;
 #pragma unroll
   for (int i = 0; i < 3; ++i) r = fma(fma(-x, r, 1.0), r, r);
-  return y == 0.0 ? y : r;   // x is infinite (or its reciprocal subnormal)
+  return y == 0.0 ? 1.0 / x : r;
 }
 
 // The selection of one token, in lane k < K the k-th expert, with the row's

@@ -38,3 +38,17 @@ def test_tiny_logits(cuda, scoring):
     wide[::2, 31] = 3e-20
     for kw in (dict(), dict(n_group=8, topk_group=3, group_top=1)):
         check(wide.to(torch.bfloat16).to(cuda), None, 6, scoring=scoring, **kw)
+
+
+@pytest.mark.gpu
+def test_subnormal_scores(cuda):
+    """Sigmoids between the smallest subnormal and the smallest normal 64-bit
+    number (logits of -708.4 to -709.7) still order their experts; below them
+    the formula's exp overflows and the scores are zero."""
+    x = torch.tensor([[-709.5, -709.0, -708.75, -709.25, -710.0, -711.0, -708.0, -707.0],
+                      [-720.0, -709.75, -709.5, -708.5, -800.0, -708.5, -900.0, -709.0]]).to(cuda)
+    for kw in (dict(), dict(n_group=4, topk_group=2, group_top=1), dict(n_group=4, topk_group=3, group_top=2)):
+        for K in (1, 3, 4):
+            check(x, None, K, **kw)
+            check(x, torch.zeros(8, device=cuda), K, **kw)
+    check(x, None, 8)
