@@ -11,7 +11,7 @@
 // NaN keys and sums rank above every number.
 //
 // The selection is the one of the formula in 64-bit arithmetic. It is made in
-// fp32 with a bound on every key's error. A token whose order that bound does
+// fp32 with a bound on every key's error (own_units). A token whose order that bound does
 // not settle (two neighbours of the selection, the last selected and the first
 // left out, the last kept and the first dropped group), or that has a NaN key,
 // is put aside and selected in 64 bits when its warp is through: about two of
@@ -254,9 +254,25 @@ __device__ __forceinline__ void sort_desc(uint32_t (&k)[N]) {
           }
 }
 
+// Error bounds of the fp32 keys, in units of 2^-23 (a rounding is half a unit
+// of its result; ex2.approx and expf are off by 2 at most, rcp.approx by 1).
+//   softmax  Shared by the row's scores, through the reciprocal of their sum:
+//            additions, at most 11 one after the other (a lane's slots in
+//            fours, the fours in pairs, 5 steps over the warp) 5.5; ex2 2; its
+//            argument (l - max) log2 e, two roundings and the constant's, 1.12
+//            |l - max| in a term, 4.4 in the sum (the mean of |l - max| under
+//            the scores is below 3.9 up to 512 experts); the quotient 0.5:
+//            12.4. (One after the other, 31 additions of a lane had taken the
+//            sum 13.5 units off.) A score of its own: by expf 2, its rounded
+//            argument |l - max| / 2 and the product 0.5; by ex2 2.5 and 1.12
+//            |l - max|, which is 0.42 of the row's largest score at most.
+//   sigmoid  expf 2, sum 0.5, quotient 1; by ex2 2.2 of the score 1.
+// Above them second-order terms. The sum with the bias adds half a unit of the
+// key, and so does each sum or difference made of keys and bounds below.
+__device__ __forceinline__ float own_units(bool softmax) { return softmax ? 16.f : 8.f; }
+
 // An expert's full-precision values, and a bound on its key's distance from
-// the formula's: expf (2 units of 2^-23; softmax: its rounded argument as
-// well), sum and quotient, and the sum with the bias.
+// the formula's.
 struct Pick {
   float x, b, s, key, err;
 };
@@ -269,7 +285,7 @@ __device__ __forceinline__ Pick eval(const RouteParams& p, int t, int e, float m
   r.s = p.softmax ? expf(a) * inv : rcp(1.f + expf(-a));
   r.key = r.s + r.b;
   // below -104 the exp is zero, and so is the first term (-inf as well)
-  r.err = (r.s * (8.f + (p.softmax ? fminf(-a, 128.f) : 0.f)) + fabsf(r.key)) * kUlp + 1e-37f;
+  r.err = (r.s * (own_units(p.softmax) + (p.softmax ? fminf(-a, 128.f) : 0.f)) + 2.f * fabsf(r.key)) * kUlp + 1e-37f;
   return r;
 }
 
@@ -392,12 +408,17 @@ __global__ void __launch_bounds__(kThreads, NL <= 8 ? 2 : 1)
 #pragma unroll
         for (int i = 0; i < NL; ++i) mx = fmaxf(mx, x[i]);
         mx = unorder32(__reduce_max_sync(kFull, order32(mx)));
-        float sum = 0.f;
+        float part[NL / 4];
 #pragma unroll
         for (int i = 0; i < NL; ++i) {
           x[i] = ex2((x[i] - mx) * kLog2e);   // 0 in a slot without an expert
-          sum += x[i];
+          part[i / 4] = i % 4 == 0 ? x[i] : part[i / 4] + x[i];
         }
+#pragma unroll
+        for (int n = NL / 8; n >= 1; n >>= 1)
+#pragma unroll
+          for (int i = 0; i < n; ++i) part[i] += part[i + n];
+        float sum = part[0];
 #pragma unroll
         for (int o = 16; o >= 1; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
         inv = 1.f / sum;
@@ -421,9 +442,9 @@ __global__ void __launch_bounds__(kThreads, NL <= 8 ? 2 : 1)
       // whether 64 bits tell the score of logit a (less the largest, softmax; not tiny) from those of smaller ones
       auto apart = [&](float a) { return a > -600.f && (p.softmax || a <= 16.f); };
 
-      // ---- groups. A key is off by at most 2^-20 of the row's largest score
-      // (its approximations) and at most NL units above its word; a sum's word
-      // has the group in its low bits
+      // ---- groups. A key's score is off by own_units of the row's largest
+      // (`inv` at most), and the key at most NL - 1 units above its word; a sum's
+      // word has the group in its low bits. Two sums of two keys are compared
       if (p.keep < p.G) {
         uint32_t k1 = key[0], k2 = key[1];
         for (int o = 1; o < L; o <<= 1) {
@@ -440,7 +461,7 @@ __global__ void __launch_bounds__(kThreads, NL <= 8 ? 2 : 1)
         } else if (real) {
           const float f1 = unorder32(k1 & ~kSlots);
           const float f2 = p.top == 2 && p.S > 1 ? unorder32(k2 & ~kSlots) : 0.f;
-          off = (fabsf(f1) + fabsf(f2)) * (NL * kUlp) + inv * (32.f * kUlp);
+          off = (fabsf(f1) + fabsf(f2)) * ((NL + 2) * kUlp) + inv * (4.f * own_units(p.softmax) * kUlp);
           word = (order32(f1 + f2) & ~gmask) | (gmask - g);
         }
         uint32_t low = 0xffffffffu, high = 0;   // the last kept and the first dropped sum
@@ -493,7 +514,7 @@ __global__ void __launch_bounds__(kThreads, NL <= 8 ? 2 : 1)
         const bool ordered = c.key - nk > c.err + ne || (c.x == nx && c.b == nb && sel < ni) || lane >= p.K - 1;
         // the first one left out: no key left is above its word's range
         m = __reduce_max_sync(kFull, key[0]);
-        const uint32_t high = m ? order32(unorder32(m | kSlots) + inv * (8.f * kUlp)) : 0u;
+        const uint32_t high = m ? order32(unorder32(m | kSlots) + inv * (own_units(p.softmax) * kUlp)) : 0u;
         sure = sure && ordered && (lane >= p.K || order32(c.key - c.err) > high);
       }
       if (__all_sync(kFull, sure)) write(t, sel, c.s);

@@ -52,3 +52,30 @@ def test_subnormal_scores(cuda):
             check(x, None, K, **kw)
             check(x, torch.zeros(8, device=cuda), K, **kw)
     check(x, None, 8)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("E,G", [(510, 17), (512, 1), (256, 8)])
+def test_softmax_keys_that_nearly_tie(cuda, E, G):
+    """One expert with most of the score against one whose bias brings its key
+    within a few 2^-23 of it. The row's sum of many equal terms carries an
+    error of its own in fp32 (up to 13 such units where a lane adds 30 of them
+    one after the other), which is not the two keys' but the first one's alone."""
+    unit = 2.0 ** -23
+    far = torch.cat([torch.linspace(-7.95, -7.88, 24), torch.linspace(-6.5, -4.0, 8)]).tolist()
+    for v in far:
+        x = torch.full((1, E), v)
+        x[0, 3] = 0.0
+        s = torch.softmax(x.double(), 1)[0]
+        for gap in (-6, -3, -1.5, 1.5, 3, 6):
+            bias = torch.full((E,), -10.0)
+            bias[3] = -s[3].float()
+            for other in (1, E - 2):           # in the same group and in another
+                b = bias.clone()
+                b[other] = (s[3] + bias[3].double() - s[other] + gap * unit).float()
+                key = s + b.double()
+                assert (key[other] > key[3]) == (gap > 0)
+                for K in (1, 2):
+                    check(x.to(cuda), b.to(cuda), K, G, G, 1, "softmax", False)
+                if G > 1:
+                    check(x.to(cuda), b.to(cuda), 1, G, 1, 1, "softmax", False)
