@@ -248,9 +248,9 @@ __device__ void epilogue(const DecodeParams& p, const Tile& tl, const float (&ac
         if (p.epi == kEpiDownF32) {
           static_cast<float*>(p.out)[o] = a + b;
         } else {
-          float y = bf16_rn(a);
-          if (p.bias != nullptr) y = bf16_rn(y + b);
-          if (scaled) y = bf16_rn(y * in.w[nt][i]);
+          float y = bf16r(a);
+          if (p.bias != nullptr) y = bf16r(y + b);
+          if (scaled) y = bf16r(y * in.w[nt][i]);
           static_cast<__nv_bfloat16*>(p.out)[o] = __float2bfloat16_rn(y);
         }
       }

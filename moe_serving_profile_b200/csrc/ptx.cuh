@@ -579,16 +579,9 @@ B200_DEVI void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memo
 
 // ---------------------------------------------------------------- numerics
 // Round-to-nearest-even float -> bf16, returned as a float holding the bf16
-// value (exactly the value torch produces for `x.to(torch.bfloat16)`).
+// value (exactly the value torch produces for `x.to(torch.bfloat16)`, NaN
+// included, which an addition to the bits would turn into a number).
 B200_DEVI float bf16r(float x) { return __bfloat162float(__float2bfloat16_rn(x)); }
-
-// Round-to-nearest-even float -> bf16 bits with integer ops (keeps the
-// conversion pipe free; identical to cvt.rn for finite values and infinities).
-B200_DEVI uint32_t bf16_rn_bits(float f) {
-  const uint32_t u = __float_as_uint(f);
-  return (u + 0x7fffu + ((u >> 16) & 1u)) >> 16;
-}
-B200_DEVI float bf16_rn(float f) { return __uint_as_float(bf16_rn_bits(f) << 16); }
 
 B200_DEVI uint32_t pack_bf16x2(float lo, float hi) {
   __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);

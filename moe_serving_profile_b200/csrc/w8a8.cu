@@ -128,8 +128,8 @@ __device__ __forceinline__ Tile decode_tile(int t, const int* prefix, const W8A8
 }
 
 __device__ __forceinline__ float swiglu_bf16(float g, float u) {
-  const float gb = bf16_rn(g), ub = bf16_rn(u);
-  return bf16_rn(bf16_rn(gb / (1.f + expf(-gb))) * ub);
+  const float gb = bf16r(g), ub = bf16r(u);
+  return bf16r(bf16r(gb / (1.f + expf(-gb))) * ub);
 }
 
 // Promotion scales of one 128-column group, staged per thread through a
@@ -367,7 +367,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (half == 1) {
 #pragma unroll
           for (int n = 0; n < CB; ++n)
-            ux16[(n0 + n) * 64 + (r - 64)] = static_cast<uint16_t>(__float_as_uint(bf16_rn(tot[n])) >> 16);
+            ux16[(n0 + n) * 64 + (r - 64)] = static_cast<uint16_t>(__float_as_uint(bf16r(tot[n])) >> 16);
         }
         named_bar_sync(1, kEpi);
         if (half == 0 && tl.ft * 64 + r < p.n_feat) {
@@ -387,8 +387,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int n = 0; n < CB; ++n) {
             if (n0 + n < tl.nrows) {
-              float y = bf16_rn(tot[n]);
-              if (scaled) y = bf16_rn(y * rowv[n0 + n]);
+              float y = bf16r(tot[n]);
+              if (scaled) y = bf16r(y * rowv[n0 + n]);
               out16[(long long)(tl.row0 + n0 + n) * p.ldo + tl.ft * 128 + r] =
                   static_cast<uint16_t>(__float_as_uint(y) >> 16);
             }
