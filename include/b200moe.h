@@ -140,7 +140,7 @@ int b200moe_act_quant_fp8(int device, void* stream, const void* x, long long ldx
 /* Int8 activation quantisation of the int8 experts: per bf16 row r,
  * s[r] = amax / 127 over its k_valid values (1 where that is zero) and
  * q[r][c] = x[r][c] / s[r] rounded to nearest even; 0 for k_valid <= c < k_pad.
- * A row that holds NaN or an infinity gets that as its scale.
+ * A row that holds NaN or an infinity gets NaN as its scale.
  * inverse (device int32 [rows][copies], the inverse of b200moe_permute) or
  * NULL: when given, row r is quantised once and written to each of the places
  * inverse[r][0 .. copies - 1] of the rows_out output rows (places outside
@@ -174,7 +174,8 @@ int b200moe_scatter_rows_8bit(int device, void* stream, const void* q, int row_b
  *     the rows and scales of b200moe_w8a8_gemm, from y before its rounding
  *   quant B200MOE_QUANT_INT8: scale[t] = amax / 127 over the row, q = y / scale
  *     rounded to nearest even: the rows and scales of b200moe_int8_gemm
- *   scale 1 where the quotient is zero; q = 0 for H <= c < k_pad.
+ *   scale 1 where the quotient is zero, NaN where a value of the row (of the
+ *   128 columns) is NaN or infinite; q = 0 for H <= c < k_pad.
  * x, residual, residual_out, out: bf16 rows of ldx, ldr, ldro, ldo elements
  * (multiples of 8, 16-byte aligned); weight: bf16 or fp32 [H]; H % 8 == 0,
  * H <= 32768; k_pad % 16 == 0, H <= k_pad <= 32768. */

@@ -11,8 +11,9 @@
 // act_quant_int8: the int8 part for bf16 rows, each written to its `copies`
 // places of the permuted order.
 // amax is an unsigned maximum of the magnitudes' bits, which ranks NaN above
-// infinity: a row that holds one gets a NaN or infinite scale and its products
-// come out NaN instead of plausible.
+// infinity above every number. A row (group) that holds NaN or an infinity has
+// values that no 8-bit code times a scale can stand for: its scale is NaN, and
+// all its products come out NaN instead of plausible.
 //
 // Bound by memory: one block per row holds it in registers between the passes
 // (V vectors of 8 columns per thread), all its loads issued before the first
@@ -53,15 +54,15 @@ __device__ __forceinline__ uint32_t mag_max(const float (&f)[8], uint32_t m) {
   return m;
 }
 
-// Division by one scale: s = amax / top, or 1 where that is zero (a row or
-// group of zeros, or of values so small that the quotient underflows: they
-// quantise to 0).
+// Division by one scale: s = amax / top, 1 where that is zero (a row or group
+// of zeros, or of values so small that the quotient underflows: they quantise
+// to 0), NaN where amax is not finite.
 struct Divider {
   float s, r, top;
-  bool plain;   // magnitudes at which the remainder steps could underflow, infinity and NaN
+  bool plain;   // magnitudes at which the remainder steps could underflow, and NaN
   __device__ __forceinline__ Divider(uint32_t amax, float top_) : top(top_) {
     s = __fdiv_rn(__uint_as_float(amax), top);
-    s = s == 0.f ? 1.f : s;
+    s = amax >= 0x7f800000u ? __uint_as_float(0x7fffffffu) : s == 0.f ? 1.f : s;
     r = __frcp_rn(s);
     plain = !(s > 0x1p-80f && s < 0x1p125f);
   }
