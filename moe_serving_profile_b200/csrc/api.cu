@@ -55,8 +55,10 @@ void* g_permute_scratch_ptr[kMaxDevices] = {};
 
 int use_device(int device, int** status) {
   B200_CHECK(device >= 0 && device < kMaxDevices, "device %d out of range", device);
-  int now = -1;
-  if (cudaGetDevice(&now) != cudaSuccess || now != device) B200_CUDA(cudaSetDevice(device));
+  // also where it is the current one already: in a host thread's first call only
+  // this makes the device's context current, which the tensor maps' encoding (a
+  // driver call) needs; it takes 0.05 us
+  B200_CUDA(cudaSetDevice(device));
   std::lock_guard<std::mutex> lock(g_mu);
   if (g_status_ptr[device] == nullptr) {
     void* p = nullptr;
