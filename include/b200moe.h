@@ -390,7 +390,10 @@ int b200moe_int8_gemm(int device, void* stream, const b200moe_gemm_args* args, c
  * x holds `rows` bf16 rows of ldx elements whose k_valid columns are quantised
  * to args->k_pad columns, row r to its `copies` places inverse[r][..] of the
  * args->b_rows permuted rows (inverse NULL: to r), of the launch's experts
- * only. The GEMM's first weight tiles load while the rows are quantised.
+ * only. The GEMM's first weight tiles load while the rows are quantised. A
+ * dense launch (offsets NULL) needs rows * copies >= max_rows; without inverse
+ * offsets are kept within [0, min(max_rows, rows)], and with it every row of a
+ * segment has to be a place of inverse.
  * workspace: b200moe_int8_project_workspace(args->b_rows, args->k_pad) bytes of
  * device memory the call may overwrite, 256-byte aligned; it must not be in
  * use by another call that may run at the same time. */

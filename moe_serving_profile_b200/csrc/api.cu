@@ -1027,6 +1027,13 @@ int b200moe_int8_project(int device, void* stream, const b200moe_gemm_args* a, c
   b200::QuantInt8Params p{};
   rc = act_quant_int8_params(p, x, ldx, rows, k_valid, a->k_pad, inverse, copies, a->b_rows);
   if (rc) return rc;
+  // every row that the GEMM reads is one that x gives: all max_rows of a dense
+  // launch, those up to `rows` of segments that x's rows lie in themselves
+  B200_CHECK(a->offsets || (long long)rows * copies >= a->max_rows, "%d rows of x (%d copies) for %d dense rows", rows,
+             copies, a->max_rows);
+  b200moe_gemm_args given = *a;
+  if (a->offsets && !inverse) given.max_rows = std::min(a->max_rows, rows);
+  if (given.max_rows == 0) return B200MOE_OK;
   B200_CHECK(workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0 &&
                  workspace_bytes >= b200moe_int8_project_workspace(a->b_rows, a->k_pad),
              "workspace must be 256-byte aligned and hold %zu bytes (got %zu)",
@@ -1043,7 +1050,7 @@ int b200moe_int8_project(int device, void* stream, const b200moe_gemm_args* a, c
   rc = use_device(device, &sp);
   if (rc) return rc;
   if (rows > 0) B200_CUDA(b200::launch_act_quant_int8(static_cast<cudaStream_t>(stream), p));
-  return int8_gemm_launch(device, sp, stream, a, p.q, p.scale, w_scale, bias, rows > 0);
+  return int8_gemm_launch(device, sp, stream, &given, p.q, p.scale, w_scale, bias, rows > 0);
 }
 
 int b200moe_combine(int device, void* stream, const void* rows, long long ld_rows,
