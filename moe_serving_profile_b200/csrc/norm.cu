@@ -140,7 +140,7 @@ __global__ void __launch_bounds__(V == 4 ? 1024 : 256) add_rmsnorm_kernel(const 
     if (v < nvec) {
       h[i] = x[v];
       if (r) add[i] = r[v];
-      if (!p.weight_f32) wv[i] = __ldg(reinterpret_cast<const uint4*>(p.weight) + v);
+      if (!p.weight_f32) wv[i] = reinterpret_cast<const uint4*>(p.weight)[v];
     }
   }
   float sq = 0.f;
@@ -170,8 +170,8 @@ __global__ void __launch_bounds__(V == 4 ? 1024 : 256) add_rmsnorm_kernel(const 
     unpack8(h[i], y);
     if (p.weight_f32) {
       if (v >= nvec) return;
-      const float4 a = __ldg(reinterpret_cast<const float4*>(p.weight) + 2 * v);
-      const float4 b = __ldg(reinterpret_cast<const float4*>(p.weight) + 2 * v + 1);
+      const float4 a = reinterpret_cast<const float4*>(p.weight)[2 * v];
+      const float4 b = reinterpret_cast<const float4*>(p.weight)[2 * v + 1];
       w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
       w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
     } else {
@@ -308,7 +308,7 @@ __global__ void __launch_bounds__(128) scatter_rows_8bit_kernel(const ScatterRow
     const int dest = dest_rows(p.inverse, t, c0, p.copies, lo, hi);
     const int n = min(32, p.copies - c0);
     for (int v = threadIdx.x; v < (nvec + 31) / 32 * 32; v += blockDim.x) {   // whole warps: the copies are traded
-      const uint4 val = v < nvec ? __ldg(src + v) : make_uint4(0, 0, 0, 0);
+      const uint4 val = v < nvec ? src[v] : make_uint4(0, 0, 0, 0);
       for (int c = 0; c < n; ++c) {
         const int at = __shfl_sync(kFull, dest, c);
         if (at >= 0 && v < nvec) reinterpret_cast<uint4*>(p.out + (long long)at * p.row_bytes)[v] = val;

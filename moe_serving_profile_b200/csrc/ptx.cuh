@@ -509,7 +509,9 @@ B200_DEVI bool wait_bounded_cluster(uint64_t* bar, uint32_t parity, int* status)
 // grid_dep_wait still waits until this grid has ended.
 B200_DEVI void grid_dep_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 // Wait until the stream's previous kernel has ended and its writes are visible
-// (at once for a launch that does not overlap it).
+// (at once for a launch that does not overlap it). What it wrote is read by
+// plain loads only: the non-coherent ones (__ldg) are for memory that nothing
+// writes while this kernel lives, and its life began before that end.
 B200_DEVI void grid_dep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 // The beginning of a kernel whose successor may start early: in this order, so
 // that whatever the successor reads before its own wait was written before

@@ -92,20 +92,19 @@ __device__ __noinline__ Selected select64(const RouteParams& p, int t) {
     const int o = slot_offset(sub, L, i);
     const bool in = g < p.G && o < p.S;
     live |= in ? 1u << i : 0u;
-    bias[i] = in && p.bias ? __ldg(p.bias + g * p.S + o) : 0.f;
+    bias[i] = in && p.bias ? p.bias[g * p.S + o] : 0.f;
   }
   // (one branch for all loads: they are then under way together)
   const long long row = (long long)t * p.ld + g * p.S;
   if (p.bf16) {
 #pragma unroll
     for (int i = 0; i < NL; ++i)
-      x[i] = ((live >> i) & 1u) ? __bfloat162float(__ldg(reinterpret_cast<const __nv_bfloat16*>(p.logits) + row +
-                                                         slot_offset(sub, L, i)))
+      x[i] = ((live >> i) & 1u) ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p.logits)[row + slot_offset(sub, L, i)])
                                 : -INFINITY;
   } else {
 #pragma unroll
     for (int i = 0; i < NL; ++i)
-      x[i] = ((live >> i) & 1u) ? __ldg(reinterpret_cast<const float*>(p.logits) + row + slot_offset(sub, L, i))
+      x[i] = ((live >> i) & 1u) ? reinterpret_cast<const float*>(p.logits)[row + slot_offset(sub, L, i)]
                                 : -INFINITY;
   }
   double v[NL];
@@ -332,13 +331,13 @@ __global__ void __launch_bounds__(kThreads, NL <= 8 ? 2 : 1)
       if (VEC) {   // S % 4 == 0: the four slots of a vector are live together
         if (FULL || ((live >> i) & 1u)) {
           if (p.bf16) {
-            const uint2 v = __ldg(reinterpret_cast<const uint2*>(reinterpret_cast<const __nv_bfloat16*>(p.logits) + at));
+            const uint2 v = *reinterpret_cast<const uint2*>(reinterpret_cast<const __nv_bfloat16*>(p.logits) + at);
             x[i] = __uint_as_float(v.x << 16);
             x[i + 1] = __uint_as_float(v.x & 0xffff0000u);
             x[i + 2] = __uint_as_float(v.y << 16);
             x[i + 3] = __uint_as_float(v.y & 0xffff0000u);
           } else {
-            const float4 v = __ldg(reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p.logits) + at));
+            const float4 v = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p.logits) + at);
             x[i] = v.x;
             x[i + 1] = v.y;
             x[i + 2] = v.z;
@@ -349,8 +348,7 @@ __global__ void __launch_bounds__(kThreads, NL <= 8 ? 2 : 1)
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           if ((live >> (i + j)) & 1u)
-            x[i + j] = p.bf16 ? __bfloat162float(__ldg(reinterpret_cast<const __nv_bfloat16*>(p.logits) + at + j))
-                              : __ldg(reinterpret_cast<const float*>(p.logits) + at + j);
+            x[i + j] = load_logit(p, t, g * p.S + slot_offset(sub, L, i + j));
       }
     }
   };
