@@ -17,7 +17,13 @@ import torch
 
 from moe_serving_profile_b200 import _lib
 from moe_serving_profile_b200._lib import check, lib   # first: a missing library is its ImportError
-from moe_serving_profile_b200 import _ext
+
+try:
+    from moe_serving_profile_b200 import _ext
+except ImportError as e:   # missing, or built for another torch: the calls below that need it say so
+    from moe_serving_profile_b200._noext import NoBinding
+
+    _ext = NoBinding(e)
 
 
 def _dev(t: torch.Tensor, what: str) -> int:

@@ -1,0 +1,51 @@
+"""The torch binding where it does not load (CPU): what goes through ctypes stays
+usable, and calls that need the binding say how to build it."""
+
+from __future__ import annotations
+
+import subprocess
+import sys
+import textwrap
+
+from tests.conftest import ROOT
+
+
+def run(code: str) -> str:
+    r = subprocess.run([sys.executable, "-c", textwrap.dedent(code)], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+    return r.stdout
+
+
+def test_package_without_the_binding():
+    out = run("""
+        import sys
+        sys.modules["moe_serving_profile_b200._ext"] = None     # its import fails
+        import torch
+        from moe_serving_profile_b200 import experts, gpt_oss, layout, native, norm, ops, qwen3, router
+        w = layout.bf16_experts(*(torch.zeros(2, *s, dtype=torch.bfloat16) for s in ((16, 64), (16, 64), (64, 16))))
+        assert w.n_experts == 2
+        x = torch.zeros(4, 64, dtype=torch.bfloat16)
+        calls = [
+            lambda: ops.route_grouped(torch.zeros(4, 8), None, 2),
+            lambda: ops.act_quant_int8(x),
+            lambda: ops.add_rmsnorm(x, torch.ones(64), 1e-6),
+            lambda: norm.AddRMSNorm(64)(x),
+            lambda: ops.scatter_rows_8bit(None, None, 1),
+            lambda: ops.int8_gemm(None, None),
+            lambda: ops.int8_project(None, x),
+            lambda: ops.QuantRows(x, x),
+            lambda: layout.int8_linear(torch.zeros(8, 64, dtype=torch.int8), torch.ones(8)),
+        ]
+        for call in calls:
+            try:
+                call()
+            except ImportError as e:
+                assert "moe_serving_profile_b200.build" in str(e)
+            else:
+                raise SystemExit("accepted")
+        try:
+            ops.act_quant_fp8(x)                                # through ctypes: its own check
+        except ValueError as e:
+            print("ok", e)
+        """)
+    assert out.startswith("ok")
