@@ -40,10 +40,27 @@ def _stale() -> bool:
     return any(p.stat().st_mtime > built for p in deps)
 
 
+def ext_key() -> str:
+    """What the torch binding is built for; the binding holds its own as ``built_for``."""
+    import sysconfig
+
+    import torch
+
+    return f"torch {torch.__version__} {sysconfig.get_config_var('SOABI')}"
+
+
+def _ext_stale() -> bool:
+    if not EXT.exists():
+        return True
+    built = EXT.stat().st_mtime
+    return (any(p.stat().st_mtime > built for p in (CSRC / "ext.cpp", INCLUDE / "b200moe.h"))
+            or ext_key().encode() + b"\0" not in EXT.read_bytes())
+
+
 def build_ext(force: bool = False) -> Path:
-    """Compile the torch binding if its source or the header is newer."""
-    deps = [CSRC / "ext.cpp", INCLUDE / "b200moe.h"]
-    if not force and EXT.exists() and all(p.stat().st_mtime <= EXT.stat().st_mtime for p in deps):
+    """Compile the torch binding if its source or the header is newer, or if it
+    was built for another torch or Python."""
+    if not force and not _ext_stale():
         return EXT
     import sysconfig
 
@@ -52,7 +69,7 @@ def build_ext(force: bool = False) -> Path:
     root = Path(torch.__file__).resolve().parent
     tmp = EXT.with_suffix(".so.tmp")
     subprocess.run([
-        "g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+        "g++", "-O2", "-std=c++17", "-fPIC", "-shared", f'-DB200MOE_BUILT_FOR="{ext_key()}"', f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
         "-I", str(root / "include"), "-I", str(root / "include" / "torch" / "csrc" / "api" / "include"),
         "-I", sysconfig.get_paths()["include"], "-I", str(Path(nvcc()).parents[1] / "include"), "-I", str(INCLUDE),
         str(CSRC / "ext.cpp"), "-o", str(tmp), "-L", str(root / "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu",

@@ -372,6 +372,7 @@ Tensor int8_project(const Int8Matrix& m, const Tensor& x, const OptTensor& offse
 }  // namespace
 
 PYBIND11_MODULE(_ext, mod) {
+  mod.attr("built_for") = B200MOE_BUILT_FOR;   // the torch and Python of the build, by its command
   py::class_<QuantRows>(mod, "QuantRows",
                         "Rows in 8 bits with their scales: e4m3 ``q`` [rows, k_pad] with fp32\n``scale`` [rows, "
                         "ceil(k_pad / 128)] (W8A8 FP8 experts) or int8 ``q`` with\n``scale`` [rows] (int8 experts and "

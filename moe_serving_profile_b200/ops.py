@@ -20,6 +20,10 @@ from moe_serving_profile_b200._lib import check, lib   # first: a missing librar
 
 try:
     from moe_serving_profile_b200 import _ext
+    from moe_serving_profile_b200.build import ext_key
+
+    if getattr(_ext, "built_for", None) != ext_key():   # another torch's tensors are laid out otherwise
+        raise ImportError(f"built for {getattr(_ext, 'built_for', 'an unknown torch')}, running {ext_key()}")
 except ImportError as e:   # missing, or built for another torch: the calls below that need it say so
     from moe_serving_profile_b200._noext import NoBinding
 

@@ -49,3 +49,45 @@ def test_package_without_the_binding():
             print("ok", e)
         """)
     assert out.startswith("ok")
+
+
+def test_binding_of_another_torch_is_not_used():
+    out = run("""
+        import sys, types
+        other = types.ModuleType("moe_serving_profile_b200._ext")
+        other.built_for = "torch 1.0 cpython-30"
+        sys.modules["moe_serving_profile_b200._ext"] = other
+        import torch
+        from moe_serving_profile_b200 import ops
+        try:
+            ops.add_rmsnorm(torch.zeros(4, 64, dtype=torch.bfloat16), torch.ones(64), 1e-6)
+        except ImportError as e:
+            print(e)
+        """)
+    assert "built for torch 1.0 cpython-30" in out
+
+
+def test_binding_of_another_torch_is_rebuilt(tmp_path, monkeypatch):
+    """A torch of another version, with no file newer than the binding."""
+    from moe_serving_profile_b200 import build
+
+    assert not build._ext_stale()
+    runs = []
+
+    def compile_(cmd, check):
+        runs.append(cmd)
+        with open(cmd[cmd.index("-o") + 1], "wb") as f:
+            f.write(b"\0" + build.ext_key().encode() + b"\0")
+
+    ext = tmp_path / "_ext.so"
+    ext.write_bytes(build.EXT.read_bytes())
+    monkeypatch.setattr(build, "EXT", ext)
+    monkeypatch.setattr(build.subprocess, "run", compile_)
+    build.build_ext()
+    assert not runs                                     # the torch that it was built for
+    import torch
+    monkeypatch.setattr(torch, "__version__", torch.__version__ + ".post1")
+    build.build_ext()
+    assert len(runs) == 1 and any("post1" in a for a in runs[0])
+    build.build_ext()
+    assert len(runs) == 1
