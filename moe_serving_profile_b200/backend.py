@@ -35,12 +35,21 @@ def check_runtime(family: str, device, dtype: torch.dtype, storage: str) -> None
     _lib.version()
 
 
-def backend_metadata(family: str, numerics: str) -> dict:
-    """Labels of the kernels one layer call runs (the reference's keys)."""
+def backend_metadata(family: str, numerics: str, storage: str | None = None) -> dict:
+    """Labels of the kernels one layer call runs (the reference's keys), for
+    experts in ``storage`` (default: the checkpoints', fp8 or mxfp4)."""
     if numerics not in NUMERICS:
         raise ValueError(f"numerics must be one of {NUMERICS}, got {numerics!r}")
-    weights = "mxfp4_e2m1_ue8m0" if family == "gpt_oss" else "fp8_e4m3_block128"
-    kind = "w8a8_dynamic_act_128" if numerics == "efficient" and family == "qwen3" else "weight_only"
+    if storage is None:
+        storage = "mxfp4" if family == "gpt_oss" else "fp8"
+    elif storage not in STORAGE[family]:
+        raise ValueError(f"b200 {family} experts support storage {STORAGE[family]}, got {storage!r}")
+    if storage == "int8" and numerics != "efficient":
+        raise ValueError("int8 experts have the numerics 'efficient' only")
+    weights = {"mxfp4": "mxfp4_e2m1_ue8m0", "fp8": "fp8_e4m3_block128", "int8": "int8_channel", "bf16": "bf16"}[storage]
+    kind = {"fp8": "w8a8_dynamic_act_128", "int8": "w8a8_dynamic_act_row"}.get(storage, "weight_only")
+    if numerics != "efficient":
+        kind = "weight_only"
     return {
         "experts": f"b200_tcgen05_grouped_{weights}_{kind}",
         "router": "b200_fused_router",
