@@ -385,6 +385,9 @@ int b200moe_w8a8_gemm(int device, void* stream, const b200moe_gemm_args* args, c
  * not written; offsets are kept within [0, max_rows]. */
 int b200moe_int8_gemm(int device, void* stream, const b200moe_gemm_args* args, const void* q,
                       const float* q_scale, const float* w_scale, const float* bias);
+/* The token tile that b200moe_int8_gemm takes for token_tile 0 and offsets, over
+ * `rows` rows of `n_experts` experts (host only). */
+int b200moe_int8_token_tile(int rows, int n_experts);
 
 /* b200moe_act_quant_int8 of x and b200moe_int8_gemm on its rows, in one call:
  * x holds `rows` bf16 rows of ldx elements whose k_valid columns are quantised

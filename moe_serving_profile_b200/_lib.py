@@ -43,6 +43,7 @@ EXPORTED = (
     "b200moe_permute_noalloc",
     "b200moe_expert_gemm",
     "b200moe_w8a8_gemm",
+    "b200moe_int8_token_tile",
     "b200moe_int8_gemm",
     "b200moe_int8_project_workspace",
     "b200moe_int8_project",
@@ -196,6 +197,8 @@ def _load() -> ctypes.CDLL:
     lib.b200moe_expert_gemm.argtypes = [c_int, c_void_p, POINTER(GemmArgs)]
     lib.b200moe_w8a8_gemm.restype = c_int
     lib.b200moe_w8a8_gemm.argtypes = [c_int, c_void_p, POINTER(GemmArgs), c_void_p, c_void_p]
+    lib.b200moe_int8_token_tile.restype = c_int
+    lib.b200moe_int8_token_tile.argtypes = [c_int, c_int]
     lib.b200moe_int8_gemm.restype = c_int
     lib.b200moe_int8_gemm.argtypes = [c_int, c_void_p, POINTER(GemmArgs), c_void_p, c_void_p, c_void_p, c_void_p]
     lib.b200moe_int8_project_workspace.restype = c_size_t

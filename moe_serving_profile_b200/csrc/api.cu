@@ -843,6 +843,17 @@ int b200moe_w8a8_gemm(int device, void* stream, const b200moe_gemm_args* a, cons
   return B200MOE_OK;
 }
 
+int b200moe_int8_token_tile(int rows, int n_experts) {
+  // Three times the mean rows per expert (16 rows a tile take as long as 128
+  // do, a second tile of an expert its weights' copies again), up to 128; 256
+  // from a mean of 112. Gate/up of 128 experts, us at tiles 64 / 128 / 256:
+  // mean 32 68 / 68 / 69 (skewed load 75 / 70 / 69), mean 62 78 / 71 / 72,
+  // mean 128 129 / 92 / 82; their down projection: mean 32 39 / 39 / 51,
+  // mean 62 52 / 43 / 56.
+  const long long r = std::max(rows, 0), e = std::max(n_experts, 1);
+  return r >= 112 * e ? 256 : static_cast<int>(std::min(128, std::max(16, pow2_ceil(static_cast<int>((3 * r + e - 1) / e)))));
+}
+
 static int int8_gemm_check(const b200moe_gemm_args* a, const float* w_scale) {
   B200_CHECK(a->weight && w_scale && a->out, "weight, w_scale, out are required");
   B200_CHECK(a->offsets || (a->n_experts == 1 && a->expert_begin == 0), "more than one expert needs offsets");
@@ -880,14 +891,7 @@ static int int8_gemm_launch(int device, int* sp, void* stream, const b200moe_gem
   const bool is_gated = a->planes == 2;
   int bn = a->token_tile;
   if (bn == 0 && a->offsets) {
-    // Three times the mean rows per expert (16 rows a tile take as long as 128
-    // do, a second tile of an expert its weights' copies again), up to 128; 256
-    // from a mean of 112. Gate/up of 128 experts, us at tiles 64 / 128 / 256:
-    // mean 32 68 / 68 / 69 (skewed load 75 / 70 / 69), mean 62 78 / 71 / 72,
-    // mean 128 129 / 92 / 82; their down projection: mean 32 39 / 39 / 51,
-    // mean 62 52 / 43 / 56.
-    const long long rows = a->max_rows, e = a->n_experts;
-    bn = rows >= 112 * e ? 256 : std::min(128, std::max(16, pow2_ceil(static_cast<int>((3 * rows + e - 1) / e))));
+    bn = b200moe_int8_token_tile(a->max_rows, a->n_experts);
   } else if (bn == 0) {
     // one expert: the smallest tile whose tiles fill the SMs at most once, so
     // that few rows still use most of them (4096 x 4096, 256 rows, us at tiles

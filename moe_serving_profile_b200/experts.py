@@ -133,8 +133,9 @@ def _local_range(w: ExpertWeights, perm: ops.Permutation, num_experts: int, expe
 
 def _int8_tile(rows: int, experts: int) -> int:
     """The token tile of an int8 launch over ``rows`` rows of ``experts``
-    experts: the library's own choice (b200moe_int8_gemm), made from the global
-    expert count (exact sums: the tile changes no result)."""
+    experts: the library's own choice (b200moe_int8_token_tile, restated here
+    to save the call), made from the global expert count (exact sums: the tile
+    changes no result)."""
     if rows >= 112 * experts:
         return 256
     want = -(-3 * rows // experts)
