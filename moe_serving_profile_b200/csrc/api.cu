@@ -854,6 +854,13 @@ int b200moe_int8_token_tile(int rows, int n_experts) {
   return r >= 112 * e ? 256 : static_cast<int>(std::min(128, std::max(16, pow2_ceil(static_cast<int>((3 * r + e - 1) / e)))));
 }
 
+static int int8_feat_tiles(const b200moe_gemm_args* a) { return a->feat_pad / (a->planes == 2 ? 64 : 128); }
+
+// Tiles of ascending offsets at most.
+static long long int8_most_tiles(const b200moe_gemm_args* a, int bn) {
+  return (long long)(std::min(a->n_experts, a->max_rows) + a->max_rows / bn) * int8_feat_tiles(a);
+}
+
 static int int8_gemm_check(const b200moe_gemm_args* a, const float* w_scale) {
   B200_CHECK(a->weight && w_scale && a->out, "weight, w_scale, out are required");
   B200_CHECK(a->offsets || (a->n_experts == 1 && a->expert_begin == 0), "more than one expert needs offsets");
@@ -880,6 +887,12 @@ static int int8_gemm_check(const b200moe_gemm_args* a, const float* w_scale) {
   B200_CHECK(a->token_tile == 0 || a->token_tile == 16 || a->token_tile == 32 || a->token_tile == 64 ||
                  a->token_tile == 128 || a->token_tile == 256,
              "token_tile must be 0, 16, 32, 64, 128 or 256");
+  // the kernel counts row chunks in 32 bits; offsets that do not ascend may
+  // give every expert all rows
+  const int bn = a->token_tile ? a->token_tile : b200moe_int8_token_tile(a->max_rows, a->n_experts);
+  if (a->offsets && (a->n_experts * ((a->max_rows + (long long)bn - 1) / bn) > 0x7fffffffll ||
+                     int8_most_tiles(a, bn) > b200::kInt8MaxTiles))
+    return fail(B200MOE_ERR_UNSUPPORTED, "too many rows (%d of %d experts, token tile %d)", a->max_rows, a->n_experts, bn);
   return B200MOE_OK;
 }
 
@@ -896,12 +909,12 @@ static int int8_gemm_launch(int device, int* sp, void* stream, const b200moe_gem
     // one expert: the smallest tile whose tiles fill the SMs at most once, so
     // that few rows still use most of them (4096 x 4096, 256 rows, us at tiles
     // 32 / 64 / 128 / 256: 22 / 14 / 15 / 19), else 256
-    const long long ft = a->feat_pad / (is_gated ? 64 : 128);
+    const long long ft = int8_feat_tiles(a);
     for (bn = a->max_rows <= 16 ? 16 : 32; bn < 256 && (a->max_rows + bn - 1) / bn * ft > g_sm_count[device];) bn *= 2;
   }
-  const int feat_tiles = a->feat_pad / (is_gated ? 64 : 128);
-  const long long tiles_ub = (long long)(std::min(a->n_experts, a->max_rows) + a->max_rows / bn) * feat_tiles;
-  if (tiles_ub > 0x7fffffffll) return fail(B200MOE_ERR_UNSUPPORTED, "too many tiles");
+  const int feat_tiles = int8_feat_tiles(a);
+  const long long tiles_ub = int8_most_tiles(a, bn);
+  if (tiles_ub > b200::kInt8MaxTiles) return fail(B200MOE_ERR_UNSUPPORTED, "too many tiles");
 
   b200::Int8Params p{};
   p.offsets = a->offsets;

@@ -146,6 +146,14 @@ __device__ __forceinline__ int count_chunks(const Int8Params& p, int* prefix, in
   return acc;
 }
 
+// Tiles of a launch: none after a wait gave up. Ascending offsets give fewer
+// than kInt8MaxTiles (the host has checked); others that give more are flagged.
+__device__ __forceinline__ int tile_count(const Int8Params& p, int chunks, int feat_tiles, int gave_up) {
+  const long long n = (long long)chunks * feat_tiles;
+  if (n > kInt8MaxTiles) atomicOr(p.status, kStatusBadTile);
+  return gave_up || n > kInt8MaxTiles ? 0 : static_cast<int>(n);
+}
+
 // Columns first * 16 .. + 15, + 32 .. + 47, ... of one accumulator (this
 // warp's lanes at `acc`, NB banks of BN columns): added, scaled, gated or
 // weighted, and stored as feature f of the rows at `out`.
@@ -238,10 +246,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == 0) {
     // what the row chunks are counted from may come from the previous kernel
     if (!p.early) grid_dep_wait();
-    const int bad = *reinterpret_cast<volatile int*>(p.status) & kStatusWaitTimeout;
+    const int gave_up = *reinterpret_cast<volatile int*>(p.status) & kStatusWaitTimeout;
     const int chunks = count_chunks<BN>(p, prefix, starts);
     if (lane == 0) {
-      *s_total = bad ? 0 : chunks * p.feat_tiles;   // after a wait gave up: nothing to do
+      *s_total = tile_count(p, chunks, p.feat_tiles, gave_up);
       for (int i = 0; i < p.ns; ++i) {
         mbar_init(&full[i], 1);
         mbar_init(&empty[i], 1);
@@ -437,10 +445,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp == 0) {
     if (!p.early) grid_dep_wait();
-    const int bad = *reinterpret_cast<volatile int*>(p.status) & kStatusWaitTimeout;
+    const int gave_up = *reinterpret_cast<volatile int*>(p.status) & kStatusWaitTimeout;
     const int chunks = count_chunks<BN>(p, prefix, starts);
     if (lane == 0) {
-      *s_total = bad ? 0 : chunks * pairs;
+      *s_total = tile_count(p, chunks, pairs, gave_up);
       for (int i = 0; i < p.ns; ++i) {
         mbar_init(&full[i], 1);
         mbar_init(&empty[i], 1);

@@ -154,6 +154,7 @@ struct Int8Params {
   int early;                   // only q and qs depend on the stream's previous kernel
   uint32_t stage_bytes, x_off, bar_off, tmem_cols;
 };
+constexpr int kInt8MaxTiles = 0x7fff0000;   // a tile's number and the step to a CTA's next one fit an int
 constexpr int kInt8Threads = 352;    // weight copies, MMAs, 8 epilogue warps, token row copies
 const void* int8_kernel_ptr(int bn); // token tile 16, 32, 64, 128 or 256; else NULL
 const void* int8_pair_kernel_ptr();  // CTA pairs, token tile 256
