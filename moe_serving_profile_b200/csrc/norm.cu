@@ -56,16 +56,17 @@ __device__ __forceinline__ uint32_t mag_max(const float (&f)[8], uint32_t m) {
 
 // Division by one scale: s = amax / top, 1 where that is zero (a row or group
 // of zeros, or of values so small that the quotient underflows: they quantise
-// to 0), NaN where amax is not finite.
+// to 0). The scale that is stored is NaN where s is not finite.
 struct Divider {
   float s, r, top;
-  bool plain;   // magnitudes at which the remainder steps could underflow, and NaN
+  bool plain;   // magnitudes at which the remainder steps could underflow, infinity and NaN
   __device__ __forceinline__ Divider(uint32_t amax, float top_) : top(top_) {
     s = __fdiv_rn(__uint_as_float(amax), top);
-    s = amax >= 0x7f800000u ? __uint_as_float(0x7fffffffu) : s == 0.f ? 1.f : s;
+    s = s == 0.f ? 1.f : s;
     r = __frcp_rn(s);
     plain = !(s > 0x1p-80f && s < 0x1p125f);
   }
+  __device__ __forceinline__ float stored() const { return s < INFINITY ? s : __uint_as_float(0x7fffffffu); }
   __device__ __forceinline__ float operator()(float x) const {
     if (plain) return fminf(fmaxf(__fdiv_rn(x, s), -top), top);   // a subnormal scale may be short of amax / top
     float t = x * r;
@@ -198,7 +199,7 @@ __global__ void __launch_bounds__(V == 4 ? 1024 : 256) add_rmsnorm_kernel(const 
       const Divider d(m, 448.f);
       if (v < nvec) q[v] = pack_e4m3(y, d);
       else if (v < npad) q[v] = make_uint2(0, 0);
-      if ((v & 15) == 0 && (v >> 4) < groups) p.scale[t * groups + (v >> 4)] = d.s;
+      if ((v & 15) == 0 && (v >> 4) < groups) p.scale[t * groups + (v >> 4)] = d.stored();
     }
     if (p.quant == 0) return;
     // columns and groups past the vectors that the threads hold
@@ -221,7 +222,7 @@ __global__ void __launch_bounds__(V == 4 ? 1024 : 256) add_rmsnorm_kernel(const 
     }
   }
   const Divider d(block_max(amax, max_buf), 127.f);
-  if (threadIdx.x == 0) p.scale[t] = d.s;
+  if (threadIdx.x == 0) p.scale[t] = d.stored();
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     const int v = threadIdx.x + i * blockDim.x;
@@ -287,7 +288,7 @@ __global__ void __launch_bounds__(V == 4 ? 1024 : 256) act_quant_int8_kernel(con
         if (v < nvec) q[v] = o[i];
       }
       for (int v = nvec + threadIdx.x; v < npad; v += blockDim.x) q[v] = make_uint2(0, 0);
-      if (threadIdx.x == 0) p.scale[at] = d.s;
+      if (threadIdx.x == 0) p.scale[at] = d.stored();
     }
   }
 }
