@@ -61,17 +61,6 @@ __device__ __forceinline__ unsigned long long order64(double v) {
   return b < 0 ? ~static_cast<unsigned long long>(b) : (static_cast<unsigned long long>(b) | (1ull << 63));
 }
 
-// 1 / x for x >= 1: the hardware's estimate and Newton's iteration; a division
-// where the estimate is zero (x infinite, or its reciprocal subnormal).
-__device__ __forceinline__ double rcp64(double x) {
-  double y;
-  asm("rcp.approx.ftz.f64 %0, %1;" : "=d"(y) : "d"(x));
-  double r = y;
-#pragma unroll
-  for (int i = 0; i < 3; ++i) r = fma(fma(-x, r, 1.0), r, r);
-  return y == 0.0 ? 1.0 / x : r;
-}
-
 // The selection of one token, in lane k < K the k-th expert, with the row's
 // largest logit and the reciprocal of its softmax sum (0 and 1 with sigmoid).
 struct Selected {
@@ -125,14 +114,14 @@ __device__ __noinline__ Selected select64(const RouteParams& p, int t) {
   }
   if (!p.softmax) {
 #pragma unroll
-    for (int i = 0; i < NL; ++i) v[i] = rcp64(1.0 + v[i]);
+    for (int i = 0; i < NL; ++i) v[i] = __drcp_rn(1.0 + v[i]);
   }
 #pragma unroll
   for (int i = 0; i < NL; ++i) sum += ((live >> i) & 1u) ? v[i] : 0.0;
   if (p.softmax) {
 #pragma unroll
     for (int o = 16; o >= 1; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
-    const double inv = rcp64(sum);
+    const double inv = __drcp_rn(sum);
 #pragma unroll
     for (int i = 0; i < NL; ++i) v[i] *= inv;
     out.inv = static_cast<float>(inv);

@@ -79,3 +79,13 @@ def test_softmax_keys_that_nearly_tie(cuda, E, G):
                     check(x.to(cuda), b.to(cuda), K, G, G, 1, "softmax", False)
                 if G > 1:
                     check(x.to(cuda), b.to(cuda), 1, G, 1, 1, "softmax", False)
+
+
+@pytest.mark.gpu
+def test_sigmoids_one_step_above_a_half(cuda):
+    """1 / (1 + exp(-2.4e-16)) rounds up to the number above 0.5, correctly
+    rounded; an estimate that is one step short would tie it with 0.5."""
+    x = torch.tensor([[0.0, 2.4e-16, -1.0, 0.0, 2.4e-16, -1e-30], [-2.0, 0.0, 0.0, 2.4e-16, 1e-20, -3.0]]).to(cuda)
+    for dtype in (torch.float32, torch.bfloat16):
+        for kw in (dict(), dict(n_group=3, topk_group=2, group_top=1)):
+            check(x.to(dtype), None, 3, **kw)
