@@ -256,7 +256,8 @@ __device__ __forceinline__ void sort_desc(uint32_t (&k)[N]) {
 //            |l - max|, which is 0.42 of the row's largest score at most.
 //   sigmoid  expf 2, sum 0.5, quotient 1; by ex2 2.2 of the score 1.
 // Above them second-order terms. The sum with the bias adds half a unit of the
-// key, and so does each sum or difference made of keys and bounds below.
+// key; the bound has a whole one, which holds the other key's half where a key
+// is compared with the word of one that is left out.
 __device__ __forceinline__ float own_units(bool softmax) { return softmax ? 16.f : 8.f; }
 
 // An expert's full-precision values, and a bound on its key's distance from
@@ -273,7 +274,7 @@ __device__ __forceinline__ Pick eval(const RouteParams& p, int t, int e, float m
   r.s = p.softmax ? expf(a) * inv : rcp(1.f + expf(-a));
   r.key = r.s + r.b;
   // below -104 the exp is zero, and so is the first term (-inf as well)
-  r.err = (r.s * (own_units(p.softmax) + (p.softmax ? fminf(-a, 128.f) : 0.f)) + 2.f * fabsf(r.key)) * kUlp + 1e-37f;
+  r.err = (r.s * (own_units(p.softmax) + (p.softmax ? fminf(-a, 128.f) : 0.f)) + fabsf(r.key)) * kUlp + 1e-37f;
   return r;
 }
 
@@ -501,8 +502,8 @@ __global__ void __launch_bounds__(kThreads, NL <= 8 ? 2 : 1)
         const bool ordered = c.key - nk > c.err + ne || (c.x == nx && c.b == nb && sel < ni) || lane >= p.K - 1;
         // the first one left out: no key left is above its word's range
         m = __reduce_max_sync(kFull, key[0]);
-        const uint32_t high = m ? order32(unorder32(m | kSlots) + inv * (own_units(p.softmax) * kUlp)) : 0u;
-        sure = sure && ordered && (lane >= p.K || order32(c.key - c.err) > high);
+        const uint32_t high = m ? order32(__fadd_ru(unorder32(m | kSlots), inv * (own_units(p.softmax) * kUlp))) : 0u;
+        sure = sure && ordered && (lane >= p.K || order32(__fsub_rd(c.key, c.err)) > high);
       }
       if (__all_sync(kFull, sure)) write(t, sel, c.s);
       else aside |= 1u << turn;
