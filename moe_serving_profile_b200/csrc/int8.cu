@@ -92,7 +92,8 @@ __device__ __forceinline__ float row_weight(const Int8Params& p, int row) {
 
 // g / (1 + exp(-a g)) * u with the hardware exp2 and reciprocal: off by
 // |a g| + 8 steps of 2^-23 at most, far inside the bf16 rounding that follows.
-// Infinite exponentials give 0, NaN stays NaN.
+// Where the reciprocal would be subnormal (a g below -87.3) the result is 0,
+// which is off by less than 2^-119 |u / a|. NaN stays NaN.
 __device__ __forceinline__ float glu(float g, float u, float nlog) {   // nlog = -a log2(e)
   float e, r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * nlog));

@@ -2,7 +2,7 @@
 
 ``AddRMSNorm`` adds the attention output to the residual stream, norms the sum
 and, for experts that compute in 8 bits, returns the normed rows in their
-8-bit form as well, so that the experts do not read and quantise them again::
+8-bit form as well: the codes of the fp32 rows, before their rounding to bf16::
 
     n = norm(attn_out, residual)
     _, weights, indices = router(n.out)
