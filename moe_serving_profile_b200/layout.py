@@ -210,12 +210,13 @@ def fp8_experts(gate: torch.Tensor, gate_scale: torch.Tensor, up: torch.Tensor,
 
 def quantize_int8(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """[..., channels, K] -> int8 of the same shape and fp32 scales [...,
-    channels]: amax / 127 per channel (1 for a channel of zeros), round to
-    nearest even."""
+    channels]: amax / 127 per channel (1 for a channel of zeros, NaN for one
+    that holds NaN or an infinity, with codes 0), round to nearest even."""
     w = w.float()
     scale = w.abs().amax(dim=-1) / 127.0
-    scale = torch.where(scale > 0, scale, torch.ones_like(scale))
-    return torch.round(w / scale[..., None]).clamp_(-127, 127).to(torch.int8), scale
+    scale = torch.where(scale == 0, torch.ones_like(scale), scale)
+    scale = torch.where(scale.isfinite(), scale, torch.full_like(scale, torch.nan))
+    return torch.round(w / scale[..., None]).clamp_(-127, 127).nan_to_num_(0.0).to(torch.int8), scale
 
 
 def _int8_rows(t: torch.Tensor) -> torch.Tensor:

@@ -76,3 +76,35 @@ def test_layer_from_a_norm(cuda, quant):
         assert torch.equal(s[:, 0], n0.rows.scale[:, 0])
         assert torch.equal(n.rows.q.view(torch.uint8)[:, :128], n0.rows.q.view(torch.uint8)[:, :128])
     assert _lib.device_status(0) == 0
+
+
+def test_weights_that_are_not_finite():
+    """A channel with NaN or an infinity has the scale NaN: its products are NaN,
+    where a scale of 1 made them zero."""
+    w = torch.randn(6, 64, generator=torch.Generator().manual_seed(0)) * 0.02
+    w[1, 3], w[2, 5], w[3, 7], w[4] = float("nan"), float("inf"), float("-inf"), 0.0
+    q, s = layout.quantize_int8(w)
+    bad = torch.tensor([False, True, True, True, False, False])
+    assert s[bad].isnan().all() and s[~bad].isfinite().all() and s[4] == 1
+    assert (q[bad] == 0).all() and (q[4] == 0).all()
+    good = layout.quantize_int8(w[~bad])
+    assert torch.equal(q[~bad], good[0]) and torch.equal(s[~bad], good[1])
+    # in a layer the channel of either gate plane stays NaN
+    lin = layout.int8_linear(*layout.quantize_int8(w.repeat(4, 1)))
+    assert int(lin.scale.isnan().sum()) == 12
+
+
+@pytest.mark.gpu
+def test_products_of_weights_that_are_not_finite(cuda):
+    g = torch.Generator().manual_seed(6)
+    E, H, I, T = 2, 128, 64, 9
+    gate, up, down = ((torch.randn(E, *s, generator=g) * 0.1).to(cuda) for s in ((I, H), (I, H), (H, I)))
+    gate[0, 5, 3], up[0, 9, 1] = float("nan"), float("inf")
+    x = torch.randn(T, H, generator=g).to(torch.bfloat16).to(cuda)
+    off = torch.tensor([0, T, T], dtype=torch.int32, device=cuda)
+    for epi in (_lib.EPI_SWIGLU_F32, _lib.EPI_CLAMP_SWIGLU_F32):
+        w = layout.int8_experts_from(gate, up, down, gated_epilogue=epi)
+        act = ops.int8_project(w.m1, x, offsets=off)[:, :I]
+        bad = torch.zeros(I, dtype=torch.bool, device=cuda)
+        bad[5] = bad[9] = True
+        assert act[:, bad].isnan().all() and act[:, ~bad].isfinite().all()
