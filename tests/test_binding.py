@@ -71,7 +71,6 @@ def test_binding_of_another_torch_is_rebuilt(tmp_path, monkeypatch):
     """A torch of another version, with no file newer than the binding."""
     from moe_serving_profile_b200 import build
 
-    assert not build._ext_stale()
     runs = []
 
     def compile_(cmd, check):
@@ -80,7 +79,7 @@ def test_binding_of_another_torch_is_rebuilt(tmp_path, monkeypatch):
             f.write(b"\0" + build.ext_key().encode() + b"\0")
 
     ext = tmp_path / "_ext.so"
-    ext.write_bytes(build.EXT.read_bytes())
+    ext.write_bytes(build.EXT.read_bytes())      # newer than every source
     monkeypatch.setattr(build, "EXT", ext)
     monkeypatch.setattr(build.subprocess, "run", compile_)
     build.build_ext()
